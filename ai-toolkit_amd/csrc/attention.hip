@@ -1255,8 +1255,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(AitkAttnArgs p) {
         {
           const f32x2_t c2v = {c2, c2}, lv = {-L2, -L2}, dlv = {dl, dl};
 #pragma unroll
-          for (int r = 0; r < 16; r += 2) {  // register pairs (v_pk_fma_f32 / v_pk_add_f32 / v_pk_mul_f32): this kernel is vector-issue bound
-                                             // (profiles/r02_notes_attention_ablation.md); backward 4.29 -> 4.12 ms same-box at B = 4
+          for (int r = 0; r < 16; r += 2) {  // register pairs; built without the packed fp32 instructions (build.py) each step is two scalar ones
             f32x2_t a = {s[r], s[r + 1]};
             a = __builtin_elementwise_fma(a, c2v, lv);
             a[0] = __builtin_amdgcn_exp2f(a[0]);

@@ -68,10 +68,9 @@ __device__ __forceinline__ float wave_max(float v) {
 // of libm tanhf (~60 instructions): the GELU / dGELU GEMM epilogues were spending ~50 us per 256x256 tile round on it.
 // |error| ~1e-6 relative, far below the bf16 rounding of the stored result.
 __device__ __forceinline__ float sigmoid_fast_f(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
-// GELU(tanh) and its derivative on PAIRS (the two bf16 halves of a packed word): every fp32 step is a packed instruction (v_pk_mul_f32 /
-// v_pk_fma_f32 / v_pk_add_f32: two elements per issue slot), only v_exp_f32 and v_rcp_f32 stay per element — 3 + 2 issue slots per element for
-// the forward (was 7 + 2 with the scalar chain the compiler formed) and 5.5 + 2 for the derivative (12.5 + 2): the GELU / dGELU GEMM epilogues
-// are VALU-issue bound (profiles/r04_gemm8_tile_switch.md).  s = sigmoid(2u) = 1 / (1 + 2^(c x (1 + k1 x^2))), c = -2 k0 log2(e) folded.
+// GELU(tanh) and its derivative on PAIRS (the two bf16 halves of a packed word).  Written on two-vectors; the library is compiled without the packed fp32
+// instructions (build.py), so each step is two independent scalar ones and a training step of the headline workload costs 0.2 % more than with them (1225.8
+// against 1223.1 ms, mean of two runs of both libraries in turn on one card).  s = sigmoid(2u) = 1 / (1 + 2^(c x (1 + k1 x^2))), c = -2 k0 log2(e) folded.
 // The operation ORDER below is the definition: every user (GEMM epilogues, the lora_wgrad GELU re-evaluation, the scalar wrappers) goes
 // through these two functions, explicit fma only, so all of them produce the same bits.
 __device__ __forceinline__ f32x2_t gelu_sigmoid_2(f32x2_t x, f32x2_t x2) {
