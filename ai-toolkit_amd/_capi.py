@@ -209,12 +209,30 @@ class ShadowDesc(C.Structure):
     _fields_ = [("src_off", i64), ("d0", i64), ("d1", i64), ("d2", i64), ("rows", i32), ("cols", i32), ("kind", i32), ("aux", i32)]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("weight", vp), ("bias", vp), ("y", vp), ("ldy", i64), ("mean", vp), ("rstd", vp),
+                ("eps", C.c_float), ("rms", i32), ("w_f32", i32), ("M", i32), ("C", i32), ("_pad", i32)]
+
+
+class NormBwdArgs(C.Structure):
+    _fields_ = [("dy", vp), ("ld_dy", i64), ("x", vp), ("ldx", i64), ("weight", vp), ("mean", vp), ("rstd", vp), ("dres", vp), ("ld_dres", i64),
+                ("dx", vp), ("ld_dx", i64), ("dweight", vp), ("dbias", vp), ("partial", vp),
+                ("rms", i32), ("w_f32", i32), ("accumulate", i32), ("M", i32), ("C", i32), ("_pad", i32)]
+
+
+class AttnRelposArgs(C.Structure):
+    _fields_ = [("Q", vp), ("K", vp), ("V", vp), ("ldq", i64), ("ldk", i64), ("ldv", i64), ("O", vp), ("ldo", i64), ("LSE", vp), ("table", vp), ("key_mask", vp),
+                ("dO", vp), ("lddo", i64), ("dQ", vp), ("dK", vp), ("dV", vp), ("lddq", i64), ("lddk", i64), ("lddv", i64), ("dtable", vp), ("ws", vp),
+                ("scale", C.c_float), ("B", i32), ("H", i32), ("S", i32), ("num_buckets", i32), ("max_distance", i32), ("causal", i32), ("dtable_f32", i32),
+                ("accumulate", i32), ("_pad", i32)]
+
+
 EPI_BIAS, EPI_ACCUM, EPI_GELU, EPI_DGELU, EPI_GATE_RES, EPI_BIAS_ROW, EPI_ADD_AUX, EPI_COL_SCALE, EPI_SPLIT_SLAB, EPI_EMIT_T = 1, 2, 4, 8, 16, 32, 64, 128, 256, 512
 
 _STRUCTS = {0: GemmArgs, 1: LoraDownArgs, 2: LoraWgradArgs, 3: LnModArgs, 4: LnModBwdArgs, 5: GateBwdArgs,
             6: ColsumFinishArgs, 7: QkvPostArgs, 8: EwArgs, 9: AttnArgs, 10: GemvArgs, 11: NoisePackArgs,
             12: MseArgs, 13: AdamWArgs, 14: ShadowDesc, 15: GroupNormArgs, 16: RmsFullArgs, 17: DoraColscaleArgs, 18: DoraBwdArgs,
-            19: KronApplyArgs, 20: GroupNormBwdArgs, 21: DdpmNoiseArgs, 22: QuantRowsArgs, 23: WgradSrc2}
+            19: KronApplyArgs, 20: GroupNormBwdArgs, 21: DdpmNoiseArgs, 22: QuantRowsArgs, 23: WgradSrc2, 24: NormArgs, 25: NormBwdArgs, 26: AttnRelposArgs}
 
 
 ABI_VERSION = 12  # AITK_ABI_VERSION of include/aitk_mi355.h this mirror was written against
@@ -284,6 +302,11 @@ def lib():
     L.aitk_resample2x.argtypes = [vp, vp, i32, i32, i32, i32, i32, vp]
     L.aitk_pad_nhwc.argtypes = [vp, vp, i32, i32, i32, i32, vp]
     L.aitk_copy_heads.argtypes = [vp, i64, vp, i64, i64, i32, i32, i32, vp]
+    L.aitk_norm_bwd_workspace_bytes.restype = C.c_int64
+    L.aitk_norm_bwd_workspace_bytes.argtypes = [i32, i32, i32]
+    L.aitk_attn_relpos_bwd_workspace_bytes.restype = C.c_int64
+    L.aitk_attn_relpos_bwd_workspace_bytes.argtypes = [i32, i32, i32, i32]
+    L.aitk_attn_relpos_buckets.argtypes = [i32, i32, i32, vp]
     _lib = L
     return L
 

@@ -1,0 +1,785 @@
+// Attention of the text encoders (T5 / UMT5 / CLIP) with a learned relative position bias, forward and backward (gfx950).  64-wide heads, self-attention over S
+// positions, bf16 in / out, fp32 statistics, v_mfma_f32_32x32x16_bf16 throughout.
+//
+//   s[q][k] = scale q.k + table[bucket(k - q)][head],   p = softmax over the keys that the key mask (and, causal, k <= q) leaves,   o = p v
+//   ds = p (dp - delta),  dp = dO v^T,  delta[q] = dO[q].o[q];   dv = p^T dO,  dq = scale ds k,  dk = scale ds^T q,
+//   dtable[j][head] = sum of ds over all samples and all pairs whose bucket is j
+//
+// The bias is never formed as an [H, S, S] tensor.  It depends on k - q alone and is constant from the first distance `sat` of the last bucket on, so a workgroup keeps
+// one line of it in LDS (2 (sat + 96) + 1 floats: every distance a tile that touches the band |k - q| < sat can ask for).  A tile inside the band takes it as the START
+// VALUE of its score accumulators (four 16-byte LDS reads per 32 x 32 block and no arithmetic; the line is held four times, shifted by 0..3 entries, because a lane's
+// first index has any alignment); a tile outside adds one constant in the exponent.
+// A tile whose keys are all masked is neither loaded nor computed.  Masked keys arrive as zeros (their lane offset points outside the buffer descriptor), so that
+// infinities or NaN in them reach nothing; their scores are replaced by -inf, never added to.  A row without any key gives o = 0, lse = -inf and zero gradients.
+//
+// Tiles are [64 rows][64 columns] bf16, 128-byte rows, filled by LDS-DMA; physical 16-byte chunk = chunk ^ rkey(row).  The key makes both ways the tile is read free of bank
+// conflicts: b128 row fragments (eight row pairs meet eight different chunks) and 16-bit transpose reads (four rows x 64 bytes fill all 64 banks: bit 2 of the key is bit 1 of the row).
+#include "common.h"
+#include "aitk_args.h"
+
+namespace {
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) float lds_float;
+typedef int v4i_t __attribute__((ext_vector_type(4)));
+
+constexpr int TILE = 8192;          // bytes of a [64][64] bf16 tile
+constexpr int BAND_PAD = 96;        // a wave's 32 rows x 64 columns span 95 distances
+constexpr int MAX_HALF = 64;        // buckets of one sign
+constexpr float M_NONE = -3.0e38f;  // running maximum of a row that has met no key yet (finite: differences with it are never NaN)
+constexpr float DEFER = 8.0f;       // the accumulators are rescaled only when a row's maximum grew by more than 2^8 (p stays below 2^8: exact in fp32 sums)
+
+struct RelposArgs {
+  AitkAttnRelposArgs a;
+  int half, sat, line_p, _pad;  // buckets per sign, first distance of the last one, floats per shifted copy of the line
+  int first[MAX_HALF];          // first distance of every bucket of one sign
+  float* delta;                 // backward: [2][B][H][S]: dO.o, and lse with +inf for rows without a key
+  float* part;                  // backward: [B * row tiles][H][num_buckets] bucket sums
+};
+
+__device__ __forceinline__ int rkey(int row) { return (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
+__device__ __forceinline__ f32x16_t zero16() {
+  f32x16_t z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+__device__ __forceinline__ s16x8_t pack8r(const f32x16_t& a, int b) {
+  const uint4 u = make_uint4(pack2bf(a[b], a[b + 1]), pack2bf(a[b + 2], a[b + 3]), pack2bf(a[b + 4], a[b + 5]), pack2bf(a[b + 6], a[b + 7]));
+  return __builtin_bit_cast(s16x8_t, u);
+}
+__device__ __forceinline__ v4i_t make_srd(const void* base, long bytes) {
+  const unsigned long long a = (unsigned long long)base;
+  v4i_t r;
+  r.x = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffu));
+  r.y = __builtin_amdgcn_readfirstlane((int)(a >> 32));
+  r.z = __builtin_amdgcn_readfirstlane((int)bytes);
+  r.w = 0x00020000;
+  return r;
+}
+// LDS-DMA: 64 lanes x 16 (4) bytes to consecutive LDS addresses from per-lane buffer offsets; an offset outside the descriptor brings zeros.  No register is written.
+__device__ __forceinline__ void dma16(unsigned dst, unsigned voff, const v4i_t& srd) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(voff), "s"(srd) : "memory");
+}
+__device__ __forceinline__ void dma4(unsigned dst, unsigned voff, const v4i_t& srd) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(dst), "v"(voff), "s"(srd) : "memory");
+}
+__device__ __forceinline__ void dma_wait_all() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+// what a lane needs to read and fill tiles
+struct TileLane {
+  int rm[4];     // b128 row fragments: row l31 (+ 32: + 4096 bytes), contraction step ks
+  int tr[2][2];  // transpose reads: column block d, row half hi (contraction step kk: + 2048 bytes); rows in the order packed accumulators have
+  int row, chunk;
+  __device__ __forceinline__ void init(int lane, int wave) {
+    const int l31 = lane & 31, h = lane >> 5, i = lane & 15, gq = (lane >> 4) & 1;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) rm[ks] = l31 * 128 + (((2 * ks + h) ^ rkey(l31)) << 4);
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        const int r = 8 * hi + 4 * h + (i >> 2), c = 4 * d + 2 * gq + ((i & 3) >> 1);
+        tr[d][hi] = r * 128 + ((c ^ rkey(r)) << 4) + (i & 1) * 8;
+      }
+    row = wave * 8 + (lane >> 3);
+    chunk = (lane & 7) ^ rkey(row);
+  }
+};
+__device__ __forceinline__ s16x8_t frag_rm(const lds_char* tile, const TileLane& L, int blk, int ks) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) s16x8_t*>(tile + blk * 4096 + L.rm[ks]);
+}
+__device__ __forceinline__ s16x8_t frag_tr(const lds_char* tile, const TileLane& L, int kk, int d) {
+  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(tile + kk * 2048 + L.tr[d][0]));
+  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(tile + kk * 2048 + L.tr[d][1]));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// one 64-row tile of a [rows][64] slice: two DMAs per wave; rows whose bit of `keep` is 0 arrive as zeros
+__device__ __forceinline__ void stage(lds_char* tile, const TileLane& L, long ld, int row0, const v4i_t& srd, int wave, unsigned long long keep) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const int r = L.row + 32 * p;
+    unsigned off = (unsigned)(((row0 + r) * ld + L.chunk * 8) * 2);
+    if (~keep) off = (keep >> r) & 1 ? off : 0x80000000u;
+    dma16(__builtin_amdgcn_readfirstlane((unsigned)(size_t)tile + (wave + 4 * p) * 1024), off, srd);
+  }
+}
+
+// bucket of a distance n >= 0 within its sign
+__device__ __forceinline__ int bucket_of(const RelposArgs& r, int n) {
+  int j = 0;
+  for (int i = 1; i < r.half; ++i) j += r.first[i] <= n;
+  return j;
+}
+// bias of relative position d = key - query, divided by the softmax scale (it joins the scores before they are multiplied by it)
+__device__ __forceinline__ float bias_of(const RelposArgs& r, int d, int hd, float inv_scale) {
+  const int n = d > 0 ? (r.a.causal ? 0 : d) : -d;
+  const int j = bucket_of(r, n) + (d > 0 && !r.a.causal ? r.half : 0);
+  return bf2f(r.a.table[(long)j * r.a.H + hd]) * inv_scale;
+}
+// the four shifted copies: copy c, entry i = bias of distance sign * (i + c - E)
+__device__ __forceinline__ void build_line(lds_float* line, const RelposArgs& r, int hd, int sign) {
+  const int E = r.sat + BAND_PAD;
+  const float inv = 1.0f / r.a.scale;
+  for (int i = threadIdx.x; i < 2 * E + 1; i += 256) {
+    const float b = bias_of(r, sign * (i - E), hd, inv);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (i - c >= 0) line[c * r.line_p + i - c] = b;
+  }
+}
+// keep-bits of 64 key tiles [t0, t0 + 64) of one sample: lane t gets tile t0 + t.  `box`: 64 x 8 bytes of LDS, rewritten here; ends behind a barrier.
+__device__ __forceinline__ unsigned long long tile_masks(const AitkAttnRelposArgs& a, int b, int t0, int nt, unsigned long long* box, int lane, int wave) {
+  const int n = a.S - (t0 + lane) * 64;
+  unsigned long long m = t0 + lane >= nt || n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+  if (a.key_mask) {
+    __syncthreads();  // the previous group's readers are through
+    const uint8_t* row = a.key_mask + (long)b * a.S;
+    const int cnt = min(64, nt - t0);
+#pragma unroll 4
+    for (int t = wave; t < cnt; t += 4) {
+      const int k = (t0 + t) * 64 + lane;
+      const unsigned long long bits = __ballot(k < a.S && row[k < a.S ? k : 0] != 0);
+      if (lane == 0) box[t] = bits;
+    }
+    __syncthreads();
+    m &= lane < cnt ? box[lane] : 0ull;
+  }
+  return m;
+}
+__device__ __forceinline__ unsigned long long lane64(unsigned long long m, int t) {
+  const unsigned lo = __builtin_amdgcn_readlane((unsigned)m, t), hi = __builtin_amdgcn_readlane((unsigned)(m >> 32), t);
+  return (unsigned long long)hi << 32 | lo;
+}
+// workgroup -> (row tile, head, sample): the tiles of one (head, sample) stay on one XCD, whose L2 then holds their slices (block i runs on XCD i % 8)
+__device__ __forceinline__ void wg_coords(int ntiles, int H, int& tile, int& hd, int& b) {
+  const int n = gridDim.x, id = blockIdx.x, x = id & 7, per = n >> 3, rem = n & 7;
+  const int l = x * per + min(x, rem) + (id >> 3);
+  tile = l % ntiles;
+  hd = (l / ntiles) % H;
+  b = (l / ntiles) / H;
+}
+
+// ============================================================================================ forward
+// 4 waves x 32 query rows, key tiles of 64 in a double buffer.  S^T = K Q^T: a lane owns one query row, so the statistics are per-lane scalars and P^T feeds the next
+// product straight from the registers.
+template <bool BIAS, bool CAUSAL>
+__global__ __launch_bounds__(256, 3) void attn_relpos_fwd_kernel(RelposArgs r) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const AitkAttnRelposArgs& a = r.a;
+  lds_char* const sm = (lds_char*)smem;                                                      // 2 x (K tile, V tile)
+  unsigned long long* const box = reinterpret_cast<unsigned long long*>(smem + 4 * TILE);    // 64 tile masks
+  lds_float* const line = (lds_float*)(smem + 4 * TILE + 512);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5, S = a.S;
+  int tile_x, hd, b;
+  wg_coords((S + 127) / 128, a.H, tile_x, hd, b);
+  const int q0 = tile_x * 128 + wave * 32;
+  const bf16_t* Qb = a.Q + (long)b * S * a.ldq + hd * 64;
+  const v4i_t srdK = make_srd(a.K + (long)b * S * a.ldk + hd * 64, ((long)(S - 1) * a.ldk + 64) * 2);
+  const v4i_t srdV = make_srd(a.V + (long)b * S * a.ldv + hd * 64, ((long)(S - 1) * a.ldv + 64) * 2);
+  TileLane L;
+  L.init(lane, wave);
+  s16x8_t qf[4];
+  {
+    const bf16_t* qp = Qb + (long)min(q0 + l31, S - 1) * a.ldq + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qf[ks] = *reinterpret_cast<const s16x8_t*>(qp + 16 * ks);
+  }
+  const float c2 = a.scale * 1.4426950408889634f;
+  float far_past = 0.f, far_ahead = 0.f;  // the bias of the last bucket of either sign, in the log2 domain
+  const int E = r.sat + BAND_PAD;
+  const int ib = E + 4 * h - q0 - l31;  // line index of key 0 of this lane's first register
+  if constexpr (BIAS) {
+    build_line(line, r, hd, 1);
+    far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
+    far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
+    __syncthreads();
+  }
+  f32x16_t o[2] = {zero16(), zero16()};
+  float m_run = M_NONE, l_run = 0.f;
+  const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * 128 + 127) / 64 + 1) : (S + 63) / 64;
+  for (int t0 = 0; t0 < ntiles; t0 += 64) {
+    const unsigned long long masks = tile_masks(a, b, t0, ntiles, box, lane, wave);
+    unsigned long long todo = __ballot(masks != 0);
+    if (!todo) continue;
+    int t = __builtin_ctzll(todo), cur = 0;
+    unsigned long long keep = lane64(masks, t);
+    stage(sm, L, a.ldk, (t0 + t) * 64, srdK, wave, keep);
+    stage(sm + TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, keep);
+    dma_wait_all();
+    __syncthreads();
+    while (true) {
+      todo &= todo - 1;
+      const int tn = todo ? __builtin_ctzll(todo) : 0;
+      const unsigned long long keep_n = lane64(masks, tn);
+      if (todo) {
+        lds_char* nx = sm + (cur ^ 1) * 2 * TILE;
+        stage(nx, L, a.ldk, (t0 + tn) * 64, srdK, wave, keep_n);
+        stage(nx + TILE, L, a.ldv, (t0 + tn) * 64, srdV, wave, keep_n);
+      }
+      const lds_char* kt = sm + cur * 2 * TILE;
+      const lds_char* vt = kt + TILE;
+      const int kv0 = (t0 + t) * 64;
+      if (!CAUSAL || kv0 <= q0 + 31) {
+        float tb = 0.f;
+        bool near = false;
+        if constexpr (BIAS) {
+          near = true;
+          if (kv0 + 63 - q0 <= -r.sat) near = false, tb = far_past;
+          else if (kv0 - q0 - 31 >= r.sat) near = false, tb = far_ahead;
+        }
+        f32x16_t s[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s16x8_t kf[4];
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) kf[ks] = frag_rm(kt, L, j, ks);
+          if (BIAS && near) {
+            const int i0 = ib + kv0;
+            const lds_float* lp = line + (i0 & 3) * r.line_p + (i0 & ~3) + 32 * j;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(lp + 8 * g);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[j][4 * g + e] = v[e];
+            }
+          } else {
+            s[j] = zero16();
+          }
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) s[j] = mfma32(kf[ks], qf[ks], s[j]);
+        }
+        if (~keep) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const unsigned mj = (unsigned)(keep >> (32 * j)) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (!(mj & (1u << ((e & 3) + 8 * (e >> 2))))) s[j][e] = -INFINITY;
+          }
+        }
+        if (CAUSAL && kv0 + 63 > q0) {
+          const int lim = q0 + l31 - kv0 - 4 * h;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (32 * j + (e & 3) + 8 * (e >> 2) > lim) s[j][e] = -INFINITY;
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[j][e]);
+        mt = fmaf(fmaxf(mt, __shfl_xor(mt, 32, 64)), c2, tb);
+        if (!__all(mt - m_run <= DEFER)) {
+          const float m_new = fmaxf(m_run, mt);
+          const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+          l_run *= alpha;
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+          m_run = m_new;
+        }
+        const float sub = tb - m_run;
+        float ps = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[j][e], c2, sub));
+            s[j][e] = p;
+            ps += p;
+          }
+        l_run += ps;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const s16x8_t pf = pack8r(s[kk >> 1], 8 * (kk & 1));  // p in bf16 for the matrix unit; the row sum keeps the fp32 values
+#pragma unroll
+          for (int d = 0; d < 2; ++d) o[d] = mfma32(frag_tr(vt, L, kk, d), pf, o[d]);
+        }
+      }
+      dma_wait_all();
+      __syncthreads();
+      if (!todo) break;
+      t = tn;
+      keep = keep_n;
+      cur ^= 1;
+    }
+  }
+  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  const float inv = l_tot > 0.f ? 1.0f / l_tot : l_tot != l_tot ? l_tot : 0.f;
+  const int q = q0 + l31;
+  if (q < S) {
+    bf16_t* op = a.O + ((long)b * S + q) * a.ldo + hd * 64;
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint2 u = make_uint2(pack2bf(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), pack2bf(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+        *reinterpret_cast<uint2*>(op + 32 * d + 8 * g + 4 * h) = u;
+      }
+    if (h == 0) a.LSE[((long)b * a.H + hd) * S + q] = l_tot == 0.f ? -INFINITY : m_run + log2f(l_tot);
+  }
+}
+
+// ============================================================================================ backward
+// delta[q] = dO[q].o[q], and the row statistic with +inf for rows without a key (2^(s - inf) = 0: their probabilities vanish).  A wave takes 8 rows of one head.
+__global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
+  const AitkAttnRelposArgs& a = r.a;
+  const int s = blockIdx.x * 32 + (threadIdx.x >> 3), hd = blockIdx.y, b = blockIdx.z, c = (threadIdx.x & 7) * 8;
+  if (s >= a.S) return;
+  const long row = (long)b * a.S + s;
+  const uint4 x = *reinterpret_cast<const uint4*>(a.O + row * a.ldo + hd * 64 + c);
+  const uint4 y = *reinterpret_cast<const uint4*>(a.dO + row * a.lddo + hd * 64 + c);
+  float v = bf_lo(x.x) * bf_lo(y.x) + bf_hi(x.x) * bf_hi(y.x) + bf_lo(x.y) * bf_lo(y.y) + bf_hi(x.y) * bf_hi(y.y) + bf_lo(x.z) * bf_lo(y.z) +
+            bf_hi(x.z) * bf_hi(y.z) + bf_lo(x.w) * bf_lo(y.w) + bf_hi(x.w) * bf_hi(y.w);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if (c == 0) {
+    const long i = ((long)b * a.H + hd) * a.S + s;
+    const float l = a.LSE[i];
+    r.delta[i] = v;
+    r.delta[(long)a.B * a.H * a.S + i] = l == -INFINITY ? INFINITY : l;
+  }
+}
+
+// dQ (and the bucket sums of ds): 4 waves x 32 query rows over the key tiles
+template <bool BIAS, bool CAUSAL>
+__device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int tile_x, int hd, int b) {
+  const AitkAttnRelposArgs& a = r.a;
+  lds_char* const sm = (lds_char*)smem;
+  unsigned long long* const box = reinterpret_cast<unsigned long long*>(smem + 4 * TILE);
+  lds_float* const line = (lds_float*)(smem + 4 * TILE + 512);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5, S = a.S;
+  const int q0 = tile_x * 128 + wave * 32;
+  const v4i_t srdK = make_srd(a.K + (long)b * S * a.ldk + hd * 64, ((long)(S - 1) * a.ldk + 64) * 2);
+  const v4i_t srdV = make_srd(a.V + (long)b * S * a.ldv + hd * 64, ((long)(S - 1) * a.ldv + 64) * 2);
+  TileLane L;
+  L.init(lane, wave);
+  const int qc = min(q0 + l31, S - 1);
+  const bool live = q0 + l31 < S;
+  s16x8_t qf[4], gf[4];
+  {
+    const bf16_t* qp = a.Q + ((long)b * S + qc) * a.ldq + hd * 64 + 8 * h;
+    const bf16_t* gp = a.dO + ((long)b * S + qc) * a.lddo + hd * 64 + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      qf[ks] = *reinterpret_cast<const s16x8_t*>(qp + 16 * ks);
+      gf[ks] = *reinterpret_cast<const s16x8_t*>(gp + 16 * ks);
+    }
+  }
+  const long stat = ((long)b * a.H + hd) * S + qc;
+  const float delta = r.delta[stat];
+  const float l2 = live ? r.delta[(long)a.B * a.H * S + stat] : INFINITY;  // rows past the end: p = 0, ds = 0
+  const float c2 = a.scale * 1.4426950408889634f;
+  const int E = r.sat + BAND_PAD, n_line = 2 * E + 1;
+  const bool sums = BIAS && a.dtable != nullptr;
+  // bucket sums: every half wave adds its ds to accumulators of its own, one per distance (no two lanes of an instruction meet in one address, and one address sees its
+  // terms in program order: the sums do not depend on timing)
+  lds_float* const acc = line + 4 * r.line_p + (2 * wave + h) * n_line;
+  float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f;
+  const int ib = E + 4 * h - q0 - l31;
+  if constexpr (BIAS) {
+    build_line(line, r, hd, 1);
+    far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
+    far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
+    if (sums)
+      for (int i = tid; i < 8 * n_line; i += 256) (line + 4 * r.line_p)[i] = 0.f;
+    __syncthreads();
+  }
+  f32x16_t dq[2] = {zero16(), zero16()};
+  const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * 128 + 127) / 64 + 1) : (S + 63) / 64;
+  for (int t0 = 0; t0 < ntiles; t0 += 64) {
+    const unsigned long long masks = tile_masks(a, b, t0, ntiles, box, lane, wave);
+    unsigned long long todo = __ballot(masks != 0);
+    if (!todo) continue;
+    int t = __builtin_ctzll(todo), cur = 0;
+    unsigned long long keep = lane64(masks, t);
+    stage(sm, L, a.ldk, (t0 + t) * 64, srdK, wave, keep);
+    stage(sm + TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, keep);
+    dma_wait_all();
+    __syncthreads();
+    while (true) {
+      todo &= todo - 1;
+      const int tn = todo ? __builtin_ctzll(todo) : 0;
+      const unsigned long long keep_n = lane64(masks, tn);
+      if (todo) {
+        lds_char* nx = sm + (cur ^ 1) * 2 * TILE;
+        stage(nx, L, a.ldk, (t0 + tn) * 64, srdK, wave, keep_n);
+        stage(nx + TILE, L, a.ldv, (t0 + tn) * 64, srdV, wave, keep_n);
+      }
+      const lds_char* kt = sm + cur * 2 * TILE;
+      const lds_char* vt = kt + TILE;
+      const int kv0 = (t0 + t) * 64;
+      if (!CAUSAL || kv0 <= q0 + 31) {
+        float tb = 0.f;
+        int side = 0;  // 0: the band, 1: past, 2: ahead
+        if constexpr (BIAS) {
+          if (kv0 + 63 - q0 <= -r.sat) side = 1, tb = far_past;
+          else if (kv0 - q0 - 31 >= r.sat) side = 2, tb = far_ahead;
+        }
+        const float sub = tb - l2;
+        float fs = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          f32x16_t s, dp = zero16();
+          const int i0 = ib + kv0;
+          if (BIAS && side == 0) {
+            const lds_float* lp = line + (i0 & 3) * r.line_p + (i0 & ~3) + 32 * j;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(lp + 8 * g);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
+            }
+          } else {
+            s = zero16();
+          }
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) s = mfma32(frag_rm(kt, L, j, ks), qf[ks], s);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) dp = mfma32(frag_rm(vt, L, j, ks), gf[ks], dp);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, sub)) * (dp[e] - delta);
+          if (~keep) {
+            const unsigned mj = (unsigned)(keep >> (32 * j)) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (!(mj & (1u << ((e & 3) + 8 * (e >> 2))))) s[e] = 0.f;
+          }
+          if (CAUSAL && kv0 + 63 > q0) {
+            const int lim = q0 + l31 - kv0 - 4 * h - 32 * j;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if ((e & 3) + 8 * (e >> 2) > lim) s[e] = 0.f;
+          }
+          if (sums) {
+            if (side == 0) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                __hip_atomic_fetch_add(acc + i0 + 32 * j + (e & 3) + 8 * (e >> 2), s[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) fs += s[e];
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) {
+            const s16x8_t df = pack8r(s, 8 * kk);  // ds in bf16 for the matrix unit; the bucket sums above took the fp32 values
+#pragma unroll
+            for (int d = 0; d < 2; ++d) dq[d] = mfma32(frag_tr(kt, L, 2 * j + kk, d), df, dq[d]);
+          }
+        }
+        if (side == 1) fs_past += fs;
+        else fs_ahead += fs;
+      }
+      dma_wait_all();
+      __syncthreads();
+      if (!todo) break;
+      t = tn;
+      keep = keep_n;
+      cur ^= 1;
+    }
+  }
+  if (live) {
+    bf16_t* op = a.dQ + ((long)b * S + q0 + l31) * a.lddq + hd * 64;
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint2 u = make_uint2(pack2bf(dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale), pack2bf(dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale));
+        *reinterpret_cast<uint2*>(op + 32 * d + 8 * g + 4 * h) = u;
+      }
+  }
+  if (sums) {
+    lds_float* const fars = (lds_float*)smem;  // the tiles are done with (the loop ends behind a barrier; so does the set-up when no tile was visited)
+    fs_past = wave_sum(fs_past);
+    fs_ahead = wave_sum(fs_ahead);
+    if (lane == 0) {
+      fars[wave] = fs_past;
+      fars[4 + wave] = fs_ahead;
+    }
+    __syncthreads();
+    const lds_float* all = line + 4 * r.line_p;
+    if (tid < a.num_buckets) {
+      const bool ahead = tid >= r.half;
+      const int j = ahead ? tid - r.half : tid;
+      const bool last = j == r.half - 1;
+      const int n0 = r.first[j], n1 = last ? E + 1 : r.first[j + 1];
+      float v = 0.f;
+      if (last) v = ahead ? fars[4] + fars[5] + fars[6] + fars[7] : fars[0] + fars[1] + fars[2] + fars[3];
+      for (int n = n0 > 0 || !ahead ? n0 : 1; n < n1; ++n)
+        for (int w = 0; w < 8; ++w) v += all[w * n_line + E + (ahead ? n : -n)];
+      r.part[(((long)b * ((S + 127) / 128) + tile_x) * a.H + hd) * a.num_buckets + tid] = v;
+    }
+  }
+}
+
+// dK and dV: 4 waves x 32 keys over the query tiles.  S = Q K^T: a lane owns one key (column), its registers hold query rows, so the line of the bias runs backwards and
+// the row statistics come from LDS.  What a masked key computes stays in its own lane, which writes zeros.
+template <bool BIAS, bool CAUSAL>
+__device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int tile_x, int hd, int b) {
+  const AitkAttnRelposArgs& a = r.a;
+  lds_char* const sm = (lds_char*)smem;                        // 2 x (Q tile, dO tile)
+  lds_float* const st = (lds_float*)(smem + 4 * TILE);         // 2 x (64 lse, 64 delta)
+  lds_float* const line = (lds_float*)(smem + 4 * TILE + 1024);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5, S = a.S;
+  const int k0 = tile_x * 128 + wave * 32;
+  const int key = k0 + l31;
+  const bool inside = key < S;
+  const bool kept = inside && (!a.key_mask || a.key_mask[(long)b * S + (inside ? key : 0)] != 0);
+  f32x16_t dk[2] = {zero16(), zero16()}, dv[2] = {zero16(), zero16()};
+  const int ntiles = (S + 63) / 64, first_tile = CAUSAL ? tile_x * 2 : 0;
+  if (__syncthreads_or(kept)) {  // a block of keys that are all masked has zero gradients
+    const v4i_t srdQ = make_srd(a.Q + (long)b * S * a.ldq + hd * 64, ((long)(S - 1) * a.ldq + 64) * 2);
+    const v4i_t srdG = make_srd(a.dO + (long)b * S * a.lddo + hd * 64, ((long)(S - 1) * a.lddo + 64) * 2);
+    const long bh = (long)b * a.H + hd;
+    const v4i_t srdD = make_srd(r.delta + bh * S, (long)S * 4), srdL = make_srd(r.delta + ((long)a.B * a.H + bh) * S, (long)S * 4);
+    TileLane L;
+    L.init(lane, wave);
+    s16x8_t kf[4], vf[4];
+    {
+      const int kc = min(key, S - 1);
+      const bf16_t* kp = a.K + ((long)b * S + kc) * a.ldk + hd * 64 + 8 * h;
+      const bf16_t* vp = a.V + ((long)b * S + kc) * a.ldv + hd * 64 + 8 * h;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        kf[ks] = *reinterpret_cast<const s16x8_t*>(kp + 16 * ks);
+        vf[ks] = *reinterpret_cast<const s16x8_t*>(vp + 16 * ks);
+      }
+    }
+    const float c2 = a.scale * 1.4426950408889634f;
+    const int E = r.sat + BAND_PAD;
+    const int ib = E + 4 * h - key;  // line index of query 0 of this lane's first register: entry i is the bias of key - query = E - i
+    float far_past = 0.f, far_ahead = 0.f;
+    if constexpr (BIAS) {
+      build_line(line, r, hd, -1);
+      far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
+      far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
+    }
+    // rows past the end arrive as zeros: dO = 0 and delta = 0, so they add nothing to either gradient
+    auto stage_all = [&](int t, int buf) {
+      stage(sm + buf * 2 * TILE, L, a.ldq, t * 64, srdQ, wave, ~0ull);
+      stage(sm + buf * 2 * TILE + TILE, L, a.lddo, t * 64, srdG, wave, ~0ull);
+      if (wave < 2)
+        dma4(__builtin_amdgcn_readfirstlane((unsigned)(size_t)(st + buf * 128 + wave * 64)), (unsigned)((t * 64 + lane) * 4), wave ? srdD : srdL);
+    };
+    stage_all(first_tile, 0);
+    dma_wait_all();
+    __syncthreads();
+    for (int t = first_tile, cur = 0; t < ntiles; ++t, cur ^= 1) {
+      if (t + 1 < ntiles) stage_all(t + 1, cur ^ 1);
+      const lds_char* qt = sm + cur * 2 * TILE;
+      const lds_char* gt = qt + TILE;
+      const int qt0 = t * 64;
+      float tb = 0.f;
+      bool near = false;
+      if constexpr (BIAS) {
+        near = true;
+        if (k0 + 31 - qt0 <= -r.sat) near = false, tb = far_past;
+        else if (k0 - qt0 - 63 >= r.sat) near = false, tb = far_ahead;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f32x16_t s, dp = zero16();
+        if (BIAS && near) {
+          const int i0 = ib + qt0;
+          const lds_float* lp = line + (i0 & 3) * r.line_p + (i0 & ~3) + 32 * j;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(lp + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
+          }
+        } else {
+          s = zero16();
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) s = mfma32(frag_rm(qt, L, j, ks), kf[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) dp = mfma32(frag_rm(gt, L, j, ks), vf[ks], dp);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4_t l2 = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 32 * j + 8 * g + 4 * h);
+          const f32x4_t de = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 64 + 32 * j + 8 * g + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], c2, tb - l2[e]));
+            if (CAUSAL && qt0 + 32 * j + 8 * g + 4 * h + e < key) p = 0.f;
+            s[4 * g + e] = p;
+            dp[4 * g + e] = p * (dp[4 * g + e] - de[e]);
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const s16x8_t pf = pack8r(s, 8 * kk), df = pack8r(dp, 8 * kk);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            dv[d] = mfma32(frag_tr(gt, L, 2 * j + kk, d), pf, dv[d]);
+            dk[d] = mfma32(frag_tr(qt, L, 2 * j + kk, d), df, dk[d]);
+          }
+        }
+      }
+      dma_wait_all();
+      __syncthreads();
+    }
+  }
+  if (inside) {
+    bf16_t* kp = a.dK + ((long)b * S + key) * a.lddk + hd * 64;
+    bf16_t* vp = a.dV + ((long)b * S + key) * a.lddv + hd * 64;
+    const float sc = a.scale;
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint2 u = make_uint2(pack2bf(dk[d][4 * g] * sc, dk[d][4 * g + 1] * sc), pack2bf(dk[d][4 * g + 2] * sc, dk[d][4 * g + 3] * sc));
+        uint2 w = make_uint2(pack2bf(dv[d][4 * g], dv[d][4 * g + 1]), pack2bf(dv[d][4 * g + 2], dv[d][4 * g + 3]));
+        if (!kept) u = w = make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(kp + 32 * d + 8 * g + 4 * h) = u;
+        *reinterpret_cast<uint2*>(vp + 32 * d + 8 * g + 4 * h) = w;
+      }
+  }
+}
+
+// both gradients in one launch (they share nothing but their inputs): twice the workgroups, so that a single prompt fills the chip
+template <bool BIAS, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void attn_relpos_bwd_kernel(RelposArgs r) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int nt = (r.a.S + 127) / 128;
+  int tile_x, hd, b;
+  wg_coords(2 * nt, r.a.H, tile_x, hd, b);
+  if (tile_x < nt) dq_role<BIAS, CAUSAL>(r, smem, tile_x, hd, b);
+  else dkv_role<BIAS, CAUSAL>(r, smem, tile_x - nt, hd, b);
+}
+
+// dtable[j][head] (+)= sum over the samples' row tiles, in their order
+__global__ __launch_bounds__(256) void attn_relpos_dtable_kernel(RelposArgs r) {
+  const AitkAttnRelposArgs& a = r.a;
+  const int i = blockIdx.x * 256 + threadIdx.x, n = a.H * a.num_buckets;
+  if (i >= n) return;
+  const int rows = a.B * ((a.S + 127) / 128);
+  float v = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < rows; ++k) v += r.part[(long)k * n + i];
+  const long at = (long)(i % a.num_buckets) * a.H + i / a.num_buckets;
+  if (a.dtable_f32) {
+    float* out = reinterpret_cast<float*>(a.dtable) + at;
+    *out = a.accumulate ? *out + v : v;
+  } else {
+    bf16_t* out = reinterpret_cast<bf16_t*>(a.dtable) + at;
+    *out = f2bf(a.accumulate ? bf2f(*out) + v : v);
+  }
+}
+
+// first distance of every bucket of one sign: exact up to half / 2, then the smallest n with (n / e)^L >= (max_distance / e)^j for step j of L.  The two sides are
+// products of whole numbers: closer than 1e-9 in the logarithm means equal (the border belongs to the farther bucket).
+int bucket_table(int num_buckets, int max_distance, int causal, int* first) {
+  const int half = causal ? num_buckets : num_buckets / 2;
+  if (num_buckets <= 0 || (!causal && (num_buckets & 1)) || half < 2 || half > MAX_HALF) return 0;
+  const int e = half / 2, L = half - e;
+  if (max_distance <= e || max_distance > 1024) return 0;
+  int n = e;
+  for (int j = 0; j < half; ++j) {
+    if (j <= e) {
+      first[j] = j;
+      continue;
+    }
+    while (L * logl((long double)n / e) < (j - e) * logl((long double)max_distance / e) - 1e-9L) ++n;
+    first[j] = n;
+  }
+  return half;
+}
+
+bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
+bool bad_view(const void* p, int64_t ld, const AitkAttnRelposArgs* a) { return (ld % 8) || ld < (int64_t)a->H * 64 || mis16(p); }
+
+int check(const AitkAttnRelposArgs* a, bool bwd, RelposArgs& r) {
+  if (!a || a->B <= 0 || a->H <= 0 || a->S <= 0 || a->H > 65535 || a->B > 65535 || !(a->scale > 0.f) || a->scale > 3.0e38f) return AITK_ERR_SHAPE;
+  if ((int64_t)a->B * a->H * ((a->S + 127) / 128) * 2 > 0x7fffffff) return AITK_ERR_SHAPE;
+  if (!a->Q || !a->K || !a->V || !a->O || !a->LSE) return AITK_ERR_ARG;
+  if (bad_view(a->Q, a->ldq, a) || bad_view(a->K, a->ldk, a) || bad_view(a->V, a->ldv, a) || bad_view(a->O, a->ldo, a)) return AITK_ERR_ALIGN;
+  int64_t widest = a->ldk > a->ldv ? a->ldk : a->ldv;
+  if (bwd) {
+    if (!a->dO || !a->dQ || !a->dK || !a->dV || !a->ws || (a->dtable && !a->table)) return AITK_ERR_ARG;
+    if (bad_view(a->dO, a->lddo, a) || bad_view(a->dQ, a->lddq, a) || bad_view(a->dK, a->lddk, a) || bad_view(a->dV, a->lddv, a) || mis16(a->ws)) return AITK_ERR_ALIGN;
+    if (a->ldq > widest) widest = a->ldq;
+    if (a->lddo > widest) widest = a->lddo;
+  }
+  if (((int64_t)a->S + 64) * widest * 2 >= 0x7fffffff) return AITK_ERR_SHAPE;  // a head's slice is one buffer descriptor with 31-bit offsets
+  r.a = *a;
+  r.half = r.sat = r.line_p = 0;
+  r.delta = r.part = nullptr;
+  for (int i = 0; i < MAX_HALF; ++i) r.first[i] = 0;
+  if (a->table) {
+    r.half = bucket_table(a->num_buckets, a->max_distance, a->causal, r.first);
+    if (!r.half) return AITK_ERR_SHAPE;
+    r.sat = r.first[r.half - 1];
+    r.line_p = (2 * (r.sat + BAND_PAD) + 5 + 63) / 64 * 64 + 16;  // 64 bytes modulo the 256 that the banks span: the four copies meet in no bank
+  }
+  return AITK_OK;
+}
+
+template <typename K>
+int launch(K kernel, unsigned grid, size_t lds, const RelposArgs& r, hipStream_t s) {
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, s, r);
+  AITK_LAUNCH_CHECK();
+  return AITK_OK;
+}
+}  // namespace
+
+extern "C" int aitk_attn_relpos_buckets(int32_t num_buckets, int32_t max_distance, int32_t causal, int32_t* first) {
+  int f[MAX_HALF];
+  if (!first) return AITK_ERR_ARG;
+  const int half = bucket_table(num_buckets, max_distance, causal, f);
+  if (!half) return AITK_ERR_SHAPE;
+  for (int i = 0; i < half; ++i) first[i] = f[i];
+  return half;
+}
+
+extern "C" int aitk_attn_relpos_fwd(const AitkAttnRelposArgs* a, aitk_stream_t stream) {
+  RelposArgs r;
+  const int rc = check(a, false, r);
+  if (rc != AITK_OK) return rc;
+  const unsigned grid = (unsigned)((a->S + 127) / 128) * a->H * a->B;
+  const size_t lds = 4 * TILE + 512 + (size_t)4 * r.line_p * 4;
+  hipStream_t s = (hipStream_t)stream;
+  if (a->table) return a->causal ? launch(attn_relpos_fwd_kernel<true, true>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<true, false>, grid, lds, r, s);
+  return a->causal ? launch(attn_relpos_fwd_kernel<false, true>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<false, false>, grid, lds, r, s);
+}
+
+extern "C" int64_t aitk_attn_relpos_bwd_workspace_bytes(int32_t B, int32_t H, int32_t S, int32_t num_buckets) {
+  if (B <= 0 || H <= 0 || S <= 0 || num_buckets < 0) return 0;
+  return ((int64_t)2 * B * H * S + (int64_t)B * ((S + 127) / 128) * H * num_buckets) * 4;
+}
+
+extern "C" int aitk_attn_relpos_bwd(const AitkAttnRelposArgs* a, aitk_stream_t stream) {
+  RelposArgs r;
+  int rc = check(a, true, r);
+  if (rc != AITK_OK) return rc;
+  r.delta = a->ws;
+  r.part = a->ws + (int64_t)2 * a->B * a->H * a->S;
+  hipStream_t s = (hipStream_t)stream;
+  hipLaunchKernelGGL(attn_relpos_delta_kernel, dim3((a->S + 31) / 32, a->H, a->B), dim3(256), 0, s, r);
+  AITK_LAUNCH_CHECK();
+  const unsigned grid = (unsigned)((a->S + 127) / 128) * a->H * a->B * 2;
+  const size_t lds = 4 * TILE + 1024 + (size_t)4 * r.line_p * 4 + (a->dtable ? (size_t)8 * (2 * (r.sat + BAND_PAD) + 1) * 4 : 0);
+  if (a->table) rc = a->causal ? launch(attn_relpos_bwd_kernel<true, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<true, false>, grid, lds, r, s);
+  else rc = a->causal ? launch(attn_relpos_bwd_kernel<false, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<false, false>, grid, lds, r, s);
+  if (rc != AITK_OK) return rc;
+  if (a->dtable) {
+    hipLaunchKernelGGL(attn_relpos_dtable_kernel, dim3((a->H * a->num_buckets + 255) / 256), dim3(256), 0, s, r);
+    AITK_LAUNCH_CHECK();
+  }
+  return AITK_OK;
+}

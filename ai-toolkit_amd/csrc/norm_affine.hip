@@ -1,0 +1,356 @@
+// LayerNorm / RMSNorm with a learned weight (and bias), forward and backward, the gradients of weight and bias included (gfx950).  The norms of the text
+// encoders (CLIP: layer norm with bias; T5 / UMT5: RMS norm without mean or bias) and of the UNet transformer blocks.
+//
+//   layer:  xh = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps);   rms:  xh = x rstd,  rstd = 1 / sqrt(mean(x^2) + eps)
+//   y  = xh w (+ b)
+//   dx = rstd (g - c1 - xh c2) (+ dres),  g = dy w,  c1 = mean(g) (layer; 0 for rms),  c2 = mean(g xh)
+//   dw = sum over rows of dy xh,  db = sum over rows of dy
+//
+// Bound by memory: forward reads x and writes y, backward reads x and dy (and dres) and writes dx; everything else stays in registers.  A row is held by LPR
+// lanes as NV packed 16-byte vectors each (16 lanes for narrow rows, so that a wave works on four of them; one wave up to 2048 columns; four waves beyond, where a
+// single wave would not have the registers for the column sums) and read ONCE: mean, centred squares and the output come from the registers.  Statistics and sums are
+// fp32; x, y, dy, dx are bf16 and each output element is rounded once.
+#include "common.h"
+#include "aitk_args.h"
+
+namespace {
+
+__device__ __forceinline__ void up8(const uint4& v, float* f) {
+  f[0] = bf_lo(v.x); f[1] = bf_hi(v.x); f[2] = bf_lo(v.y); f[3] = bf_hi(v.y);
+  f[4] = bf_lo(v.z); f[5] = bf_hi(v.z); f[6] = bf_lo(v.w); f[7] = bf_hi(v.w);
+}
+__device__ __forceinline__ uint4 dn8(const float* f) {
+  return make_uint4(pack2bf(f[0], f[1]), pack2bf(f[2], f[3]), pack2bf(f[4], f[5]), pack2bf(f[6], f[7]));
+}
+// 8 consecutive elements of a weight / bias vector (bf16 or fp32)
+__device__ __forceinline__ void load_w8(const void* w, int f32, int c, float* f) {
+  if (f32) {
+    const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + c);
+    const float4 a = q[0], b = q[1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    up8(*reinterpret_cast<const uint4*>(reinterpret_cast<const bf16_t*>(w) + c), f);
+  }
+}
+
+// sum over the LPR lanes of a row; rows of more than one wave meet in `slot` (one float per wave of the workgroup), which the caller alternates so that one
+// barrier per sum is enough.  Every lane of the workgroup calls it the same number of times.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, float* slot) {
+#pragma unroll
+  for (int o = (LPR > 64 ? 64 : LPR) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (LPR > 64) {
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) slot[wave] = v;
+    __syncthreads();
+    const int w0 = wave & ~(LPR / 64 - 1);
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < LPR / 64; ++i) v += slot[w0 + i];
+  }
+  return v;
+}
+
+template <int LPR, int NV, bool RMS>
+__global__ __launch_bounds__(256) void norm_fwd_kernel(AitkNormArgs p) {
+  constexpr int RPW = 256 / LPR;  // rows a workgroup works on at a time
+  __shared__ float red[2][2][4];
+  const int t = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+  const float inv_c = 1.0f / (float)p.C;
+  int par = 0;
+  for (long base = (long)blockIdx.x * RPW; base < p.M; base += (long)gridDim.x * RPW, par ^= 1) {
+    const long m = base + grp;
+    const bool live = m < p.M;
+    const bf16_t* xr = p.x + (live ? m : 0) * p.ldx;
+    uint4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + LPR * i) * 8;
+      v[i] = c < p.C ? *reinterpret_cast<const uint4*>(xr + c) : make_uint4(0, 0, 0, 0);
+    }
+    float mean = 0.f;
+    if constexpr (!RMS) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float f[8];
+        up8(v[i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += f[e];
+      }
+      mean = row_sum<LPR>(s, red[par][0]) * inv_c;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[8];
+      up8(v[i], f);
+      if ((t + LPR * i) * 8 < p.C) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q += (f[e] - mean) * (f[e] - mean);
+      }
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<LPR>(q, red[par][1]) * inv_c + p.eps);
+    if (!live) continue;
+    if (t == 0) {
+      if (p.mean) p.mean[m] = mean;
+      if (p.rstd) p.rstd[m] = rstd;
+    }
+    bf16_t* yr = p.y + m * p.ldy;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + LPR * i) * 8;
+      if (c < p.C) {
+        float f[8], w[8], b[8] = {};
+        up8(v[i], f);
+        load_w8(p.weight, p.w_f32, c, w);
+        if (p.bias) load_w8(p.bias, p.w_f32, c, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = fmaf((f[e] - mean) * rstd, w[e], b[e]);
+        *reinterpret_cast<uint4*>(yr + c) = dn8(f);
+      }
+    }
+  }
+}
+
+// Backward.  A workgroup of 512 threads walks its rows with the next row's x and dy in flight; each thread owns fixed columns and sums dy xh and dy over its rows in
+// registers; the column sums of all its rows leave the workgroup as ONE row of partials (one workgroup per CU above 2048 columns, two below).
+#define NB_THREADS 512
+#define NB_SLOTS(LPR) ((LPR) == 256 ? 1 : 4)  // column sums of so many row groups meet in LDS at a time (at most 32 KiB)
+template <int LPR, int NV, bool RMS, bool GRADS>
+__global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p) {
+  constexpr int RPW = NB_THREADS / LPR;
+  __shared__ float red[2][2][NB_THREADS / 64];
+  extern __shared__ __attribute__((aligned(16))) float colsum[];  // [SLOTS][C] when GRADS
+  const int t = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+  const float inv_c = 1.0f / (float)p.C;
+  float dw[NV][8] = {}, db[NV][8] = {};
+  uint4 xv[NV], gv[NV];
+  auto fetch = [&](long m, uint4* xo, uint4* go) {
+    const long r = m < p.M ? m : 0;
+    const bf16_t* xr = p.x + r * p.ldx;
+    const bf16_t* gr = p.dy + r * p.ld_dy;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + LPR * i) * 8;
+      xo[i] = c < p.C ? *reinterpret_cast<const uint4*>(xr + c) : make_uint4(0, 0, 0, 0);
+      go[i] = c < p.C ? *reinterpret_cast<const uint4*>(gr + c) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  const long step = (long)gridDim.x * RPW;
+  long base = (long)blockIdx.x * RPW;
+  fetch(base + grp, xv, gv);
+  int par = 0;
+  for (; base < p.M; base += step, par ^= 1) {
+    const long m = base + grp;
+    const bool live = m < p.M;
+    const long mr = live ? m : 0;
+    const float mean = RMS ? 0.f : p.mean[mr], rstd = p.rstd[mr];
+    uint4 xn[NV], gn[NV], rv[NV];
+    if (base + step < p.M) fetch(m + step, xn, gn);
+    if (p.dres) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (t + LPR * i) * 8;
+        rv[i] = c < p.C ? *reinterpret_cast<const uint4*>(p.dres + mr * p.ld_dres + c) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + LPR * i) * 8;
+      if (c < p.C) {
+        float x[8], g[8], w[8];
+        up8(xv[i], x);
+        up8(gv[i], g);
+        load_w8(p.weight, p.w_f32, c, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float xh = (x[e] - mean) * rstd, gw = g[e] * w[e];
+          s1 += gw;
+          s2 = fmaf(gw, xh, s2);
+          if (GRADS && live) {
+            dw[i][e] = fmaf(g[e], xh, dw[i][e]);
+            db[i][e] += g[e];
+          }
+        }
+      }
+    }
+    const float c1 = RMS ? 0.f : row_sum<LPR>(s1, red[par][0]) * inv_c;
+    const float c2 = row_sum<LPR>(s2, red[par][1]) * inv_c;
+    if (live) {
+      bf16_t* dr = p.dx + m * p.ld_dx;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (t + LPR * i) * 8;
+        if (c < p.C) {
+          float x[8], g[8], w[8], r[8] = {};
+          up8(xv[i], x);
+          up8(gv[i], g);
+          if (p.dres) up8(rv[i], r);
+          load_w8(p.weight, p.w_f32, c, w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float xh = (x[e] - mean) * rstd;
+            r[e] = fmaf(rstd, g[e] * w[e] - c1 - xh * c2, r[e]);
+          }
+          *reinterpret_cast<uint4*>(dr + c) = dn8(r);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      xv[i] = xn[i];
+      gv[i] = gn[i];
+    }
+  }
+  if constexpr (GRADS) {
+    if constexpr (LPR < 64) {  // the row groups of one wave hold the same columns
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int o = LPR; o < 64; o <<= 1) {
+            dw[i][e] += __shfl_xor(dw[i][e], o, 64);
+            if (!RMS) db[i][e] += __shfl_xor(db[i][e], o, 64);
+          }
+    }
+    // the row groups of the workgroup meet in LDS in a fixed order, one vector after the other
+    constexpr int G = LPR < 64 ? NB_THREADS / 64 : RPW, SLOTS = NB_SLOTS(LPR);
+    const int g = LPR < 64 ? threadIdx.x >> 6 : grp;
+    const bool holds = LPR >= 64 || (threadIdx.x & 63) < LPR;
+    for (int v = 0; v < (RMS ? 1 : 2); ++v) {
+      for (int r0 = 0; r0 < G; r0 += SLOTS) {
+        __syncthreads();
+        if (holds && g >= r0 && g < r0 + SLOTS) {
+          float* dst = colsum + (g - r0) * p.C;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const int c = (t + LPR * i) * 8;
+            if (c < p.C) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float a = v ? db[i][e] : dw[i][e];
+                dst[c + e] = r0 ? dst[c + e] + a : a;
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();
+      float* out = p.partial + ((long)blockIdx.x * (RMS ? 1 : 2) + v) * p.C;
+      for (int c = threadIdx.x; c < p.C; c += NB_THREADS) {
+        float a = colsum[c];
+        for (int k = 1; k < SLOTS; ++k) a += colsum[k * p.C + c];
+        out[c] = a;
+      }
+    }
+  }
+}
+
+// the workgroups' partials [nwg][V][C] -> dw, db: 32 columns per workgroup (8 float4 lanes x 32 slices of the workgroups), fixed order
+__global__ __launch_bounds__(256) void norm_wgrad_finish_kernel(const float* partial, int nwg, int V, int C, float* dw, float* db, int accumulate) {
+  __shared__ float4 part[32][8];
+  const int j = threadIdx.x & 7, sl = threadIdx.x >> 3;
+  const int c = blockIdx.x * 32 + j * 4, v = blockIdx.y;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c < C) {
+#pragma unroll 8
+    for (int w = sl; w < nwg; w += 32) {
+      const float4 a = *reinterpret_cast<const float4*>(partial + ((long)w * V + v) * C + c);
+      s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
+    }
+  }
+  part[sl][j] = s;
+  __syncthreads();
+  float* out = v ? db : dw;
+  if (threadIdx.x < 32) {
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    if (out && col < C) {
+      float a = 0.f;
+      for (int k = 0; k < 32; ++k) a += reinterpret_cast<const float*>(&part[k][0])[threadIdx.x];
+      out[col] = accumulate ? out[col] + a : a;
+    }
+  }
+}
+
+bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
+
+int bwd_grid(int M, int C) {
+  const int rpw = C <= 512 ? NB_THREADS / 16 : C <= 2048 ? NB_THREADS / 64 : NB_THREADS / 256;
+  const int n = (M + rpw - 1) / rpw;
+  const int most = C <= 2048 ? 512 : 256;
+  return n < most ? n : most;
+}
+
+template <int LPR, int NV>
+void launch_fwd(const AitkNormArgs& a, hipStream_t s) {
+  const long n = ((long)a.M + 256 / LPR - 1) / (256 / LPR);
+  const dim3 grid((unsigned)(n < 4096 ? n : 4096));
+  if (a.rms) hipLaunchKernelGGL((norm_fwd_kernel<LPR, NV, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((norm_fwd_kernel<LPR, NV, false>), grid, dim3(256), 0, s, a);
+}
+template <int LPR, int NV>
+void launch_bwd(const AitkNormBwdArgs& a, hipStream_t s) {
+  const bool grads = a.dweight || a.dbias;
+  const dim3 grid(bwd_grid(a.M, a.C));
+  const size_t lds = grads ? (size_t)NB_SLOTS(LPR) * a.C * 4 : 0;
+  if (a.rms) {
+    if (grads) hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, true, true>), grid, dim3(NB_THREADS), lds, s, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, true, false>), grid, dim3(NB_THREADS), lds, s, a);
+  } else {
+    if (grads) hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, false, true>), grid, dim3(NB_THREADS), lds, s, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, false, false>), grid, dim3(NB_THREADS), lds, s, a);
+  }
+}
+}  // namespace
+
+extern "C" int aitk_norm_fwd(const AitkNormArgs* a, aitk_stream_t stream) {
+  if (!a || a->M <= 0 || a->C <= 0 || (a->C % 8) || a->C > 8192) return AITK_ERR_SHAPE;
+  if (!a->x || !a->weight || !a->y || (a->rms && (a->bias || a->mean))) return AITK_ERR_ARG;
+  if ((a->ldx % 8) || (a->ldy % 8) || a->ldx < a->C || a->ldy < a->C || mis16(a->x) || mis16(a->y) || mis16(a->weight) || mis16(a->bias)) return AITK_ERR_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  const int C = a->C;
+  if (C <= 128) launch_fwd<16, 1>(*a, s);
+  else if (C <= 256) launch_fwd<16, 2>(*a, s);
+  else if (C <= 512) launch_fwd<16, 4>(*a, s);
+  else if (C <= 1024) launch_fwd<64, 2>(*a, s);
+  else if (C <= 1536) launch_fwd<64, 3>(*a, s);
+  else if (C <= 2048) launch_fwd<64, 4>(*a, s);
+  else if (C <= 4096) launch_fwd<256, 2>(*a, s);
+  else launch_fwd<256, 4>(*a, s);
+  AITK_LAUNCH_CHECK();
+  return AITK_OK;
+}
+
+extern "C" int64_t aitk_norm_bwd_workspace_bytes(int32_t M, int32_t C, int32_t rms) {
+  if (M <= 0 || C <= 0) return 0;
+  return (int64_t)bwd_grid(M, C) * (rms ? 1 : 2) * C * 4;
+}
+
+extern "C" int aitk_norm_bwd(const AitkNormBwdArgs* a, aitk_stream_t stream) {
+  if (!a || a->M <= 0 || a->C <= 0 || (a->C % 8) || a->C > 8192) return AITK_ERR_SHAPE;
+  const bool grads = a->dweight || a->dbias;
+  if (!a->dy || !a->x || !a->weight || !a->rstd || !a->dx || (!a->rms && !a->mean) || (a->rms && a->dbias) || (grads && !a->partial)) return AITK_ERR_ARG;
+  if ((a->ld_dy % 8) || (a->ldx % 8) || (a->ld_dx % 8) || (a->dres && ((a->ld_dres % 8) || a->ld_dres < a->C)) || a->ld_dy < a->C || a->ldx < a->C ||
+      a->ld_dx < a->C || mis16(a->dy) || mis16(a->x) || mis16(a->weight) || mis16(a->dres) || mis16(a->dx) || mis16(a->partial))
+    return AITK_ERR_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  const int C = a->C;
+  if (C <= 128) launch_bwd<16, 1>(*a, s);
+  else if (C <= 256) launch_bwd<16, 2>(*a, s);
+  else if (C <= 512) launch_bwd<16, 4>(*a, s);
+  else if (C <= 1024) launch_bwd<64, 2>(*a, s);
+  else if (C <= 1536) launch_bwd<64, 3>(*a, s);
+  else if (C <= 2048) launch_bwd<64, 4>(*a, s);
+  else if (C <= 4096) launch_bwd<256, 2>(*a, s);
+  else launch_bwd<256, 4>(*a, s);
+  AITK_LAUNCH_CHECK();
+  if (grads) {
+    const int V = a->rms ? 1 : 2;
+    hipLaunchKernelGGL(norm_wgrad_finish_kernel, dim3((C + 31) / 32, V), dim3(256), 0, s, a->partial, bwd_grid(a->M, C), V, C, a->dweight, a->dbias, a->accumulate);
+    AITK_LAUNCH_CHECK();
+  }
+  return AITK_OK;
+}

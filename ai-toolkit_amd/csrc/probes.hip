@@ -91,6 +91,9 @@ extern "C" int aitk_sizeof(int32_t which) {
     case 21: return (int)sizeof(AitkDdpmNoiseArgs);
     case 22: return (int)sizeof(AitkQuantRowsArgs);
     case 23: return (int)sizeof(AitkWgradSrc2);
+    case 24: return (int)sizeof(AitkNormArgs);
+    case 25: return (int)sizeof(AitkNormBwdArgs);
+    case 26: return (int)sizeof(AitkAttnRelposArgs);
     default: return -1;
   }
 }

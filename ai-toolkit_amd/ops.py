@@ -1195,3 +1195,159 @@ def attn_small_bwd(q, k, v, o, lse, do, dq, dk, dv, *, B, H, S, D, scale, Skv=0)
     a.lddq, a.lddk, a.lddv = _row_major(dq, "dq"), _row_major(dk, "dk"), _row_major(dv, "dv")
     a.delta = _ptr(workspace(B * H * S * 4, q.device, "attn_delta"))
     _call("aitk_attn_small_bwd", C.byref(a))
+
+
+# ---------------------------------------------------------------------------------------------------------- text-encoder block
+# Norms with a learned weight, attention with a learned relative position bias, the gated feed-forward projections.  Arguments that the kernels cannot take raise
+# ValueError before anything is launched; scratch is a torch allocation of the call (current stream's, and a capturing graph's own pool), never a buffer that two
+# streams or two captured graphs would share.
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _rows(t, name, rows, cols):
+    """bf16 [rows, cols] view with unit inner stride, a row pitch of whole 16-byte chunks and a 16-byte aligned start -> the row pitch"""
+    _need(t.dtype == BF16, f"{name}: expected bf16, got {t.dtype}")
+    _need(t.dim() == 2 and tuple(t.shape) == (rows, cols), f"{name}: expected [{rows}, {cols}], got {tuple(t.shape)}")
+    ld = t.stride(0) if rows > 1 else max(t.stride(0), -(-cols // 8) * 8)  # the pitch of a single row is nobody's
+    _need(cols == 1 or t.stride(1) == 1, f"{name}: the inner stride must be 1, got strides {t.stride()}")
+    _need(ld >= cols and ld % 8 == 0 and t.data_ptr() % 16 == 0, f"{name}: rows must be 16-byte aligned and must not overlap (strides {t.stride()})")
+    return ld
+
+
+def _vec(t, name, n, dtypes):
+    _need(t.dtype in dtypes, f"{name}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    _need(t.dim() == 1 and t.numel() == n and t.is_contiguous(), f"{name}: expected a contiguous [{n}], got {tuple(t.shape)} strides {t.stride()}")
+    _need(t.data_ptr() % 16 == 0, f"{name}: must be 16-byte aligned")
+
+
+def _on_device(**tensors):
+    """every operand lives on the current GPU: the launch goes to its current stream"""
+    for name, t in tensors.items():
+        if t is not None:
+            _need(t.is_cuda, f"{name}: expected a tensor on the GPU, got {t.device}")
+            _need(t.device.index == torch.cuda.current_device(), f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _scratch(nbytes, device):
+    return torch.empty(max(1, (nbytes + 3) // 4), dtype=torch.float32, device=device)
+
+
+def norm_fwd(x, weight, y, *, bias=None, rms=False, mean=None, rstd=None, eps=1e-6):
+    """y = xh * weight (+ bias) per row of x [M, C] bf16: xh = (x - mean) / sqrt(var + eps) (layer norm) or x / sqrt(mean(x^2) + eps) (rms: no mean, no bias).
+    weight / bias [C] bf16 or fp32 (both the same); mean / rstd: fp32 [M], written for norm_bwd (mean: layer norm only).  y may be x.  C % 8 == 0, C <= 8192."""
+    _need(x.dim() == 2, f"x: expected [M, C], got {tuple(x.shape)}")
+    M, Cc = x.shape
+    _need(Cc > 0 and Cc % 8 == 0 and Cc <= 8192, f"x: C must be a multiple of 8 up to 8192, got {Cc}")
+    _need(eps >= 0, f"eps must not be negative, got {eps}")
+    a = _capi.NormArgs()
+    a.ldx, a.ldy = _rows(x, "x", M, Cc), _rows(y, "y", M, Cc)
+    _vec(weight, "weight", Cc, (BF16, torch.float32))
+    if bias is not None:
+        _need(not rms, "bias: an RMS norm has none")
+        _vec(bias, "bias", Cc, (weight.dtype,))
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t is not None:
+            _need(t.dtype == torch.float32 and t.dim() == 1 and t.numel() == M and t.is_contiguous(), f"{name}: expected a contiguous fp32 [{M}]")
+    _need(mean is None or not rms, "mean: an RMS norm has none")
+    _on_device(x=x, weight=weight, y=y, bias=bias, mean=mean, rstd=rstd)
+    if M == 0:
+        return y
+    a.x, a.weight, a.bias, a.y, a.mean, a.rstd = _ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd)
+    a.eps, a.rms, a.w_f32, a.M, a.C = eps, int(rms), int(weight.dtype == torch.float32), M, Cc
+    _call("aitk_norm_fwd", C.byref(a))
+    return y
+
+
+def norm_bwd(dy, x, weight, rstd, dx, *, mean=None, rms=False, dres=None, dweight=None, dbias=None, accumulate=False):
+    """dx = norm_fwd's gradient . dy (+ dres) from the saved rstd (and, layer norm, mean); dweight / dbias (fp32 [C], either may be left out) = the gradients of weight
+    and bias, added to what they hold with `accumulate`.  dx may be dy, x or dres.  Deterministic."""
+    _need(x.dim() == 2, f"x: expected [M, C], got {tuple(x.shape)}")
+    M, Cc = x.shape
+    _need(Cc > 0 and Cc % 8 == 0 and Cc <= 8192, f"x: C must be a multiple of 8 up to 8192, got {Cc}")
+    a = _capi.NormBwdArgs()
+    a.ld_dy, a.ldx, a.ld_dx = _rows(dy, "dy", M, Cc), _rows(x, "x", M, Cc), _rows(dx, "dx", M, Cc)
+    if dres is not None:
+        a.ld_dres = _rows(dres, "dres", M, Cc)
+    _vec(weight, "weight", Cc, (BF16, torch.float32))
+    _need((mean is None) == bool(rms), "mean: a layer norm needs the saved mean, an RMS norm has none")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t is not None:
+            _need(t.dtype == torch.float32 and t.dim() == 1 and t.numel() == M and t.is_contiguous(), f"{name}: expected a contiguous fp32 [{M}]")
+    _need(dbias is None or not rms, "dbias: an RMS norm has no bias")
+    for t, name in ((dweight, "dweight"), (dbias, "dbias")):
+        if t is not None:
+            _vec(t, name, Cc, (torch.float32,))
+    _on_device(dy=dy, x=x, weight=weight, rstd=rstd, dx=dx, mean=mean, dres=dres, dweight=dweight, dbias=dbias)
+    if M == 0:
+        if not accumulate:
+            host_call(lambda: [t.zero_() for t in (dweight, dbias) if t is not None])
+        return dx
+    if dweight is not None or dbias is not None:
+        part = _scratch(_capi.lib().aitk_norm_bwd_workspace_bytes(M, Cc, int(rms)), x.device)
+        a.partial = _ptr(part)
+    a.dy, a.x, a.weight, a.mean, a.rstd, a.dres, a.dx = _ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dres), _ptr(dx)
+    a.dweight, a.dbias = _ptr(dweight), _ptr(dbias)
+    a.rms, a.w_f32, a.accumulate, a.M, a.C = int(rms), int(weight.dtype == torch.float32), int(accumulate), M, Cc
+    _call("aitk_norm_bwd", C.byref(a))
+    return dx
+
+
+def _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal):
+    _need(B >= 0 and H > 0 and S >= 0, f"B, H, S: got {B}, {H}, {S}")
+    _need(0.0 < scale < float("inf"), f"scale must be positive and finite, got {scale}")
+    a = _capi.AttnRelposArgs()
+    a.ldq, a.ldk, a.ldv, a.ldo = (_rows(t, n, B * S, H * 64) for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")))
+    _need(lse.dtype == torch.float32 and lse.numel() == B * H * S and lse.is_contiguous(), f"lse: expected a contiguous fp32 [{B}, {H}, {S}]")
+    if table is not None:
+        _need(table.dtype == BF16 and table.dim() == 2 and table.shape[1] == H and table.is_contiguous(), f"table: expected a contiguous bf16 [num_buckets, {H}]")
+        a.num_buckets, a.max_distance = table.shape[0], max_distance
+        _need(_capi.lib().aitk_attn_relpos_buckets(a.num_buckets, max_distance, int(causal), (C.c_int32 * 64)()) > 0,
+              f"table: {a.num_buckets} buckets up to distance {max_distance} (causal={bool(causal)}): 2 to 64 buckets of each sign, whose exact half must end below max_distance <= 1024")
+    if key_mask is not None:
+        _need(key_mask.dtype in (torch.bool, torch.uint8), f"key_mask: expected bool or uint8 (non-zero = attend), got {key_mask.dtype}")
+        _need(tuple(key_mask.shape) == (B, S) and key_mask.is_contiguous(), f"key_mask: expected a contiguous [{B}, {S}], got {tuple(key_mask.shape)}")
+    a.scale, a.B, a.H, a.S, a.causal = scale, B, H, S, int(causal)
+    _need((S + 64) * max(t.stride(0) if B * S > 1 else 0 for t in (q, k, v)) * 2 < 2 ** 31 - 1, "a head's slice of q / k / v must stay below 2 GiB")
+    return a
+
+
+def _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask):
+    a.Q, a.K, a.V, a.O, a.LSE, a.table, a.key_mask = _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(table), _ptr(key_mask)
+
+
+def attn_relpos_fwd(q, k, v, table, o, lse, *, B, H, S, scale=1.0, key_mask=None, max_distance=128, causal=False):
+    """o = softmax(scale q k^T + table[bucket(key - query)]) v: the text encoders' attention with a learned relative position bias.  q, k, v, o: [B*S, H*64] bf16 views
+    (row pitch = token pitch); table: bf16 [num_buckets, H] (T5's relative_attention_bias.weight) or None (no bias: CLIP); lse: fp32 [B, H, S], written for the backward.
+    key_mask: bool / uint8 [B, S], non-zero = attend; causal: keys up to the query, all buckets for the past.  A row that the masks leave empty gives 0 (lse = -inf);
+    what masked keys hold reaches nothing, NaN and infinities too."""
+    a = _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
+    _on_device(q=q, k=k, v=v, table=table, o=o, lse=lse, key_mask=key_mask)
+    if B * S == 0:
+        return o
+    _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask)
+    _call("aitk_attn_relpos_fwd", C.byref(a))
+    return o
+
+
+def attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable=None, *, B, H, S, scale=1.0, key_mask=None, max_distance=128, causal=False, accumulate=False):
+    """dq, dk, dv ([B*S, H*64] bf16 views) and, if given, dtable ([num_buckets, H] bf16 or fp32: the table's gradient, added to what it holds with `accumulate` — T5's layers
+    share one table) from attn_relpos_fwd's operands, o and lse.  The probabilities are recomputed; every sum has a fixed order.  dtable's fp32 form is as exact as the
+    bf16 operands o and do it is formed from, not more."""
+    a = _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
+    a.lddo, a.lddq, a.lddk, a.lddv = (_rows(t, n, B * S, H * 64) for t, n in ((do, "do"), (dq, "dq"), (dk, "dk"), (dv, "dv")))
+    _need((S + 64) * (do.stride(0) if B * S > 1 else 0) * 2 < 2 ** 31 - 1, "a head's slice of do must stay below 2 GiB")
+    if dtable is not None:
+        _need(table is not None, "dtable: there is no table")
+        _need(dtable.dtype in (BF16, torch.float32) and dtable.shape == table.shape and dtable.is_contiguous(), f"dtable: expected a contiguous bf16 or fp32 {tuple(table.shape)}")
+    _on_device(q=q, k=k, v=v, table=table, o=o, lse=lse, do=do, dq=dq, dk=dk, dv=dv, dtable=dtable, key_mask=key_mask)
+    if B * S == 0:
+        if dtable is not None and not accumulate:
+            host_call(lambda: dtable.zero_())
+        return
+    _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask)
+    ws = _scratch(_capi.lib().aitk_attn_relpos_bwd_workspace_bytes(B, H, S, a.num_buckets if dtable is not None else 0), q.device)
+    a.dO, a.dQ, a.dK, a.dV, a.dtable, a.ws = _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), _ptr(ws)
+    a.dtable_f32, a.accumulate = int(dtable is not None and dtable.dtype == torch.float32), int(accumulate)
+    _call("aitk_attn_relpos_bwd", C.byref(a))

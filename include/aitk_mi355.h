@@ -588,6 +588,59 @@ typedef struct AitkDdpmNoiseArgs {
 } AitkDdpmNoiseArgs;
 int aitk_ddpm_noise_nhwc(const AitkDdpmNoiseArgs* args, aitk_stream_t stream);
 
+/* ---- text-encoder block: norms with a learned weight.  The encoders run through `transformers` on the reference's side (toolkit/train_tools.py:234-574); these are the
+ * operators a native encoder layer, or a trainer that also trains the norms, calls.
+ * y = xh * weight (+ bias), xh = (x - mean) * rstd (layer norm) or x * rstd (rms != 0: no mean, no bias); weight / bias [C] bf16, or fp32 with w_f32.
+ * mean / rstd (fp32 [M], may be NULL; mean only for layer norm) are what the backward needs.  C % 8 == 0, C <= 8192, row pitches % 8 == 0, 16-byte aligned. y may be x. */
+typedef struct AitkNormArgs {
+  const aitk_bf16* x; int64_t ldx;
+  const void* weight; const void* bias; /* bias may be NULL */
+  aitk_bf16* y; int64_t ldy;
+  float* mean; float* rstd;
+  float eps; int32_t rms, w_f32, M, C, _pad;
+} AitkNormArgs;
+int aitk_norm_fwd(const AitkNormArgs* args, aitk_stream_t stream);
+/* dx = d/dx of the above . dy (+ dres; dx may be dy, x or dres); dweight / dbias (fp32 [C], either may be NULL) = the column sums of dy * xh / dy, added to what is
+ * there with accumulate != 0.  partial: aitk_norm_bwd_workspace_bytes bytes, only read when a gradient is asked for.  Deterministic: no atomics. */
+typedef struct AitkNormBwdArgs {
+  const aitk_bf16* dy; int64_t ld_dy;
+  const aitk_bf16* x; int64_t ldx;
+  const void* weight;
+  const float* mean; const float* rstd;
+  const aitk_bf16* dres; int64_t ld_dres;
+  aitk_bf16* dx; int64_t ld_dx;
+  float* dweight; float* dbias;
+  float* partial;
+  int32_t rms, w_f32, accumulate, M, C, _pad;
+} AitkNormBwdArgs;
+int64_t aitk_norm_bwd_workspace_bytes(int32_t M, int32_t C, int32_t rms);
+int aitk_norm_bwd(const AitkNormBwdArgs* args, aitk_stream_t stream);
+
+/* Attention of the text encoders: 64-wide heads, self-attention over S positions, o = softmax(scale q.k + table[bucket(k - q)][head]) v over the keys that key_mask
+ * (uint8 / bool [B, S], non-zero = attend; NULL = all) and, causal != 0, k <= q leave.  Q, K, V, O, ... are [B*S, >= H*64] views with head h at column 64 h.
+ * table: bf16 [num_buckets, H] (T5's relative_attention_bias.weight), NULL = no bias (CLIP).  Buckets: of each sign's `half` (num_buckets / 2, the second half for keys
+ * ahead of the query; causal: all num_buckets for the past) the first half / 2 are one distance each, the others split the logarithm up to max_distance, the last takes
+ * the rest; 2 <= half <= 64, half / 2 < max_distance <= 1024.  LSE [B, H, S] fp32 is in the scaled log2 domain like AitkAttnArgs.LSE.
+ * A row without any key gives o = 0, lse = -inf and zero gradients; what masked keys hold (NaN and infinities too) reaches nothing.
+ * Backward writes dQ, dK, dV and, if dtable is set, [num_buckets, H] bucket sums (bf16, or fp32 with dtable_f32; added to what is there with accumulate): the bias's gradient,
+ * summed in fp32 in a fixed order.  Deterministic.  ws: aitk_attn_relpos_bwd_workspace_bytes bytes (num_buckets 0 without dtable).
+ * A head's slice stays below 2 GiB ((S + 64) * row pitch * 2 bytes); pitches % 8 == 0, 16-byte aligned. */
+typedef struct AitkAttnRelposArgs {
+  const aitk_bf16* Q; const aitk_bf16* K; const aitk_bf16* V; int64_t ldq, ldk, ldv;
+  aitk_bf16* O; int64_t ldo;
+  float* LSE;
+  const aitk_bf16* table; const uint8_t* key_mask;
+  const aitk_bf16* dO; int64_t lddo;
+  aitk_bf16* dQ; aitk_bf16* dK; aitk_bf16* dV; int64_t lddq, lddk, lddv;
+  void* dtable; float* ws;
+  float scale; int32_t B, H, S, num_buckets, max_distance, causal, dtable_f32, accumulate, _pad;
+} AitkAttnRelposArgs;
+int aitk_attn_relpos_fwd(const AitkAttnRelposArgs* args, aitk_stream_t stream);
+int64_t aitk_attn_relpos_bwd_workspace_bytes(int32_t B, int32_t H, int32_t S, int32_t num_buckets);
+int aitk_attn_relpos_bwd(const AitkAttnRelposArgs* args, aitk_stream_t stream);
+/* host only: first[j] = the first distance of bucket j within one sign (64 entries of room) -> half, or AITK_ERR_SHAPE for a bucketing that is not supported */
+int aitk_attn_relpos_buckets(int32_t num_buckets, int32_t max_distance, int32_t causal, int32_t* first);
+
 /* ---- hardware probes (test infrastructure for layout assumptions; not on the product path) ---- */
 /* host-side evaluation of the attention kernels' workgroup -> (row tile, head, batch) map for a 1-D grid of n blocks (XCD-grouped order) */
 int aitk_probe_attn_wg_coords(int32_t n, int32_t id, int32_t ntiles, int32_t H, int32_t* out3);

@@ -1,0 +1,227 @@
+"""aitk_attn_relpos_fwd / _bwd (attention with a learned relative position bias) on the MI355X against a plain 64-bit computation, within bounds that count the kernels'
+roundings (tests/relpos_ref.py): lengths from one token to several thousand around every tile border, key masks that leave rows empty or hold NaN and infinities, causal
+order, bucketings, fused and padded layouts, accumulation, determinism, another stream, replayed graphs."""
+import pytest
+import torch
+
+from tests import relpos_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _inputs(B, H, S, *, scale=1.0, layout="fused", seed=0, buckets=32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def rnd(*shape, std=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * std).to(BF16)
+
+    std = 0.35 * scale ** -0.5
+    C = H * 64
+    if layout == "fused":  # column blocks of one projection's output
+        buf = torch.cat([rnd(B * S, C, std=std), rnd(B * S, C, std=std), rnd(B * S, C)], 1)
+        q, k, v = buf[:, :C], buf[:, C:2 * C], buf[:, 2 * C:]
+        grads = torch.zeros(B * S, 3 * C, dtype=BF16, device="cuda")
+        dq, dk, dv = grads[:, :C], grads[:, C:2 * C], grads[:, 2 * C:]
+        o, do = torch.zeros(B * S, C, dtype=BF16, device="cuda"), rnd(B * S, C)
+    else:  # every operand its own row pitch
+        q, k, v = rnd(B * S, C + 8, std=std)[:, :C], rnd(B * S, C + 24, std=std)[:, 8:8 + C], rnd(B * S, C + 16)[:, 16:]
+        dq, dk, dv, o = (torch.zeros(B * S, C + 8 * i, dtype=BF16, device="cuda")[:, :C] for i in (1, 2, 3, 4))
+        do = rnd(B * S, C + 8)[:, :C]
+    table = rnd(buckets, H, std=0.7)
+    return q, k, v, table, o, do, dq, dk, dv
+
+
+def _mask(kind, B, S, seed=0):
+    if kind is None:
+        return None
+    g = torch.Generator(device="cuda").manual_seed(100 + seed)
+    m = torch.zeros(B, S, dtype=torch.bool, device="cuda")
+    for b in range(B):
+        if kind == "prefix":  # the first sample keeps nothing, the last everything
+            m[b, :S * b // max(1, B - 1)] = True
+        elif kind == "holes":
+            m[b] = torch.rand(S, generator=g, device="cuda") < 0.5
+        elif kind == "tail":  # left padding: whole tiles at the front are masked
+            m[b, S - 1 - (S // 3) * (b % 3):] = True
+    return m
+
+
+def _near(got, want, tol, name):
+    d = (got.double() - want).abs()
+    assert torch.isfinite(got).all(), name
+    over = d - tol
+    assert (over <= 0).all(), f"{name}: {int((over > 0).sum())} of {d.numel()} elements over their bound, worst by {float(over.max()):.3g} (error {float(d.max()):.3g})"
+
+
+def _run(B, H, S, *, bias=True, causal=False, mask=None, scale=1.0, layout="fused", buckets=32, max_distance=128, seed=0, poison=False, table_grad=torch.float32, train=True):
+    from ai_toolkit_amd import ops
+
+    q, k, v, table, o, do, dq, dk, dv = _inputs(B, H, S, scale=scale, layout=layout, seed=seed, buckets=buckets)
+    table = table if bias else None
+    m = _mask(mask, B, S, seed)
+    if poison:  # what masked positions hold: NaN, infinities and the type's lowest value
+        dead = (~m).view(-1)
+        junk = torch.tensor([float("nan"), float("inf"), float("-inf"), torch.finfo(BF16).min], dtype=BF16, device="cuda")
+        rows = torch.arange(B * S, device="cuda")
+        for t in (k, v):
+            t[dead] = junk[rows[dead] % 4][:, None].expand(-1, t.shape[1])
+    kw = dict(B=B, H=H, S=S, scale=scale, key_mask=m, max_distance=max_distance, causal=causal)
+    want = ref.attention(q, k, v, table, do=do if train else None, **kw)
+    lse = torch.zeros(B, H, S, dtype=torch.float32, device="cuda")
+    ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+    torch.cuda.synchronize()
+    _near(o, want["o"], want["tol_o"], "o")
+    empty = torch.isinf(want["lse"])
+    assert torch.equal(torch.isinf(lse) & (lse < 0), empty)
+    assert ((lse.double() - want["lse"]).masked_fill(empty, 0).abs() <= 2.0 ** -16 * (1 + want["lse"].masked_fill(empty, 0).abs())).all()
+    if not train:
+        return
+    dtable = torch.full_like(table, 7.0, dtype=table_grad) if bias else None
+    ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable, **kw)
+    torch.cuda.synchronize()
+    for name, t in (("dv", dv), ("dq", dq), ("dk", dk)):
+        _near(t, want[name], want["tol_" + name], name)
+    if bias:
+        extra = ref.U * want["dtable"].abs() if table_grad == BF16 else 0.0
+        _near(dtable, want["dtable"], want["tol_dtable"] * (1 + ref.U) + extra + 1e-30, "dtable")
+
+
+@pytest.mark.parametrize("S", [1, 2, 31, 32, 33, 63, 64, 65, 77, 91, 127, 128, 129, 200, 333])
+@pytest.mark.parametrize("causal", [False, True])
+def test_lengths_around_the_tile_borders(S, causal):
+    _run(2, 3, S, causal=causal, seed=S)
+
+
+@pytest.mark.parametrize("kind", ["prefix", "holes", "tail"])
+@pytest.mark.parametrize("S", [5, 64, 130, 333])
+@pytest.mark.parametrize("causal", [False, True])
+def test_key_masks(kind, S, causal):
+    _run(3, 2, S, mask=kind, causal=causal, seed=S)
+
+
+@pytest.mark.parametrize("kind", ["prefix", "holes", "tail"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_what_masked_keys_hold_reaches_nothing(kind, bias):
+    _run(3, 2, 200, mask=kind, bias=bias, poison=True)
+
+
+@pytest.mark.parametrize("buckets,max_distance,causal", [(16, 64, False), (64, 256, False), (8, 16, False), (4, 3, False), (128, 1024, False), (32, 128, True), (64, 300, True), (2, 5, True)])
+def test_bucketings(buckets, max_distance, causal):
+    _run(1, 2, 700, buckets=buckets, max_distance=max_distance, causal=causal)
+
+
+@pytest.mark.parametrize("bias,causal,scale", [(False, True, 0.125), (False, False, 0.125), (True, False, 0.125), (True, True, 0.3)])
+def test_without_bias_and_with_a_scale(bias, causal, scale):
+    _run(2, 4, 150, bias=bias, causal=causal, scale=scale, layout="pitched")
+
+
+def test_pitched_layout_leaves_the_gaps_alone():
+    _run(2, 3, 130, layout="pitched", mask="holes")
+
+
+def test_table_gradient_in_bf16():
+    _run(2, 4, 257, table_grad=BF16)
+
+
+@pytest.mark.parametrize("mask", [None, "tail", "prefix"])
+def test_more_than_one_group_of_key_tiles(mask):
+    """over 4096 keys: the tile masks come in groups of 64; left padding masks whole tiles of the first group"""
+    _run(2, 1, 4200, mask=mask, train=mask != "prefix")
+
+
+def test_large_encoder_shape():
+    _run(2, 64, 512, mask="prefix", seed=3)
+
+
+def test_accumulates_into_a_shared_table_and_repeats_bit_for_bit():
+    from ai_toolkit_amd import ops
+
+    B, H, S = 2, 4, 300
+    q, k, v, table, o, do, dq, dk, dv = _inputs(B, H, S)
+    lse = torch.zeros(B, H, S, dtype=torch.float32, device="cuda")
+    kw = dict(B=B, H=H, S=S, key_mask=_mask("holes", B, S))
+    ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+    one = torch.empty(32, H, device="cuda")
+    ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, one, **kw)
+    first = [t.clone() for t in (o, dq, dk, dv, one)]
+    two = one.clone()
+    ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, two, accumulate=True, **kw)
+    assert torch.equal(two, one + one)
+    for _ in range(5):
+        ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+        ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, one, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(first, (o, dq, dk, dv, one)))
+
+
+def test_gradients_against_differences():
+    """a loss sum(o dO) moved along random directions of q, k, v and the table: central differences of the 64-bit definition against the kernels' gradients.  The step's own
+    error is far below the bound of the contraction, which is the sum of the elements' bounds."""
+    from ai_toolkit_amd import ops
+
+    B, H, S = 1, 2, 90
+    q, k, v, table, o, do, dq, dk, dv = _inputs(B, H, S, layout="pitched")
+    kw = dict(B=B, H=H, S=S, scale=0.5, key_mask=_mask("holes", B, S), max_distance=64, causal=False)
+    lse = torch.zeros(B, H, S, dtype=torch.float32, device="cuda")
+    ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+    dtable = torch.empty(32, H, device="cuda")
+    ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable, **kw)
+    want = ref.attention(q, k, v, table, do=do, **kw)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    base = {"q": q.double(), "k": k.double(), "v": v.double(), "table": table.double()}
+    for name, got in (("q", dq), ("k", dk), ("v", dv), ("table", dtable)):
+        d = torch.randn(base[name].shape, generator=g, device="cuda", dtype=torch.float64)
+
+        def loss(h):
+            x = dict(base)
+            x[name] = x[name] + h * d
+            return float((ref.attention(x["q"], x["k"], x["v"], x["table"], **kw)["o"] * do.double()).sum())
+
+        h = 1e-5
+        slope = (loss(h) - loss(-h)) / (2 * h)
+        bound = float((want["tol_d" + name] * d.abs()).sum())
+        assert abs(float((got.double() * d).sum()) - slope) <= bound + 1e-6 * abs(slope), name
+
+
+def test_on_another_stream_and_in_replayed_graphs():
+    from ai_toolkit_amd import ops
+
+    B, H, S = 2, 3, 140
+    sets = [_inputs(B, H, S, seed=s) for s in (1, 2)]
+    kw = dict(B=B, H=H, S=S, key_mask=_mask("holes", B, S))
+
+    def step(x, lse, dtable):
+        q, k, v, table, o, do, dq, dk, dv = x
+        ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+        ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable, **kw)
+
+    lses = [torch.zeros(B, H, S, device="cuda") for _ in sets]
+    dts = [torch.zeros(32, H, device="cuda") for _ in sets]
+    for x, l, d in zip(sets, lses, dts):
+        step(x, l, d)
+    torch.cuda.synchronize()
+    want = [[t.clone() for t in (x[4], x[6], x[7], x[8], d)] for x, d in zip(sets, dts)]
+    side = torch.cuda.Stream()
+    graphs = []
+    with torch.cuda.stream(side):
+        for x, l, d in zip(sets, lses, dts):
+            for t in (x[4], x[6], x[7], x[8], d):
+                t.zero_()
+            step(x, l, d)
+        side.synchronize()
+        assert all(torch.equal(a, b) for x, d, w in zip(sets, dts, want) for a, b in zip((x[4], x[6], x[7], x[8], d), w))
+        for x, l, d in zip(sets, lses, dts):  # two graphs with scratch of their own
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=side):
+                step(x, l, d)
+            graphs.append(gr)
+    torch.cuda.synchronize()
+    for rep in range(4):
+        for x, d in zip(sets, dts):
+            for t in (x[4], x[6], x[7], x[8], d):
+                t.fill_(rep)
+        for gr in graphs if rep % 2 else graphs[::-1]:
+            gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, d, w in zip(sets, dts, want) for a, b in zip((x[4], x[6], x[7], x[8], d), w)), rep
+        step(sets[0], lses[0], dts[0])  # eager work between the replays

@@ -1,0 +1,135 @@
+"""aitk_norm_fwd / _bwd (layer norm and RMS norm with a learned weight, the weight's and bias's gradients) on the MI355X against plain 64-bit formulas.
+
+Bounds: every bf16 result is rounded once (2^-8 relative).  fp32 arithmetic: sums over C <= 8192 columns or over the rows of one thread and the tree above them are off by
+less than 2^-14 of the sum of the terms' absolute values (at most a few hundred sequential additions, 2^-24 each), everything else by a few 2^-24."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+U, FP = 2.0 ** -8, 2.0 ** -14
+
+
+def _ref(x, w, b, dy, dres, rms, eps):
+    x, w, dy = x.double(), w.double(), dy.double()
+    mean = torch.zeros_like(x[:, :1]) if rms else x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    xh = (x - mean) * rstd
+    size = (x.abs() + mean.abs()) * rstd  # what xh is computed from
+    y = xh * w + (0 if b is None else b.double())
+    tol_y = U * y.abs() + FP * (size * w.abs() + (0 if b is None else b.double().abs())) + 1e-30
+    g = dy * w
+    c1 = torch.zeros_like(mean) if rms else g.mean(1, keepdim=True)
+    c2 = (g * xh).mean(1, keepdim=True)
+    dx = rstd * (g - c1 - xh * c2)
+    size_dx = rstd * (g.abs() + g.abs().mean(1, keepdim=True) + size * (g.abs() * size).mean(1, keepdim=True))
+    if dres is not None:
+        dx = dx + dres.double()
+        size_dx = size_dx + dres.double().abs()
+    dw, db = (dy * xh).sum(0), dy.sum(0)
+    return dict(y=(y, tol_y), dx=(dx, U * dx.abs() + FP * size_dx + 1e-30), dw=(dw, FP * (dy.abs() * size).sum(0) + 1e-30), db=(db, FP * dy.abs().sum(0) + 1e-30),
+                mean=(mean[:, 0], FP * x.abs().mean(1) + 1e-30), rstd=(rstd[:, 0], FP * rstd[:, 0]))
+
+
+def _near(got, want, name):
+    d = (got.double() - want[0]).abs()
+    assert torch.isfinite(got).all(), name
+    assert (d <= want[1]).all(), f"{name}: worst over its bound by {float((d - want[1]).max()):.3g}"
+
+
+def _case(M, C, rms, *, wdtype=BF16, bias=True, dres=False, pitch=0, eps=1e-6, seed=0, offset=0.0):
+    from ai_toolkit_amd import ops
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    wide = lambda t: torch.cat([t, t[:, :pitch]], 1)[:, :C] if pitch else t  # noqa: E731
+    x = wide((rnd(M, C) * (0.5 + torch.rand(C, generator=g, device="cuda")) + offset).to(BF16))
+    w = (1 + 0.3 * rnd(C)).to(wdtype)
+    b = rnd(C).to(wdtype) if bias and not rms else None
+    dy, dr = wide(rnd(M, C).to(BF16)), rnd(M, C).to(BF16) if dres else None
+    y, dx = wide(torch.zeros(M, C, dtype=BF16, device="cuda")), wide(torch.zeros(M, C, dtype=BF16, device="cuda"))
+    mean, rstd = None if rms else torch.zeros(M, device="cuda"), torch.zeros(M, device="cuda")
+    dw, db = torch.full((C,), 3.0, device="cuda"), None if rms else torch.full((C,), 3.0, device="cuda")
+    want = _ref(x, w, b, dy, dr, rms, eps)
+    ops.norm_fwd(x, w, y, bias=b, rms=rms, mean=mean, rstd=rstd, eps=eps)
+    ops.norm_bwd(dy, x, w, rstd, dx, mean=mean, rms=rms, dres=dr, dweight=dw, dbias=db)
+    torch.cuda.synchronize()
+    _near(y, want["y"], "y")
+    _near(rstd, want["rstd"], "rstd")
+    _near(dx, want["dx"], "dx")
+    _near(dw, want["dw"], "dweight")
+    if not rms:
+        _near(mean, want["mean"], "mean")
+        _near(db, want["db"], "dbias")
+    return x, w, b, dy, dr, y, dx, mean, rstd, dw, db
+
+
+@pytest.mark.parametrize("C", [8, 64, 128, 136, 256, 264, 512, 520, 768, 1000, 1024, 1280, 1536, 1544, 2048, 2056, 4096, 4104, 8192])
+@pytest.mark.parametrize("rms", [False, True])
+def test_widths(C, rms):
+    _case(37, C, rms, dres=C % 16 == 0, seed=C)
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 7, 31, 33, 257, 1025, 5000])
+@pytest.mark.parametrize("C", [64, 768, 4096])
+@pytest.mark.parametrize("rms", [False, True])
+def test_row_counts(M, C, rms):
+    _case(M, C, rms, dres=M % 2 == 0, seed=M)
+
+
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("wdtype", [BF16, torch.float32])
+def test_weight_types_pitches_and_offsets(rms, wdtype):
+    _case(65, 640, rms, wdtype=wdtype, pitch=24, dres=True)
+    _case(65, 640, rms, wdtype=wdtype, bias=False, offset=20.0)  # a mean far from zero
+    _case(65, 2560, rms, wdtype=wdtype, eps=1e-5, pitch=8)
+
+
+def test_results_may_overwrite_operands():
+    from ai_toolkit_amd import ops
+
+    x, w, b, dy, dr, y, dx, mean, rstd, dw, db = _case(50, 1280, False, dres=True)
+    x2 = x.clone()
+    ops.norm_fwd(x2, w, x2, bias=b)
+    assert torch.equal(x2, y)
+    for target in ("dy", "x", "dres"):
+        t = {"dy": dy.clone(), "x": x.clone(), "dres": dr.clone()}
+        ops.norm_bwd(t["dy"], t["x"], w, rstd, t[target], mean=mean, dres=t["dres"])
+        assert torch.equal(t[target], dx), target
+
+
+def test_accumulates_and_repeats_bit_for_bit():
+    from ai_toolkit_amd import ops
+
+    x, w, b, dy, dr, y, dx, mean, rstd, dw, db = _case(3001, 768, False)
+    dw2, db2 = dw.clone(), db.clone()
+    ops.norm_bwd(dy, x, w, rstd, dx, mean=mean, dweight=dw2, dbias=db2, accumulate=True)
+    assert torch.equal(dw2, dw + dw) and torch.equal(db2, db + db)
+    only = torch.zeros_like(dw)  # one of the two alone
+    for _ in range(5):
+        ops.norm_bwd(dy, x, w, rstd, dx, mean=mean, dbias=only)
+        assert torch.equal(only, db)
+
+
+def test_no_rows():
+    from ai_toolkit_amd import ops
+
+    e = torch.empty(0, 64, dtype=BF16, device="cuda")
+    s = torch.empty(0, device="cuda")
+    dw = torch.ones(64, device="cuda")
+    ops.norm_fwd(e, torch.ones(64, dtype=BF16, device="cuda"), e, rms=True, rstd=s)
+    ops.norm_bwd(e, e, torch.ones(64, dtype=BF16, device="cuda"), s, e, rms=True, dweight=dw, accumulate=True)
+    assert bool((dw == 1).all())
+    ops.norm_bwd(e, e, torch.ones(64, dtype=BF16, device="cuda"), s, e, rms=True, dweight=dw)
+    assert bool((dw == 0).all())
+
+
+def test_a_row_that_is_not_finite_stays_in_its_row():
+    from ai_toolkit_amd import ops
+
+    x = torch.randn(9, 256, device="cuda").to(BF16)
+    x[4, 7] = float("inf")
+    y = torch.zeros_like(x)
+    ops.norm_fwd(x, torch.ones(256, dtype=BF16, device="cuda"), y)
+    bad = ~torch.isfinite(y).all(1)
+    assert bad.tolist() == [i == 4 for i in range(9)]
