@@ -24,6 +24,7 @@ typedef int v4i_t __attribute__((ext_vector_type(4)));
 
 constexpr int TILE = 8192;          // bytes of a [64][64] bf16 tile
 constexpr int BAND_PAD = 96;        // a wave's 32 rows x 64 columns span 95 distances
+constexpr int SKEW_P = 68;          // floats per row of a skewed 32 x 32 block (63 diagonals + 3 of slack)
 constexpr int MAX_HALF = 64;        // buckets of one sign
 constexpr float M_NONE = -3.0e38f;  // running maximum of a row that has met no key yet (finite: differences with it are never NaN)
 constexpr float DEFER = 8.0f;       // the accumulators are rescaled only when a row's maximum grew by more than 2^8 (p stays below 2^8: exact in fp32 sums)
@@ -163,28 +164,31 @@ __device__ __forceinline__ void wg_coords(int ntiles, int H, int& tile, int& hd,
 }
 
 // ============================================================================================ forward
-// 4 waves x 32 query rows, key tiles of 64 in a double buffer.  S^T = K Q^T: a lane owns one query row, so the statistics are per-lane scalars and P^T feeds the next
-// product straight from the registers.
-template <bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256, 3) void attn_relpos_fwd_kernel(RelposArgs r) {
+// 4 waves, key tiles of 64 in a double buffer.  S^T = K Q^T: a lane owns one query row, so the statistics are per-lane scalars and P^T feeds the next product straight from
+// the registers.  KVS = 1: 128 query rows, every wave walks all key tiles.  KVS = 2: 64 query rows, two waves share 32 of them and take every other key tile; their
+// (maximum, sum, output) meet in LDS at the end.  For launches of at most one 128-row workgroup per CU: twice the workgroups, half the steps (1 x 64 heads x 512: 18.0 -> 15.7 us,
+3 x 6 x 333: 13.7 -> 11.3 us; with two workgroups per CU it loses: 1 x 32 x 2048 61.7 -> 71.5 us).
+template <bool BIAS, bool CAUSAL, int KVS>
+__global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const AitkAttnRelposArgs& a = r.a;
-  lds_char* const sm = (lds_char*)smem;                                                      // 2 x (K tile, V tile)
-  unsigned long long* const box = reinterpret_cast<unsigned long long*>(smem + 4 * TILE);    // 64 tile masks
-  lds_float* const line = (lds_float*)(smem + 4 * TILE + 512);
+  constexpr int ROWS = 128 / KVS, STEP = 2 * KVS * TILE;  // query rows of a workgroup; bytes of one stage (KVS x (K tile, V tile))
+  lds_char* const sm = (lds_char*)smem;
+  unsigned long long* const box = reinterpret_cast<unsigned long long*>(smem + 2 * STEP);  // 64 tile masks
+  lds_float* const line = (lds_float*)(smem + 2 * STEP + 512);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5, S = a.S;
+  const int qg = wave / KVS, part = wave % KVS;
   int tile_x, hd, b;
-  wg_coords((S + 127) / 128, a.H, tile_x, hd, b);
-  const int q0 = tile_x * 128 + wave * 32;
-  const bf16_t* Qb = a.Q + (long)b * S * a.ldq + hd * 64;
+  wg_coords((S + ROWS - 1) / ROWS, a.H, tile_x, hd, b);
+  const int q0 = tile_x * ROWS + qg * 32;
   const v4i_t srdK = make_srd(a.K + (long)b * S * a.ldk + hd * 64, ((long)(S - 1) * a.ldk + 64) * 2);
   const v4i_t srdV = make_srd(a.V + (long)b * S * a.ldv + hd * 64, ((long)(S - 1) * a.ldv + 64) * 2);
   TileLane L;
   L.init(lane, wave);
   s16x8_t qf[4];
   {
-    const bf16_t* qp = Qb + (long)min(q0 + l31, S - 1) * a.ldq + 8 * h;
+    const bf16_t* qp = a.Q + ((long)b * S + min(q0 + l31, S - 1)) * a.ldq + hd * 64 + 8 * h;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) qf[ks] = *reinterpret_cast<const s16x8_t*>(qp + 16 * ks);
   }
@@ -192,38 +196,51 @@ __global__ __launch_bounds__(256, 3) void attn_relpos_fwd_kernel(RelposArgs r) {
   float far_past = 0.f, far_ahead = 0.f;  // the bias of the last bucket of either sign, in the log2 domain
   const int E = r.sat + BAND_PAD;
   const int ib = E + 4 * h - q0 - l31;  // line index of key 0 of this lane's first register
-  if constexpr (BIAS) {
-    build_line(line, r, hd, 1);
-    far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
-    far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
-    __syncthreads();
-  }
   f32x16_t o[2] = {zero16(), zero16()};
   float m_run = M_NONE, l_run = 0.f;
-  const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * 128 + 127) / 64 + 1) : (S + 63) / 64;
+  const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * ROWS + ROWS - 1) / 64 + 1) : (S + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += 64) {
     const unsigned long long masks = tile_masks(a, b, t0, ntiles, box, lane, wave);
     unsigned long long todo = __ballot(masks != 0);
-    if (!todo) continue;
-    int t = __builtin_ctzll(todo), cur = 0;
-    unsigned long long keep = lane64(masks, t);
-    stage(sm, L, a.ldk, (t0 + t) * 64, srdK, wave, keep);
-    stage(sm + TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, keep);
+    // the next KVS tiles of the group into one stage; this wave's own tile and its keep-bits (0: nothing for it in this step)
+    auto fetch = [&](lds_char* dst, int& mine, unsigned long long& keep) {
+      mine = 0;
+      keep = 0;
+#pragma unroll
+      for (int i = 0; i < KVS; ++i) {
+        if (todo) {
+          const int t = __builtin_ctzll(todo);
+          const unsigned long long k = lane64(masks, t);
+          stage(dst + 2 * i * TILE, L, a.ldk, (t0 + t) * 64, srdK, wave, k);
+          stage(dst + (2 * i + 1) * TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, k);
+          if (KVS == 1 || part == i) {
+            mine = t;
+            keep = k;
+          }
+          todo &= todo - 1;
+        }
+      }
+    };
+    int t, cur = 0;
+    unsigned long long keep;
+    bool more = todo != 0;
+    if (more) fetch(sm, t, keep);
+    if (BIAS && t0 == 0) {  // with the first tiles on their way
+      build_line(line, r, hd, 1);
+      far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
+      far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
+    }
     dma_wait_all();
     __syncthreads();
-    while (true) {
-      todo &= todo - 1;
-      const int tn = todo ? __builtin_ctzll(todo) : 0;
-      const unsigned long long keep_n = lane64(masks, tn);
-      if (todo) {
-        lds_char* nx = sm + (cur ^ 1) * 2 * TILE;
-        stage(nx, L, a.ldk, (t0 + tn) * 64, srdK, wave, keep_n);
-        stage(nx + TILE, L, a.ldv, (t0 + tn) * 64, srdV, wave, keep_n);
-      }
-      const lds_char* kt = sm + cur * 2 * TILE;
+    while (more) {
+      more = todo != 0;
+      int tn = 0;
+      unsigned long long keep_n = 0;
+      if (more) fetch(sm + (cur ^ 1) * STEP, tn, keep_n);
+      const lds_char* kt = sm + cur * STEP + part * 2 * TILE;
       const lds_char* vt = kt + TILE;
       const int kv0 = (t0 + t) * 64;
-      if (!CAUSAL || kv0 <= q0 + 31) {
+      if (keep && (!CAUSAL || kv0 <= q0 + 31)) {
         float tb = 0.f;
         bool near = false;
         if constexpr (BIAS) {
@@ -305,13 +322,35 @@ __global__ __launch_bounds__(256, 3) void attn_relpos_fwd_kernel(RelposArgs r) {
       }
       dma_wait_all();
       __syncthreads();
-      if (!todo) break;
       t = tn;
       keep = keep_n;
       cur ^= 1;
     }
   }
-  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  if constexpr (KVS == 2) {
+    lds_float* const mine = (lds_float*)smem + qg * (34 * 64) + lane;  // the tiles are done with: every loop ends behind a barrier
+    if (part) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        mine[e * 64] = o[0][e];
+        mine[(16 + e) * 64] = o[1][e];
+      }
+      mine[32 * 64] = m_run;
+      mine[33 * 64] = l_tot;
+    }
+    __syncthreads();
+    if (part) return;
+    const float m2 = mine[32 * 64], l2 = mine[33 * 64];
+    const float m = fmaxf(m_run, m2), a1 = __builtin_amdgcn_exp2f(m_run - m), a2 = __builtin_amdgcn_exp2f(m2 - m);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      o[0][e] = o[0][e] * a1 + mine[e * 64] * a2;
+      o[1][e] = o[1][e] * a1 + mine[(16 + e) * 64] * a2;
+    }
+    l_tot = l_tot * a1 + l2 * a2;
+    m_run = m;
+  }
   const float inv = l_tot > 0.f ? 1.0f / l_tot : l_tot != l_tot ? l_tot : 0.f;
   const int q = q0 + l31;
   if (q < S) {
@@ -380,9 +419,12 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   const float c2 = a.scale * 1.4426950408889634f;
   const int E = r.sat + BAND_PAD, n_line = 2 * E + 1;
   const bool sums = BIAS && a.dtable != nullptr;
-  // bucket sums: every half wave adds its ds to accumulators of its own, one per distance (no two lanes of an instruction meet in one address, and one address sees its
-  // terms in program order: the sums do not depend on timing)
-  lds_float* const acc = line + 4 * r.line_p + (2 * wave + h) * n_line;
+  // Bucket sums.  A 32 x 32 block's diagonals (one relative position each) become columns of a wave-private LDS patch: row q is written q places to the left (with up to
+  // three places of slack so that its 16-byte stores are aligned; what a row never writes stays zero), a lane then adds up one column and joins it to the wave's
+  // accumulator of that distance.  Fixed order, no atomics (an LDS float add per element: 330 us for 4 x 64 heads x 512 against 137 us).
+  lds_float* const acc = line + 4 * r.line_p + wave * n_line;
+  lds_float* const skew = line + 4 * r.line_p + (4 * n_line + 3) / 4 * 4 + wave * (32 * SKEW_P);
+  lds_float* const skew_w = skew + l31 * SKEW_P + 31 - l31 + ((l31 + 1) & 3) + 4 * h;
   float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f;
   const int ib = E + 4 * h - q0 - l31;
   if constexpr (BIAS) {
@@ -390,7 +432,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
     far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
     far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
     if (sums)
-      for (int i = tid; i < 8 * n_line; i += 256) (line + 4 * r.line_p)[i] = 0.f;
+      for (int i = tid; i < (4 * n_line + 3) / 4 * 4 + 4 * 32 * SKEW_P; i += 256) (line + 4 * r.line_p)[i] = 0.f;
     __syncthreads();
   }
   f32x16_t dq[2] = {zero16(), zero16()};
@@ -462,8 +504,14 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
           if (sums) {
             if (side == 0) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                __hip_atomic_fetch_add(acc + i0 + 32 * j + (e & 3) + 8 * (e >> 2), s[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+              for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(skew_w + 8 * g) = f32x4_t{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' stores: LDS keeps a wave's accesses in order
+              float v = 0.f;
+#pragma unroll
+              for (int q = 0; q < 32; ++q) v += skew[q * SKEW_P + ((q + 1) & 3) + lane];
+              acc[E + kv0 + 32 * j - q0 - 31 + lane] += v;
+              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             } else {
 #pragma unroll
               for (int e = 0; e < 16; ++e) fs += s[e];
@@ -515,7 +563,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       float v = 0.f;
       if (last) v = ahead ? fars[4] + fars[5] + fars[6] + fars[7] : fars[0] + fars[1] + fars[2] + fars[3];
       for (int n = n0 > 0 || !ahead ? n0 : 1; n < n1; ++n)
-        for (int w = 0; w < 8; ++w) v += all[w * n_line + E + (ahead ? n : -n)];
+        for (int w = 0; w < 4; ++w) v += all[w * n_line + E + (ahead ? n : -n)];
       r.part[(((long)b * ((S + 127) / 128) + tile_x) * a.H + hd) * a.num_buckets + tid] = v;
     }
   }
@@ -736,6 +784,17 @@ int launch(K kernel, unsigned grid, size_t lds, const RelposArgs& r, hipStream_t
   AITK_LAUNCH_CHECK();
   return AITK_OK;
 }
+
+constexpr int64_t KVS2_MOST = 256;  // workgroups of 128 rows (at most one per CU) up to which two waves share their rows
+
+template <int KVS>
+int launch_fwd(const RelposArgs& r, hipStream_t s) {
+  const AitkAttnRelposArgs& a = r.a;
+  const unsigned grid = (unsigned)((a.S + 128 / KVS - 1) / (128 / KVS)) * a.H * a.B;
+  const size_t lds = KVS * 4 * TILE + 512 + (size_t)4 * r.line_p * 4;
+  if (a.table) return a.causal ? launch(attn_relpos_fwd_kernel<true, true, KVS>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<true, false, KVS>, grid, lds, r, s);
+  return a.causal ? launch(attn_relpos_fwd_kernel<false, true, KVS>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<false, false, KVS>, grid, lds, r, s);
+}
 }  // namespace
 
 extern "C" int aitk_attn_relpos_buckets(int32_t num_buckets, int32_t max_distance, int32_t causal, int32_t* first) {
@@ -751,11 +810,8 @@ extern "C" int aitk_attn_relpos_fwd(const AitkAttnRelposArgs* a, aitk_stream_t s
   RelposArgs r;
   const int rc = check(a, false, r);
   if (rc != AITK_OK) return rc;
-  const unsigned grid = (unsigned)((a->S + 127) / 128) * a->H * a->B;
-  const size_t lds = 4 * TILE + 512 + (size_t)4 * r.line_p * 4;
   hipStream_t s = (hipStream_t)stream;
-  if (a->table) return a->causal ? launch(attn_relpos_fwd_kernel<true, true>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<true, false>, grid, lds, r, s);
-  return a->causal ? launch(attn_relpos_fwd_kernel<false, true>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<false, false>, grid, lds, r, s);
+  return (int64_t)((a->S + 127) / 128) * a->H * a->B <= KVS2_MOST ? launch_fwd<2>(r, s) : launch_fwd<1>(r, s);
 }
 
 extern "C" int64_t aitk_attn_relpos_bwd_workspace_bytes(int32_t B, int32_t H, int32_t S, int32_t num_buckets) {
@@ -773,7 +829,7 @@ extern "C" int aitk_attn_relpos_bwd(const AitkAttnRelposArgs* a, aitk_stream_t s
   hipLaunchKernelGGL(attn_relpos_delta_kernel, dim3((a->S + 31) / 32, a->H, a->B), dim3(256), 0, s, r);
   AITK_LAUNCH_CHECK();
   const unsigned grid = (unsigned)((a->S + 127) / 128) * a->H * a->B * 2;
-  const size_t lds = 4 * TILE + 1024 + (size_t)4 * r.line_p * 4 + (a->dtable ? (size_t)8 * (2 * (r.sat + BAND_PAD) + 1) * 4 : 0);
+  const size_t lds = 4 * TILE + 1024 + (size_t)4 * r.line_p * 4 + (a->dtable ? ((size_t)4 * (2 * (r.sat + BAND_PAD) + 1) + 3 + 4 * 32 * SKEW_P) * 4 : 0);
   if (a->table) rc = a->causal ? launch(attn_relpos_bwd_kernel<true, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<true, false>, grid, lds, r, s);
   else rc = a->causal ? launch(attn_relpos_bwd_kernel<false, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<false, false>, grid, lds, r, s);
   if (rc != AITK_OK) return rc;

@@ -1201,60 +1201,78 @@ def attn_small_bwd(q, k, v, o, lse, do, dq, dk, dv, *, B, H, S, D, scale, Skv=0)
 # Norms with a learned weight, attention with a learned relative position bias, the gated feed-forward projections.  Arguments that the kernels cannot take raise
 # ValueError before anything is launched; scratch is a torch allocation of the call (current stream's, and a capturing graph's own pool), never a buffer that two
 # streams or two captured graphs would share.
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
-
-
 def _rows(t, name, rows, cols):
     """bf16 [rows, cols] view with unit inner stride, a row pitch of whole 16-byte chunks and a 16-byte aligned start -> the row pitch"""
-    _need(t.dtype == BF16, f"{name}: expected bf16, got {t.dtype}")
-    _need(t.dim() == 2 and tuple(t.shape) == (rows, cols), f"{name}: expected [{rows}, {cols}], got {tuple(t.shape)}")
-    ld = t.stride(0) if rows > 1 else max(t.stride(0), -(-cols // 8) * 8)  # the pitch of a single row is nobody's
-    _need(cols == 1 or t.stride(1) == 1, f"{name}: the inner stride must be 1, got strides {t.stride()}")
-    _need(ld >= cols and ld % 8 == 0 and t.data_ptr() % 16 == 0, f"{name}: rows must be 16-byte aligned and must not overlap (strides {t.stride()})")
-    return ld
+    st = t.stride()
+    if t.dtype == BF16 and t.shape == (rows, cols) and (st[1] == 1 or cols == 1):
+        ld = st[0] if rows > 1 else max(st[0], (cols + 7) & -8)  # the pitch of a single row is nobody's
+        if ld >= cols and ld % 8 == 0 and t.data_ptr() % 16 == 0:
+            return ld
+    if t.dtype != BF16:
+        raise ValueError(f"{name}: expected bf16, got {t.dtype}")
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name}: expected [{rows}, {cols}], got {tuple(t.shape)}")
+    raise ValueError(f"{name}: rows must have unit inner stride, be 16-byte aligned and not overlap (strides {st}, address mod 16 = {t.data_ptr() % 16})")
 
 
 def _vec(t, name, n, dtypes):
-    _need(t.dtype in dtypes, f"{name}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    _need(t.dim() == 1 and t.numel() == n and t.is_contiguous(), f"{name}: expected a contiguous [{n}], got {tuple(t.shape)} strides {t.stride()}")
-    _need(t.data_ptr() % 16 == 0, f"{name}: must be 16-byte aligned")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.shape != (n,) or not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name}: expected a contiguous, 16-byte aligned [{n}], got {tuple(t.shape)} strides {t.stride()}")
 
 
 def _on_device(**tensors):
     """every operand lives on the current GPU: the launch goes to its current stream"""
+    cur = torch.cuda.current_device() if torch.cuda.is_available() else -2
     for name, t in tensors.items():
-        if t is not None:
-            _need(t.is_cuda, f"{name}: expected a tensor on the GPU, got {t.device}")
-            _need(t.device.index == torch.cuda.current_device(), f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        if t is not None and t.get_device() != cur:
+            raise ValueError(f"{name} is on {t.device}; the call launches on the current GPU" + (f", cuda:{cur}" if cur >= 0 else ", and there is none"))
+
+
+def _adr(t):
+    """device address for a pointer field (kept alive like _ptr while launches are recorded)"""
+    if t is None:
+        return None
+    if _REC is not None:
+        _REC.append(("_keepalive", (t,)))
+    return t.data_ptr()
 
 
 def _scratch(nbytes, device):
     return torch.empty(max(1, (nbytes + 3) // 4), dtype=torch.float32, device=device)
 
 
+def _norm_shape(x):
+    if x.dim() != 2 or x.shape[1] <= 0 or x.shape[1] % 8 or x.shape[1] > 8192:
+        raise ValueError(f"x: expected [M, C] with C a multiple of 8 up to 8192, got {tuple(x.shape)}")
+    return x.shape
+
+
+def _norm_stat(t, name, M):
+    if t is not None and (t.dtype != torch.float32 or t.shape != (M,) or not t.is_contiguous()):
+        raise ValueError(f"{name}: expected a contiguous fp32 [{M}], got {t.dtype} {tuple(t.shape)}")
+
+
 def norm_fwd(x, weight, y, *, bias=None, rms=False, mean=None, rstd=None, eps=1e-6):
     """y = xh * weight (+ bias) per row of x [M, C] bf16: xh = (x - mean) / sqrt(var + eps) (layer norm) or x / sqrt(mean(x^2) + eps) (rms: no mean, no bias).
     weight / bias [C] bf16 or fp32 (both the same); mean / rstd: fp32 [M], written for norm_bwd (mean: layer norm only).  y may be x.  C % 8 == 0, C <= 8192."""
-    _need(x.dim() == 2, f"x: expected [M, C], got {tuple(x.shape)}")
-    M, Cc = x.shape
-    _need(Cc > 0 and Cc % 8 == 0 and Cc <= 8192, f"x: C must be a multiple of 8 up to 8192, got {Cc}")
-    _need(eps >= 0, f"eps must not be negative, got {eps}")
+    M, Cc = _norm_shape(x)
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if rms and (bias is not None or mean is not None):
+        raise ValueError("an RMS norm has neither bias nor mean")
     a = _capi.NormArgs()
     a.ldx, a.ldy = _rows(x, "x", M, Cc), _rows(y, "y", M, Cc)
     _vec(weight, "weight", Cc, (BF16, torch.float32))
     if bias is not None:
-        _need(not rms, "bias: an RMS norm has none")
         _vec(bias, "bias", Cc, (weight.dtype,))
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t is not None:
-            _need(t.dtype == torch.float32 and t.dim() == 1 and t.numel() == M and t.is_contiguous(), f"{name}: expected a contiguous fp32 [{M}]")
-    _need(mean is None or not rms, "mean: an RMS norm has none")
+    _norm_stat(mean, "mean", M)
+    _norm_stat(rstd, "rstd", M)
     _on_device(x=x, weight=weight, y=y, bias=bias, mean=mean, rstd=rstd)
     if M == 0:
         return y
-    a.x, a.weight, a.bias, a.y, a.mean, a.rstd = _ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd)
+    a.x, a.weight, a.bias, a.y, a.mean, a.rstd = _adr(x), _adr(weight), _adr(bias), _adr(y), _adr(mean), _adr(rstd)
     a.eps, a.rms, a.w_f32, a.M, a.C = eps, int(rms), int(weight.dtype == torch.float32), M, Cc
     _call("aitk_norm_fwd", C.byref(a))
     return y
@@ -1263,19 +1281,18 @@ def norm_fwd(x, weight, y, *, bias=None, rms=False, mean=None, rstd=None, eps=1e
 def norm_bwd(dy, x, weight, rstd, dx, *, mean=None, rms=False, dres=None, dweight=None, dbias=None, accumulate=False):
     """dx = norm_fwd's gradient . dy (+ dres) from the saved rstd (and, layer norm, mean); dweight / dbias (fp32 [C], either may be left out) = the gradients of weight
     and bias, added to what they hold with `accumulate`.  dx may be dy, x or dres.  Deterministic."""
-    _need(x.dim() == 2, f"x: expected [M, C], got {tuple(x.shape)}")
-    M, Cc = x.shape
-    _need(Cc > 0 and Cc % 8 == 0 and Cc <= 8192, f"x: C must be a multiple of 8 up to 8192, got {Cc}")
+    M, Cc = _norm_shape(x)
+    if (mean is None) != bool(rms):
+        raise ValueError("mean: a layer norm needs the saved mean, an RMS norm has none")
+    if rms and dbias is not None:
+        raise ValueError("dbias: an RMS norm has no bias")
     a = _capi.NormBwdArgs()
     a.ld_dy, a.ldx, a.ld_dx = _rows(dy, "dy", M, Cc), _rows(x, "x", M, Cc), _rows(dx, "dx", M, Cc)
     if dres is not None:
         a.ld_dres = _rows(dres, "dres", M, Cc)
     _vec(weight, "weight", Cc, (BF16, torch.float32))
-    _need((mean is None) == bool(rms), "mean: a layer norm needs the saved mean, an RMS norm has none")
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t is not None:
-            _need(t.dtype == torch.float32 and t.dim() == 1 and t.numel() == M and t.is_contiguous(), f"{name}: expected a contiguous fp32 [{M}]")
-    _need(dbias is None or not rms, "dbias: an RMS norm has no bias")
+    _norm_stat(mean, "mean", M)
+    _norm_stat(rstd, "rstd", M)
     for t, name in ((dweight, "dweight"), (dbias, "dbias")):
         if t is not None:
             _vec(t, name, Cc, (torch.float32,))
@@ -1284,37 +1301,43 @@ def norm_bwd(dy, x, weight, rstd, dx, *, mean=None, rms=False, dres=None, dweigh
         if not accumulate:
             host_call(lambda: [t.zero_() for t in (dweight, dbias) if t is not None])
         return dx
+    part = None
     if dweight is not None or dbias is not None:
         part = _scratch(_capi.lib().aitk_norm_bwd_workspace_bytes(M, Cc, int(rms)), x.device)
-        a.partial = _ptr(part)
-    a.dy, a.x, a.weight, a.mean, a.rstd, a.dres, a.dx = _ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dres), _ptr(dx)
-    a.dweight, a.dbias = _ptr(dweight), _ptr(dbias)
+    a.dy, a.x, a.weight, a.mean, a.rstd, a.dres, a.dx = _adr(dy), _adr(x), _adr(weight), _adr(mean), _adr(rstd), _adr(dres), _adr(dx)
+    a.dweight, a.dbias, a.partial = _adr(dweight), _adr(dbias), _adr(part)
     a.rms, a.w_f32, a.accumulate, a.M, a.C = int(rms), int(weight.dtype == torch.float32), int(accumulate), M, Cc
     _call("aitk_norm_bwd", C.byref(a))
     return dx
 
 
 def _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal):
-    _need(B >= 0 and H > 0 and S >= 0, f"B, H, S: got {B}, {H}, {S}")
-    _need(0.0 < scale < float("inf"), f"scale must be positive and finite, got {scale}")
+    if not (B >= 0 and H > 0 and S >= 0 and 0.0 < scale < 1e30):
+        raise ValueError(f"B, H, S, scale: got {B}, {H}, {S}, {scale} (scale must be positive and finite)")
     a = _capi.AttnRelposArgs()
-    a.ldq, a.ldk, a.ldv, a.ldo = (_rows(t, n, B * S, H * 64) for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")))
-    _need(lse.dtype == torch.float32 and lse.numel() == B * H * S and lse.is_contiguous(), f"lse: expected a contiguous fp32 [{B}, {H}, {S}]")
+    n, w = B * S, H * 64
+    a.ldq, a.ldk, a.ldv, a.ldo = _rows(q, "q", n, w), _rows(k, "k", n, w), _rows(v, "v", n, w), _rows(o, "o", n, w)
+    if lse.dtype != torch.float32 or lse.numel() != n * H or not lse.is_contiguous():
+        raise ValueError(f"lse: expected a contiguous fp32 [{B}, {H}, {S}], got {lse.dtype} {tuple(lse.shape)}")
     if table is not None:
-        _need(table.dtype == BF16 and table.dim() == 2 and table.shape[1] == H and table.is_contiguous(), f"table: expected a contiguous bf16 [num_buckets, {H}]")
+        if table.dtype != BF16 or table.dim() != 2 or table.shape[1] != H or not table.is_contiguous():
+            raise ValueError(f"table: expected a contiguous bf16 [num_buckets, {H}], got {table.dtype} {tuple(table.shape)}")
         a.num_buckets, a.max_distance = table.shape[0], max_distance
-        _need(_capi.lib().aitk_attn_relpos_buckets(a.num_buckets, max_distance, int(causal), (C.c_int32 * 64)()) > 0,
-              f"table: {a.num_buckets} buckets up to distance {max_distance} (causal={bool(causal)}): 2 to 64 buckets of each sign, whose exact half must end below max_distance <= 1024")
+        half = a.num_buckets if causal else a.num_buckets // 2
+        if not 2 <= half <= 64 or (not causal and a.num_buckets % 2) or not half // 2 < max_distance <= 1024:
+            raise ValueError(f"table: {a.num_buckets} buckets up to distance {max_distance} (causal={bool(causal)}): 2 to 64 buckets of each sign, the exact half of them "
+                             "below max_distance <= 1024")
     if key_mask is not None:
-        _need(key_mask.dtype in (torch.bool, torch.uint8), f"key_mask: expected bool or uint8 (non-zero = attend), got {key_mask.dtype}")
-        _need(tuple(key_mask.shape) == (B, S) and key_mask.is_contiguous(), f"key_mask: expected a contiguous [{B}, {S}], got {tuple(key_mask.shape)}")
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, S) or not key_mask.is_contiguous():
+            raise ValueError(f"key_mask: expected a contiguous bool or uint8 [{B}, {S}] (non-zero = attend), got {key_mask.dtype} {tuple(key_mask.shape)}")
+    if (S + 64) * max(a.ldq, a.ldk, a.ldv) * 2 >= 2 ** 31 - 1 or n * H >= 2 ** 31:
+        raise ValueError(f"a head's slice of q, k and v must stay below 2 GiB and B S H below 2^31 (B, H, S = {B}, {H}, {S})")
     a.scale, a.B, a.H, a.S, a.causal = scale, B, H, S, int(causal)
-    _need((S + 64) * max(t.stride(0) if B * S > 1 else 0 for t in (q, k, v)) * 2 < 2 ** 31 - 1, "a head's slice of q / k / v must stay below 2 GiB")
     return a
 
 
 def _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask):
-    a.Q, a.K, a.V, a.O, a.LSE, a.table, a.key_mask = _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(table), _ptr(key_mask)
+    a.Q, a.K, a.V, a.O, a.LSE, a.table, a.key_mask = _adr(q), _adr(k), _adr(v), _adr(o), _adr(lse), _adr(table), _adr(key_mask)
 
 
 def attn_relpos_fwd(q, k, v, table, o, lse, *, B, H, S, scale=1.0, key_mask=None, max_distance=128, causal=False):
@@ -1336,18 +1359,19 @@ def attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable=None, *, B, H
     share one table) from attn_relpos_fwd's operands, o and lse.  The probabilities are recomputed; every sum has a fixed order.  dtable's fp32 form is as exact as the
     bf16 operands o and do it is formed from, not more."""
     a = _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
-    a.lddo, a.lddq, a.lddk, a.lddv = (_rows(t, n, B * S, H * 64) for t, n in ((do, "do"), (dq, "dq"), (dk, "dk"), (dv, "dv")))
-    _need((S + 64) * (do.stride(0) if B * S > 1 else 0) * 2 < 2 ** 31 - 1, "a head's slice of do must stay below 2 GiB")
-    if dtable is not None:
-        _need(table is not None, "dtable: there is no table")
-        _need(dtable.dtype in (BF16, torch.float32) and dtable.shape == table.shape and dtable.is_contiguous(), f"dtable: expected a contiguous bf16 or fp32 {tuple(table.shape)}")
+    n, w = B * S, H * 64
+    a.lddo, a.lddq, a.lddk, a.lddv = _rows(do, "do", n, w), _rows(dq, "dq", n, w), _rows(dk, "dk", n, w), _rows(dv, "dv", n, w)
+    if (S + 64) * a.lddo * 2 >= 2 ** 31 - 1:
+        raise ValueError("a head's slice of do must stay below 2 GiB")
+    if dtable is not None and (table is None or dtable.dtype not in (BF16, torch.float32) or dtable.shape != table.shape or not dtable.is_contiguous()):
+        raise ValueError(f"dtable: expected the table's shape, contiguous, in bf16 or fp32, got {dtable.dtype} {tuple(dtable.shape)}" + (" without a table" if table is None else ""))
     _on_device(q=q, k=k, v=v, table=table, o=o, lse=lse, do=do, dq=dq, dk=dk, dv=dv, dtable=dtable, key_mask=key_mask)
     if B * S == 0:
         if dtable is not None and not accumulate:
             host_call(lambda: dtable.zero_())
         return
-    _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask)
     ws = _scratch(_capi.lib().aitk_attn_relpos_bwd_workspace_bytes(B, H, S, a.num_buckets if dtable is not None else 0), q.device)
-    a.dO, a.dQ, a.dK, a.dV, a.dtable, a.ws = _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), _ptr(ws)
+    _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask)
+    a.dO, a.dQ, a.dK, a.dV, a.dtable, a.ws = _adr(do), _adr(dq), _adr(dk), _adr(dv), _adr(dtable), _adr(ws)
     a.dtable_f32, a.accumulate = int(dtable is not None and dtable.dtype == torch.float32), int(accumulate)
     _call("aitk_attn_relpos_bwd", C.byref(a))
