@@ -167,7 +167,7 @@ __device__ __forceinline__ void wg_coords(int ntiles, int H, int& tile, int& hd,
 // 4 waves, key tiles of 64 in a double buffer.  S^T = K Q^T: a lane owns one query row, so the statistics are per-lane scalars and P^T feeds the next product straight from
 // the registers.  KVS = 1: 128 query rows, every wave walks all key tiles.  KVS = 2: 64 query rows, two waves share 32 of them and take every other key tile; their
 // (maximum, sum, output) meet in LDS at the end.  For launches of at most one 128-row workgroup per CU: twice the workgroups, half the steps (1 x 64 heads x 512: 18.0 -> 15.7 us,
-3 x 6 x 333: 13.7 -> 11.3 us; with two workgroups per CU it loses: 1 x 32 x 2048 61.7 -> 71.5 us).
+// 3 x 6 x 333: 13.7 -> 11.3 us; with two workgroups per CU it loses: 1 x 32 x 2048 61.7 -> 71.5 us).
 template <bool BIAS, bool CAUSAL, int KVS>
 __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
