@@ -227,12 +227,24 @@ class AttnRelposArgs(C.Structure):
                 ("accumulate", i32), ("_pad", i32)]
 
 
+class GatedFfnArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("w_val", vp), ("w_gate", vp), ("ldw", i64), ("b_val", vp), ("b_gate", vp), ("out", vp), ("ld_out", i64),
+                ("hg", vp), ("ld_hg", i64), ("M", i32), ("K", i32), ("F", i32), ("act", i32)]
+
+
+class GatedFfnBwdArgs(C.Structure):
+    _fields_ = [("dh", vp), ("ld_dh", i64), ("x", vp), ("ldx", i64), ("w_val", vp), ("w_gate", vp), ("ldw", i64), ("hg", vp), ("ld_hg", i64),
+                ("dx", vp), ("ld_dx", i64), ("dw_val", vp), ("dw_gate", vp), ("ld_dw", i64), ("db_val", vp), ("db_gate", vp), ("ws", vp),
+                ("M", i32), ("K", i32), ("F", i32), ("act", i32)]
+
+
 EPI_BIAS, EPI_ACCUM, EPI_GELU, EPI_DGELU, EPI_GATE_RES, EPI_BIAS_ROW, EPI_ADD_AUX, EPI_COL_SCALE, EPI_SPLIT_SLAB, EPI_EMIT_T = 1, 2, 4, 8, 16, 32, 64, 128, 256, 512
 
 _STRUCTS = {0: GemmArgs, 1: LoraDownArgs, 2: LoraWgradArgs, 3: LnModArgs, 4: LnModBwdArgs, 5: GateBwdArgs,
             6: ColsumFinishArgs, 7: QkvPostArgs, 8: EwArgs, 9: AttnArgs, 10: GemvArgs, 11: NoisePackArgs,
             12: MseArgs, 13: AdamWArgs, 14: ShadowDesc, 15: GroupNormArgs, 16: RmsFullArgs, 17: DoraColscaleArgs, 18: DoraBwdArgs,
-            19: KronApplyArgs, 20: GroupNormBwdArgs, 21: DdpmNoiseArgs, 22: QuantRowsArgs, 23: WgradSrc2, 24: NormArgs, 25: NormBwdArgs, 26: AttnRelposArgs}
+            19: KronApplyArgs, 20: GroupNormBwdArgs, 21: DdpmNoiseArgs, 22: QuantRowsArgs, 23: WgradSrc2, 24: NormArgs, 25: NormBwdArgs, 26: AttnRelposArgs, 27: GatedFfnArgs,
+            28: GatedFfnBwdArgs}
 
 
 ABI_VERSION = 12  # AITK_ABI_VERSION of include/aitk_mi355.h this mirror was written against
@@ -307,6 +319,8 @@ def lib():
     L.aitk_attn_relpos_bwd_workspace_bytes.restype = C.c_int64
     L.aitk_attn_relpos_bwd_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.aitk_attn_relpos_buckets.argtypes = [i32, i32, i32, vp]
+    L.aitk_gated_ffn_bwd_workspace_bytes.restype = C.c_int64
+    L.aitk_gated_ffn_bwd_workspace_bytes.argtypes = [i32, i32, i32]
     _lib = L
     return L
 

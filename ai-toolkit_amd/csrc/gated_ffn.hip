@@ -1,0 +1,441 @@
+// Gated feed-forward projections of the text encoders (T5 / UMT5: tanh GELU) and of the UNet transformer blocks (erf GELU), SwiGLU too (gfx950):
+//
+//   u = x Wv^T + bv,  z = x Wg^T + bg,  h = u act(z)                                                   x [M, K], Wv / Wg [F, K], h [M, F]
+//   du = dh act(z),  dz = dh u act'(z);   dx = du Wv + dz Wg,  dWv = du^T x,  dWg = dz^T x,  dbv / dbg = column sums of du / dz
+//
+// Forward: one launch for both projections, the activation and the product.  A workgroup's B tile is BN / 2 rows of Wg next to the SAME BN / 2 rows of Wv, so a wave's accumulators
+// hold gate and value of one output element in the same register slot and h is formed in registers; [u | z] leaves (as bf16) only when a backward pass will want it.
+// Backward: one pass forms [du | dz] (bf16: the operands of the two products; the column sums take the fp32 values), one launch computes dx and both weight gradients.
+//
+// The products share one tile loop (v_mfma_f32_32x32x16_bf16, fp32 accumulators).  K-tiles of 64 go straight from global memory to LDS (buffer loads; rows and K tails outside
+// the buffer arrive as zeros) into a double buffer of 128-byte rows, 16-byte chunks XOR-swizzled by rkey(row).  An operand whose contraction index is contiguous in memory is staged
+// row by row and read as 16-byte row fragments; one whose contraction index is the ROW (W in dx; du and x in dW) is staged the same way, 64 columns by 64 rows, and read with
+// 16-bit transpose reads: no transposed copy of a weight or an activation exists anywhere.
+#include "common.h"
+#include "aitk_args.h"
+
+namespace {
+typedef __attribute__((address_space(3))) char lds_char;
+typedef int v4i_t __attribute__((ext_vector_type(4)));
+
+enum { ACT_GELU_TANH = 0, ACT_GELU_ERF = 1, ACT_SILU = 2 };
+enum { FWD = 0, GRADS = 1 };
+
+// one product of the tile loop: C[m][n] = sum over segments s, k of A[s](m, k) B[s](n, k)
+struct Prod {
+  const bf16_t* A[2];
+  const bf16_t* B[2];
+  bf16_t* C;
+  long lda, ldb, ldc;
+  int M, N, K, nseg;  // K: per segment
+};
+struct FfnArgs {
+  Prod p[3];  // FWD: p[0] (B[0] = Wg, B[1] = Wv); GRADS: dx, dWv, dWg (M = 0: not wanted)
+  const bf16_t* bv;
+  const bf16_t* bg;
+  bf16_t* hg;  // [M, 2F] = [u | z], may be NULL
+  long ld_hg;
+  int act, _pad;
+};
+
+__device__ __forceinline__ float act_f(float z, int act) {
+  if (act == ACT_GELU_TANH) return gelu_tanh_f(z);
+  if (act == ACT_GELU_ERF) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  return z / (1.0f + __expf(-z));
+}
+// act'(z) next to act(z)
+__device__ __forceinline__ void act_grad_f(float z, int act, float& f, float& d) {
+  if (act == ACT_GELU_TANH) {
+    f = gelu_tanh_f(z);
+    d = gelu_tanh_grad_f(z);
+  } else if (act == ACT_GELU_ERF) {
+    const float c = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+    f = z * c;
+    d = c + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+  } else {
+    const float s = 1.0f / (1.0f + __expf(-z));
+    f = z * s;
+    d = s * (1.0f + z * (1.0f - s));
+  }
+}
+
+__device__ __forceinline__ int rkey(int row) { return (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
+__device__ __forceinline__ v4i_t make_srd(const void* base, long bytes) {
+  const unsigned long long a = (unsigned long long)base;
+  v4i_t r;
+  r.x = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffu));
+  r.y = __builtin_amdgcn_readfirstlane((int)(a >> 32));
+  r.z = __builtin_amdgcn_readfirstlane((int)bytes);
+  r.w = 0x00020000;
+  return r;
+}
+// 64 lanes x 16 bytes to consecutive LDS addresses; an offset outside the descriptor brings zeros.  No register is written.
+__device__ __forceinline__ void dma16(unsigned dst, unsigned voff, const v4i_t& srd, unsigned soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(srd), "s"(soff) : "memory");
+}
+__device__ __forceinline__ void dma_wait_all() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+// One operand's side of the tile loop: R rows (columns of C's other side) x 64 of the contraction, KC: the contraction index is contiguous in memory.
+template <int R, int NT, bool KC>
+struct Operand {
+  static constexpr int BYTES = R * 128, NDMA = R * 8 / NT;
+  unsigned voff[KC ? NDMA : 1];
+  int rd[2];  // KC: row fragment address of contraction steps (ks & 1): chunk 2 ks + h; otherwise the transpose reads of row halves lo / hi
+  int rd2;
+  const bf16_t* base;
+  long ld;
+  long rows;  // rows (KC) or columns (otherwise) of the matrix from the tile's first on
+  __device__ __forceinline__ void init(const bf16_t* p, long ld_, int r0, int count, int tid) {
+    ld = ld_;
+    rows = count - r0;
+    base = KC ? p + (long)r0 * ld : p + r0;
+    const int lane = tid & 63, row = tid >> 3, chunk = (tid & 7) ^ rkey(row);
+    if constexpr (KC) {
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) voff[i] = (unsigned)(((row + i * (NT / 8)) * ld + chunk * 8) * 2);
+    } else {
+      voff[0] = (unsigned)((row * ld + chunk * 8) * 2);
+    }
+    const int l31 = lane & 31, h = lane >> 5, i = lane & 15, gq = (lane >> 4) & 1;
+    if constexpr (KC) {
+      rd[0] = l31 * 128 + ((h ^ rkey(l31)) << 4);
+    } else {
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        const int k = 8 * h + 4 * hi + (i >> 2), c = 2 * gq + ((i & 3) >> 1);
+        rd[hi] = k * 128 + ((c ^ rkey(k)) << 4) + (i & 1) * 8;
+      }
+    }
+  }
+  __device__ __forceinline__ void rebase(const bf16_t* p, int r0) { base = KC ? p + (long)r0 * ld : p + r0; }
+  // K-tile [k0, k0 + 64) of a segment of K: tile rows / columns past the matrix and k >= K arrive as zeros (columns past it: the neighbour's, never stored)
+  __device__ __forceinline__ void stage(unsigned dst, int k0, int K, int tid, int wave) const {
+    if constexpr (KC) {
+      const long left = rows < R ? rows : R;
+      const v4i_t srd = make_srd(base, ((left - 1) * ld + K) * 2);
+      const bool tail = k0 + 64 > K;
+      const bool out = tail && k0 + (((tid & 7) ^ rkey(tid >> 3)) * 8) >= K;
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i)
+        dma16(__builtin_amdgcn_readfirstlane(dst + i * (NT * 16) + wave * 1024), out ? 0x80000000u : voff[i], srd, (unsigned)k0 * 2);
+    } else {
+      const int kl = K - k0 < 64 ? K - k0 : 64;
+      const long cols = rows < R ? rows : R;
+      const v4i_t srd = make_srd(base + (long)k0 * ld, ((long)(kl - 1) * ld + cols) * 2);
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) {
+        // DMA i fills rows [i * NT / 8 % 64, ...) of 64-column block i * NT / 512
+        const int blk = i * NT / 512, k = i * (NT / 8) % 64;
+        dma16(__builtin_amdgcn_readfirstlane(dst + blk * 8192 + k * 128 + wave * 1024), voff[0] + (unsigned)(k * ld * 2) + blk * 128, srd, 0);
+      }
+    }
+  }
+  // fragment of the 32 rows from r on (a multiple of 32), contraction step ks
+  __device__ __forceinline__ s16x8_t frag(const lds_char* t, int r, int ks) const {
+    if constexpr (KC) {
+      return *reinterpret_cast<const __attribute__((address_space(3))) s16x8_t*>(t + r * 128 + (rd[0] ^ (ks * 32)));
+    } else {
+      const lds_char* q = t + (r >> 6) * 8192 + ks * 2048;
+      const int flip = (r & 32) * 2;  // the second 32 columns of a block: chunk + 4
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(q + (rd[0] ^ flip)));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(q + (rd[1] ^ flip)));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// The tile loop.  WR x WC waves; a wave owns MB x 32 rows and, of each half of the tile's columns, 32: columns wc * 32 + ni * BN / 2.
+template <int BM, int BN, int WR, int WC, bool AK, bool BKC, bool PAIR>
+struct TileLoop {
+  static constexpr int NT = WR * WC * 64, MB = BM / WR / 32;
+  static_assert(BN == WC * 64, "two 32-column blocks per wave");
+  static constexpr int BUF = (BM + BN) * 128;
+  f32x16_t acc[MB][2];
+  __device__ __forceinline__ void run(const Prod& p, int m0, int n0, char* smem) {
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave / WC, wc = wave % WC;
+    lds_char* const sm = (lds_char*)smem;
+    Operand<BM, NT, AK> A;
+    Operand<PAIR ? BN / 2 : BN, NT, BKC> B, B2;
+    A.init(p.A[0], p.lda, m0, p.M, tid);
+    B.init(p.B[0], p.ldb, n0, p.N, tid);
+    if constexpr (PAIR) B2.init(p.B[1], p.ldb, n0, p.N, tid);
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    const int kt_seg = (p.K + 63) / 64, nkt = kt_seg * p.nseg;
+    auto stage = [&](int t, int buf) {
+      const int s = t >= kt_seg ? 1 : 0, k0 = (t - s * kt_seg) * 64;
+      if (!PAIR && t == kt_seg) {
+        A.rebase(p.A[1], m0);
+        B.rebase(p.B[1], n0);
+      }
+      const unsigned dst = (unsigned)(size_t)sm + buf * BUF;
+      A.stage(dst, k0, p.K, tid, wave);
+      B.stage(dst + BM * 128, k0, p.K, tid, wave);
+      if constexpr (PAIR) B2.stage(dst + BM * 128 + BN * 64, k0, p.K, tid, wave);
+    };
+    stage(0, 0);
+    dma_wait_all();
+    __syncthreads();
+    for (int t = 0; t < nkt; ++t) {
+      const lds_char* at = sm + (t & 1) * BUF;
+      const lds_char* bt = at + BM * 128;
+      if (t + 1 < nkt) stage(t + 1, (t + 1) & 1);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        s16x8_t af[MB], bf[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) bf[j] = B.frag(bt, j * (BN / 2) + wc * 32, ks);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) af[i] = A.frag(at, wr * (BM / WR) + i * 32, ks);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = mfma32(bf[j], af[i], acc[i][j]);
+      }
+      dma_wait_all();
+      __syncthreads();
+    }
+  }
+};
+
+// tile order: XCD k works on a contiguous range of tiles, 8 row tiles of a column group at a time, so that its L2 sees few panels
+__device__ __forceinline__ void tile_coords(int id, int ntiles, int tm, int tn, int& m, int& n) {
+  const int l = xcd_remap(id, ntiles);
+  const int per = 8 * tn, g = l / per, first = g * 8, gm = min(tm - first, 8);
+  m = first + (l % per) % gm;
+  n = (l % per) / gm;
+}
+__device__ __forceinline__ void store4(bf16_t* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(a, b), pack2bf(c, d));
+}
+
+template <int BM, int BN, int WR, int WC>
+__global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Prod& p = a.p[0];
+  const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN / 2 - 1) / (BN / 2);
+  int ti, tj;
+  tile_coords(blockIdx.x, tm * tn, tm, tn, ti, tj);
+  TileLoop<BM, BN, WR, WC, true, true, true> T;
+  T.run(p, ti * BM, tj * (BN / 2), smem);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+  const int m_w = ti * BM + (wave / WC) * (BM / WR), n_w = tj * (BN / 2) + (wave % WC) * 32 + 4 * h;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int n = n_w + 8 * g;
+    if (n >= p.N) continue;
+    float bv[4] = {}, bg[4] = {};
+    if (a.bv) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bv[e] = bf2f(a.bv[n + e]);
+    }
+    if (a.bg) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bg[e] = bf2f(a.bg[n + e]);
+    }
+#pragma unroll
+    for (int i = 0; i < T.MB; ++i) {
+      const int m = m_w + i * 32 + l31;
+      if (m >= p.M) continue;
+      float z[4], u[4], o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[e] = T.acc[i][0][4 * g + e] + bg[e];
+        u[e] = T.acc[i][1][4 * g + e] + bv[e];
+        o[e] = u[e] * act_f(z[e], a.act);
+      }
+      store4(p.C + (long)m * p.ldc + n, o[0], o[1], o[2], o[3]);
+      if (a.hg) {
+        bf16_t* q = a.hg + (long)m * a.ld_hg + n;
+        store4(q, u[0], u[1], u[2], u[3]);
+        store4(q + p.N, z[0], z[1], z[2], z[3]);
+      }
+    }
+  }
+}
+
+template <int BM, int BN, int WR, int WC, bool AK>
+__device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, char* smem) {
+  TileLoop<BM, BN, WR, WC, AK, false, false> T;
+  T.run(p, ti * BM, tj * BN, smem);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+  const int m_w = ti * BM + (wave / WC) * (BM / WR), n_w = tj * BN + (wave % WC) * 32 + 4 * h;
+#pragma unroll
+  for (int i = 0; i < T.MB; ++i) {
+    const int m = m_w + i * 32 + l31;
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int n = n_w + j * (BN / 2) + 8 * g;
+        if (n < p.N) store4(p.C + (long)m * p.ldc + n, T.acc[i][j][4 * g], T.acc[i][j][4 * g + 1], T.acc[i][j][4 * g + 2], T.acc[i][j][4 * g + 3]);
+      }
+  }
+}
+
+// dx and the two weight gradients in one launch: dx's tiles are few and long (a contraction over 2 F), the weights' many and short; the long ones go first
+template <int BM, int BN, int WR, int WC>
+__global__ __launch_bounds__(WR * WC * 64) void gated_ffn_grads_kernel(FfnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  int id = blockIdx.x;
+#pragma unroll 1
+  for (int q = 0; q < 3; ++q) {
+    const Prod& p = a.p[q];
+    const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, n = tm * tn;
+    if (id >= n) {
+      id -= n;
+      continue;
+    }
+    int ti, tj;
+    tile_coords(id, n, tm, tn, ti, tj);
+    if (q == 0) grad_tile<BM, BN, WR, WC, true>(p, ti, tj, smem);
+    else grad_tile<BM, BN, WR, WC, false>(p, ti, tj, smem);
+    return;
+  }
+}
+
+// [du | dz] from dh and [u | z]; with SUMS the fp32 column sums of the workgroup's rows.  Memory bound: three reads, two writes.  A thread owns 8 columns.
+constexpr int DU_ROWS = 64;  // rows of a workgroup
+template <bool SUMS>
+__global__ __launch_bounds__(256) void gated_ffn_du_kernel(const bf16_t* dh, long ld_dh, const bf16_t* hg, long ld_hg, bf16_t* du, int M, int F, int act, float* part) {
+  const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8, sub = threadIdx.x >> 6;
+  const int r0 = blockIdx.y * DU_ROWS, r1 = min(M, r0 + DU_ROWS);
+  float sv[8] = {}, sz[8] = {};
+  if (c < F) {
+    for (int m = r0 + sub; m < r1; m += 4) {
+      const uint4 d4 = *reinterpret_cast<const uint4*>(dh + (long)m * ld_dh + c);
+      const uint4 u4 = *reinterpret_cast<const uint4*>(hg + (long)m * ld_hg + c);
+      const uint4 z4 = *reinterpret_cast<const uint4*>(hg + (long)m * ld_hg + F + c);
+      const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w}, zw[4] = {z4.x, z4.y, z4.z, z4.w};
+      float ov[8], oz[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = e & 1 ? bf_hi(dw[e >> 1]) : bf_lo(dw[e >> 1]), u = e & 1 ? bf_hi(uw[e >> 1]) : bf_lo(uw[e >> 1]);
+        const float z = e & 1 ? bf_hi(zw[e >> 1]) : bf_lo(zw[e >> 1]);
+        float f, s;
+        act_grad_f(z, act, f, s);
+        ov[e] = d * f;
+        oz[e] = d * u * s;
+        if (SUMS) {
+          sv[e] += ov[e];
+          sz[e] += oz[e];
+        }
+      }
+      bf16_t* q = du + (long)m * 2 * F + c;
+      *reinterpret_cast<uint4*>(q) = make_uint4(pack2bf(ov[0], ov[1]), pack2bf(ov[2], ov[3]), pack2bf(ov[4], ov[5]), pack2bf(ov[6], ov[7]));
+      *reinterpret_cast<uint4*>(q + F) = make_uint4(pack2bf(oz[0], oz[1]), pack2bf(oz[2], oz[3]), pack2bf(oz[4], oz[5]), pack2bf(oz[6], oz[7]));
+    }
+  }
+  if constexpr (SUMS) {
+    __shared__ float box[4][64][17];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      box[sub][threadIdx.x & 63][e] = sv[e];
+      box[sub][threadIdx.x & 63][8 + e] = sz[e];
+    }
+    __syncthreads();
+    if (sub < 2 && c < F) {
+      float* out = part + ((long)blockIdx.y * 2 + sub) * F + c;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = sub * 8 + e, l = threadIdx.x & 63;
+        out[e] = box[0][l][i] + box[1][l][i] + box[2][l][i] + box[3][l][i];
+      }
+    }
+  }
+}
+__global__ __launch_bounds__(256) void gated_ffn_db_kernel(const float* part, int nchunk, int F, bf16_t* dbv, bf16_t* dbg) {
+  const int c = blockIdx.x * 256 + threadIdx.x, v = blockIdx.y;
+  bf16_t* out = v ? dbg : dbv;
+  if (c >= F || !out) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < nchunk; ++k) s += part[((long)k * 2 + v) * F + c];
+  out[c] = f2bf(s);
+}
+
+bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
+bool bad(const void* p, int64_t ld, int64_t width) { return mis16(p) || (ld % 8) || ld < width || ld > (1 << 20); }
+
+template <typename K>
+int launch(K kernel, unsigned grid, unsigned threads, size_t lds, const FfnArgs& a, hipStream_t s) {
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, s, a);
+  AITK_LAUNCH_CHECK();
+  return AITK_OK;
+}
+int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return m <= 0 ? 0 : ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
+}  // namespace
+
+extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t stream) {
+  if (!q || q->M <= 0 || q->K <= 0 || q->F <= 0 || (q->K % 8) || (q->F % 8)) return AITK_ERR_SHAPE;
+  if (!q->x || !q->w_val || !q->w_gate || !q->out || q->act < 0 || q->act > 2) return AITK_ERR_ARG;
+  if (bad(q->x, q->ldx, q->K) || bad(q->w_val, q->ldw, q->K) || mis16(q->w_gate) || bad(q->out, q->ld_out, q->F) || (q->hg && bad(q->hg, q->ld_hg, 2 * (int64_t)q->F)))
+    return AITK_ERR_ALIGN;
+  FfnArgs a = {};
+  a.p[0] = Prod{{q->x, q->x}, {q->w_gate, q->w_val}, q->out, q->ldx, q->ldw, q->ld_out, q->M, q->F, q->K, 1};
+  a.bv = q->b_val;
+  a.bg = q->b_gate;
+  a.hg = q->hg;
+  a.ld_hg = q->ld_hg;
+  a.act = q->act;
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t big = tiles(q->M, q->F, 256, 128), small = tiles(q->M, q->F, 128, 64);
+  if (small > 0x7fffffff) return AITK_ERR_SHAPE;
+  if (big >= 128) return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)big, 512, 131072, a, s);
+  return launch(gated_ffn_fwd_kernel<128, 128, 2, 2>, (unsigned)small, 256, 65536, a, s);
+}
+
+extern "C" int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t F, int32_t bias_grads) {
+  if (M <= 0 || F <= 0) return 0;
+  const int64_t du = ((int64_t)M * 2 * F * 2 + 15) / 16 * 16;
+  return du + (bias_grads ? (int64_t)((M + DU_ROWS - 1) / DU_ROWS) * 2 * F * 4 : 0);
+}
+
+extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t stream) {
+  if (!q || q->M <= 0 || q->K <= 0 || q->F <= 0 || (q->K % 8) || (q->F % 8) || (q->M + DU_ROWS - 1) / DU_ROWS > 65535) return AITK_ERR_SHAPE;
+  const bool dw = q->dw_val || q->dw_gate, db = q->db_val || q->db_gate;
+  if (!q->dh || !q->hg || !q->ws || q->act < 0 || q->act > 2 || (q->dx && (!q->w_val || !q->w_gate)) || (dw && !q->x)) return AITK_ERR_ARG;
+  if (bad(q->dh, q->ld_dh, q->F) || bad(q->hg, q->ld_hg, 2 * (int64_t)q->F) || mis16(q->ws) || (q->dx && (bad(q->dx, q->ld_dx, q->K) || bad(q->w_val, q->ldw, q->K) || mis16(q->w_gate))) ||
+      (dw && (bad(q->x, q->ldx, q->K) || q->ld_dw % 8 || q->ld_dw < q->K || mis16(q->dw_val) || mis16(q->dw_gate))))
+    return AITK_ERR_ALIGN;
+  const int M = q->M, F = q->F, K = q->K;
+  if (2 * (int64_t)F > (1 << 20)) return AITK_ERR_SHAPE;
+  bf16_t* du = reinterpret_cast<bf16_t*>(q->ws);
+  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(q->ws) + ((int64_t)M * 2 * F * 2 + 15) / 16 * 16);
+  hipStream_t s = (hipStream_t)stream;
+  const int nchunk = (M + DU_ROWS - 1) / DU_ROWS;
+  const dim3 grid((F / 8 + 63) / 64, nchunk);
+  if (db) hipLaunchKernelGGL(gated_ffn_du_kernel<true>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, part);
+  else hipLaunchKernelGGL(gated_ffn_du_kernel<false>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, part);
+  AITK_LAUNCH_CHECK();
+  if (db) {
+    hipLaunchKernelGGL(gated_ffn_db_kernel, dim3((F + 255) / 256, 2), dim3(256), 0, s, part, nchunk, F, q->db_val, q->db_gate);
+    AITK_LAUNCH_CHECK();
+  }
+  FfnArgs a = {};
+  if (q->dx) a.p[0] = Prod{{du, du + F}, {q->w_val, q->w_gate}, q->dx, 2 * (long)F, q->ldw, q->ld_dx, M, K, F, 2};
+  if (q->dw_val) a.p[1] = Prod{{du, du}, {q->x, q->x}, q->dw_val, 2 * (long)F, q->ldx, q->ld_dw, F, K, M, 1};
+  if (q->dw_gate) a.p[2] = Prod{{du + F, du + F}, {q->x, q->x}, q->dw_gate, 2 * (long)F, q->ldx, q->ld_dw, F, K, M, 1};
+  int64_t big = 0, small = 0;
+  for (const Prod& p : a.p) {
+    big += tiles(p.M, p.N, 256, 256);
+    small += tiles(p.M, p.N, 128, 128);
+  }
+  if (!small) return AITK_OK;
+  if (small > 0x7fffffff) return AITK_ERR_SHAPE;
+  if (big >= 128) return launch(gated_ffn_grads_kernel<256, 256, 2, 4>, (unsigned)big, 512, 131072, a, s);
+  return launch(gated_ffn_grads_kernel<128, 128, 2, 2>, (unsigned)small, 256, 65536, a, s);
+}

@@ -94,6 +94,8 @@ extern "C" int aitk_sizeof(int32_t which) {
     case 24: return (int)sizeof(AitkNormArgs);
     case 25: return (int)sizeof(AitkNormBwdArgs);
     case 26: return (int)sizeof(AitkAttnRelposArgs);
+    case 27: return (int)sizeof(AitkGatedFfnArgs);
+    case 28: return (int)sizeof(AitkGatedFfnBwdArgs);
     default: return -1;
   }
 }

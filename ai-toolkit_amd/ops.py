@@ -1375,3 +1375,83 @@ def attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable=None, *, B, H
     a.dO, a.dQ, a.dK, a.dV, a.dtable, a.ws = _adr(do), _adr(dq), _adr(dk), _adr(dv), _adr(dtable), _adr(ws)
     a.dtable_f32, a.accumulate = int(dtable is not None and dtable.dtype == torch.float32), int(accumulate)
     _call("aitk_attn_relpos_bwd", C.byref(a))
+
+
+GATED_ACTS = {"gelu_tanh": 0, "gelu": 1, "silu": 2}
+
+
+def _ffn_shape(x, w_val, w_gate, act):
+    if act not in GATED_ACTS:
+        raise ValueError(f"act: expected one of {sorted(GATED_ACTS)}, got {act!r}")
+    if x.dim() != 2 or w_val.dim() != 2 or x.shape[1] != w_val.shape[1]:
+        raise ValueError(f"x [M, K] and w_val [F, K] do not match: {tuple(x.shape)}, {tuple(w_val.shape)}")
+    M, K = x.shape
+    F = w_val.shape[0]
+    if K <= 0 or F <= 0 or K % 8 or F % 8 or 2 * F > 1 << 20:
+        raise ValueError(f"K and F must be positive multiples of 8 (2 F up to 2^20), got K = {K}, F = {F}")
+    ldw = _rows(w_val, "w_val", F, K)
+    if _rows(w_gate, "w_gate", F, K) != ldw:
+        raise ValueError(f"w_val and w_gate must share one row pitch, got {w_val.stride(0)} and {w_gate.stride(0)}")
+    return M, K, F, ldw
+
+
+def _pitches(*lds):
+    if max(lds) > 1 << 20:
+        raise ValueError(f"row pitches must stay up to 2^20 elements, got {max(lds)}")
+
+
+def gated_ffn_fwd(x, w_val, w_gate, out, *, act="gelu_tanh", b_val=None, b_gate=None, hg=None):
+    """out = (x w_val^T + b_val) * act(x w_gate^T + b_gate) in one launch: x [M, K], weights [F, K] (one row pitch: two views of a fused [2F, K] matrix, or two matrices),
+    biases [F] or None, out [M, F], all bf16.  act: "gelu_tanh" (T5 / UMT5), "gelu" (erf: GEGLU) or "silu".  hg [M, 2F]: also leaves [value | gate] before the
+    activation, which gated_ffn_bwd needs (geglu_fwd's layout).  K % 8 == F % 8 == 0."""
+    M, K, F, ldw = _ffn_shape(x, w_val, w_gate, act)
+    a = _capi.GatedFfnArgs()
+    a.ldx, a.ld_out, a.ldw = _rows(x, "x", M, K), _rows(out, "out", M, F), ldw
+    if hg is not None:
+        a.ld_hg = _rows(hg, "hg", M, 2 * F)
+    if b_val is not None:
+        _vec(b_val, "b_val", F, (BF16,))
+    if b_gate is not None:
+        _vec(b_gate, "b_gate", F, (BF16,))
+    _pitches(a.ldx, a.ld_out, a.ld_hg, ldw)
+    _on_device(x=x, w_val=w_val, w_gate=w_gate, out=out, b_val=b_val, b_gate=b_gate, hg=hg)
+    if M == 0:
+        return out
+    a.x, a.w_val, a.w_gate, a.b_val, a.b_gate, a.out, a.hg = _adr(x), _adr(w_val), _adr(w_gate), _adr(b_val), _adr(b_gate), _adr(out), _adr(hg)
+    a.M, a.K, a.F, a.act = M, K, F, GATED_ACTS[act]
+    _call("aitk_gated_ffn_fwd", C.byref(a))
+    return out
+
+
+def gated_ffn_bwd(dh, x, w_val, w_gate, hg, *, act="gelu_tanh", dx=None, dw_val=None, dw_gate=None, db_val=None, db_gate=None):
+    """gated_ffn_fwd's gradients from dh [M, F] and the saved hg: dx [M, K], dw_val / dw_gate [F, K] (one row pitch), db_val / db_gate [F], all bf16; only what is
+    given is computed (frozen weights: dx alone).  Nothing is transposed or copied beyond the one [M, 2F] gradient of hg.  Deterministic."""
+    M, K, F, ldw = _ffn_shape(x, w_val, w_gate, act)
+    a = _capi.GatedFfnBwdArgs()
+    a.ld_dh, a.ldx, a.ld_hg, a.ldw = _rows(dh, "dh", M, F), _rows(x, "x", M, K), _rows(hg, "hg", M, 2 * F), ldw
+    if dx is not None:
+        a.ld_dx = _rows(dx, "dx", M, K)
+    if dw_val is not None:
+        a.ld_dw = _rows(dw_val, "dw_val", F, K)
+    if dw_gate is not None:
+        ld = _rows(dw_gate, "dw_gate", F, K)
+        if dw_val is not None and ld != a.ld_dw:
+            raise ValueError(f"dw_val and dw_gate must share one row pitch, got {a.ld_dw} and {ld}")
+        a.ld_dw = ld
+    if db_val is not None:
+        _vec(db_val, "db_val", F, (BF16,))
+    if db_gate is not None:
+        _vec(db_gate, "db_gate", F, (BF16,))
+    _pitches(a.ld_dh, a.ldx, a.ld_hg, ldw, a.ld_dx, a.ld_dw)
+    if M > 64 * 65535:
+        raise ValueError(f"at most {64 * 65535} rows, got {M}")
+    _on_device(dh=dh, x=x, w_val=w_val, w_gate=w_gate, hg=hg, dx=dx, dw_val=dw_val, dw_gate=dw_gate, db_val=db_val, db_gate=db_gate)
+    if M == 0:
+        host_call(lambda: [t.zero_() for t in (dw_val, dw_gate, db_val, db_gate) if t is not None])
+        return dx
+    ws = _scratch(_capi.lib().aitk_gated_ffn_bwd_workspace_bytes(M, F, int(db_val is not None or db_gate is not None)), x.device)
+    a.dh, a.x, a.w_val, a.w_gate, a.hg = _adr(dh), _adr(x), _adr(w_val), _adr(w_gate), _adr(hg)
+    a.dx, a.dw_val, a.dw_gate, a.db_val, a.db_gate, a.ws = _adr(dx), _adr(dw_val), _adr(dw_gate), _adr(db_val), _adr(db_gate), _adr(ws)
+    a.M, a.K, a.F, a.act = M, K, F, GATED_ACTS[act]
+    _call("aitk_gated_ffn_bwd", C.byref(a))
+    return dx

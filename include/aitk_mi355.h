@@ -641,6 +641,34 @@ int aitk_attn_relpos_bwd(const AitkAttnRelposArgs* args, aitk_stream_t stream);
 /* host only: first[j] = the first distance of bucket j within one sign (64 entries of room) -> half, or AITK_ERR_SHAPE for a bucketing that is not supported */
 int aitk_attn_relpos_buckets(int32_t num_buckets, int32_t max_distance, int32_t causal, int32_t* first);
 
+/* Gated feed-forward projections: u = x w_val^T + b_val, z = x w_gate^T + b_gate, out = u * act(z); x [M, K], weights [F, K] (one row pitch; a fused [2F, K] matrix is
+ * two views of it), biases [F] (may be NULL), out [M, F].  act: 0 tanh GELU (T5 "gated-gelu"), 1 erf GELU (diffusers GEGLU), 2 SiLU.  hg (may be NULL): [M, 2F] =
+ * [u | z] in bf16, what the backward needs — aitk_geglu_fwd's operand layout.  One launch.  K % 8 == F % 8 == 0, pitches % 8 == 0 and <= 2^20, 16-byte aligned. */
+typedef struct AitkGatedFfnArgs {
+  const aitk_bf16* x; int64_t ldx;
+  const aitk_bf16* w_val; const aitk_bf16* w_gate; int64_t ldw;
+  const aitk_bf16* b_val; const aitk_bf16* b_gate;
+  aitk_bf16* out; int64_t ld_out;
+  aitk_bf16* hg; int64_t ld_hg;
+  int32_t M, K, F, act;
+} AitkGatedFfnArgs;
+int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* args, aitk_stream_t stream);
+/* From dh [M, F] and the saved hg: dx [M, K], dw_val / dw_gate [F, K] (one row pitch), db_val / db_gate [F], all bf16, each may be NULL (frozen weights: dx alone).
+ * [du | dz] is formed once in bf16 in ws (aitk_gated_ffn_bwd_workspace_bytes); no transposed copy of any operand is made.  Deterministic. */
+typedef struct AitkGatedFfnBwdArgs {
+  const aitk_bf16* dh; int64_t ld_dh;
+  const aitk_bf16* x; int64_t ldx;
+  const aitk_bf16* w_val; const aitk_bf16* w_gate; int64_t ldw;
+  const aitk_bf16* hg; int64_t ld_hg;
+  aitk_bf16* dx; int64_t ld_dx;
+  aitk_bf16* dw_val; aitk_bf16* dw_gate; int64_t ld_dw;
+  aitk_bf16* db_val; aitk_bf16* db_gate;
+  void* ws;
+  int32_t M, K, F, act;
+} AitkGatedFfnBwdArgs;
+int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t F, int32_t bias_grads);
+int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* args, aitk_stream_t stream);
+
 /* ---- hardware probes (test infrastructure for layout assumptions; not on the product path) ---- */
 /* host-side evaluation of the attention kernels' workgroup -> (row tile, head, batch) map for a 1-D grid of n blocks (XCD-grouped order) */
 int aitk_probe_attn_wg_coords(int32_t n, int32_t id, int32_t ntiles, int32_t H, int32_t* out3);

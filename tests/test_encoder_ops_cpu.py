@@ -1,0 +1,231 @@
+"""The text-encoder block's entry points refuse what their kernels cannot take, before anything is launched: the C calls with AITK_ERR_* codes, the wrappers with ValueError
+(no GPU).  Also the bucketing the attention uses, against whole-number arithmetic and against the formula T5 publishes."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import ai_toolkit_amd  # noqa: F401
+from ai_toolkit_amd import _capi, ops
+from tests.relpos_ref import first_distances
+
+BF16 = torch.bfloat16
+SHAPE, ALIGN, ARG = -1, -2, -3
+
+
+def _t(*shape, dtype=BF16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+# ------------------------------------------------------------------------------------------------------------------ bucketing
+@pytest.mark.parametrize("causal", [0, 1])
+def test_buckets_are_the_whole_number_ones(causal):
+    f = (C.c_int32 * 64)()
+    lib = _capi.lib()
+    for half in (2, 3, 4, 5, 7, 8, 12, 16, 31, 32, 48, 64):
+        nb = half if causal else 2 * half
+        for md in (2, 3, 5, 8, 17, 33, 64, 100, 128, 200, 256, 300, 511, 512, 777, 1000, 1024):
+            rc = lib.aitk_attn_relpos_buckets(nb, md, causal, f)
+            if md <= half // 2:
+                assert rc == SHAPE
+            else:
+                assert rc == half and list(f[:half]) == first_distances(nb, md, causal), (nb, md, causal)
+
+
+def test_buckets_match_the_published_formula_away_from_its_rounding():
+    """floor(log(n / e) / log(max / e) (half - e)) + e; a distance whose quotient is whole belongs to the farther bucket"""
+    first = first_distances(32, 128, False)
+    for n in range(400):
+        x = 8 + math.log(max(n, 1) / 8) / math.log(16) * 8
+        want = n if n < 8 else min(15, int(math.floor(x + 1e-9)))
+        assert sum(n >= f for f in first) - 1 == want
+    lib = _capi.lib()
+    assert lib.aitk_attn_relpos_buckets(32, 128, 0, None) == ARG
+    for bad in ((0, 128), (31, 128), (2, 128), (130, 1024), (32, 8), (32, 1025), (-4, 16)):
+        assert lib.aitk_attn_relpos_buckets(bad[0], bad[1], 0, (C.c_int32 * 64)()) == SHAPE, bad
+
+
+# ------------------------------------------------------------------------------------------------------------------ C entry points
+def _norm_args():
+    a = _capi.NormArgs()
+    a.x = a.y = a.weight = 64
+    a.ldx = a.ldy = 64
+    a.M, a.C, a.eps = 4, 64, 1e-6
+    return a
+
+
+def test_c_norm_refusals():
+    lib = _capi.lib()
+    assert lib.aitk_norm_fwd(None, None) == SHAPE and lib.aitk_norm_bwd(None, None) == SHAPE
+    for field, value, code in (("M", 0, SHAPE), ("C", 60, SHAPE), ("C", 8200, SHAPE), ("x", None, ARG), ("weight", None, ARG), ("y", None, ARG), ("ldx", 60, ALIGN),
+                               ("ldy", 56, ALIGN), ("x", 72, ALIGN), ("bias", 8, ALIGN)):
+        a = _norm_args()
+        setattr(a, field, value)
+        assert lib.aitk_norm_fwd(C.byref(a), None) == code, (field, value)
+    a = _norm_args()
+    a.rms, a.mean = 1, 64
+    assert lib.aitk_norm_fwd(C.byref(a), None) == ARG
+    b = _capi.NormBwdArgs()
+    b.M, b.C = 4, 64
+    assert lib.aitk_norm_bwd(C.byref(b), None) == ARG
+    b.dy = b.x = b.weight = b.rstd = b.mean = b.dx = 64
+    b.ld_dy = b.ldx = b.ld_dx = 64
+    b.dweight = 64
+    assert lib.aitk_norm_bwd(C.byref(b), None) == ARG  # gradients without scratch
+    b.dweight, b.dres, b.ld_dres = None, 64, 32
+    assert lib.aitk_norm_bwd(C.byref(b), None) == ALIGN
+    assert lib.aitk_norm_bwd_workspace_bytes(0, 64, 0) == 0 and lib.aitk_norm_bwd_workspace_bytes(1, 64, 0) == 2 * 64 * 4
+
+
+def _attn_args():
+    a = _capi.AttnRelposArgs()
+    for f in ("Q", "K", "V", "O", "LSE", "table", "dO", "dQ", "dK", "dV", "ws"):
+        setattr(a, f, 64)
+    for f in ("ldq", "ldk", "ldv", "ldo", "lddo", "lddq", "lddk", "lddv"):
+        setattr(a, f, 128)
+    a.B, a.H, a.S, a.scale, a.num_buckets, a.max_distance = 1, 2, 10, 1.0, 32, 128
+    return a
+
+
+def test_c_attention_refusals():
+    lib = _capi.lib()
+    assert lib.aitk_attn_relpos_fwd(None, None) == SHAPE and lib.aitk_attn_relpos_bwd(None, None) == SHAPE
+    for field, value, code in (("B", 0, SHAPE), ("H", 0, SHAPE), ("S", 0, SHAPE), ("scale", 0.0, SHAPE), ("scale", -1.0, SHAPE), ("scale", float("nan"), SHAPE),
+                               ("scale", float("inf"), SHAPE), ("Q", None, ARG), ("LSE", None, ARG), ("ldq", 120, ALIGN), ("ldk", 130, ALIGN), ("V", 72, ALIGN),
+                               ("num_buckets", 31, SHAPE), ("max_distance", 8, SHAPE), ("max_distance", 4096, SHAPE), ("S", 1 << 24, SHAPE)):
+        a = _attn_args()
+        setattr(a, field, value)
+        assert lib.aitk_attn_relpos_fwd(C.byref(a), None) == code, (field, value)
+    for field, value, code in (("dO", None, ARG), ("dK", None, ARG), ("ws", None, ARG), ("lddv", 96, ALIGN), ("dQ", 8, ALIGN)):
+        a = _attn_args()
+        setattr(a, field, value)
+        assert lib.aitk_attn_relpos_bwd(C.byref(a), None) == code, (field, value)
+    a = _attn_args()
+    a.dtable, a.table = 64, None
+    assert lib.aitk_attn_relpos_bwd(C.byref(a), None) == ARG
+
+
+def test_c_gated_ffn_refusals():
+    lib = _capi.lib()
+    assert lib.aitk_gated_ffn_fwd(None, None) == SHAPE and lib.aitk_gated_ffn_bwd(None, None) == SHAPE
+
+    def fwd():
+        a = _capi.GatedFfnArgs()
+        a.x = a.w_val = a.w_gate = a.out = 64
+        a.ldx = a.ldw = 64
+        a.ld_out = 128
+        a.M, a.K, a.F = 4, 64, 128
+        return a
+
+    for field, value, code in (("M", 0, SHAPE), ("K", 60, SHAPE), ("F", 12, SHAPE), ("act", 3, ARG), ("x", None, ARG), ("out", None, ARG), ("ldx", 32, ALIGN),
+                               ("ld_out", 120, ALIGN), ("w_gate", 8, ALIGN), ("ldw", 1 << 21, ALIGN)):
+        a = fwd()
+        setattr(a, field, value)
+        assert lib.aitk_gated_ffn_fwd(C.byref(a), None) == code, (field, value)
+    b = _capi.GatedFfnBwdArgs()
+    b.M, b.K, b.F = 4, 64, 128
+    assert lib.aitk_gated_ffn_bwd(C.byref(b), None) == ARG
+    b.dh = b.hg = b.ws = 64
+    b.ld_dh, b.ld_hg = 128, 256
+    b.dx = 64
+    assert lib.aitk_gated_ffn_bwd(C.byref(b), None) == ARG  # dx without weights
+    b.dx, b.dw_val = None, 64
+    assert lib.aitk_gated_ffn_bwd(C.byref(b), None) == ARG  # a weight gradient without x
+    b.x, b.ldx, b.ld_dw = 64, 64, 60
+    assert lib.aitk_gated_ffn_bwd(C.byref(b), None) == ALIGN
+
+
+# ------------------------------------------------------------------------------------------------------------------ wrappers
+def test_norm_wrapper_refusals():
+    x, w, y = _t(4, 64), _t(64), _t(4, 64)
+    st = _t(4, dtype=torch.float32)
+    for bad, match in ((dict(x=_t(4, 60)), "multiple of 8"), (dict(x=_t(4, 8200)), "up to 8192"), (dict(x=_t(4, 64, dtype=torch.float32)), "expected bf16"),
+                       (dict(x=_t(64)), "expected"), (dict(y=_t(5, 64)), "expected"), (dict(y=_t(64, 4).t()), "inner stride"), (dict(x=_t(1, 64).expand(4, 64)), "not overlap"),
+                       (dict(x=_t(4, 68)[:, :64]), "aligned"), (dict(weight=_t(32)), "weight"), (dict(weight=_t(64, dtype=torch.float16)), "weight"),
+                       (dict(bias=_t(64, dtype=torch.float32)), "bias"), (dict(mean=_t(4)), "mean"), (dict(rstd=_t(5, dtype=torch.float32)), "rstd"), (dict(eps=-1.0), "eps"),
+                       (dict(rms=True, bias=_t(64)), "RMS"), (dict(rms=True, mean=st), "RMS"), (dict(eps=float("nan")), "eps")):
+        kw = dict(x=x, weight=w, y=y)
+        kw.update(bad)
+        with pytest.raises(ValueError, match=match):
+            ops.norm_fwd(kw.pop("x"), kw.pop("weight"), kw.pop("y"), **kw)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.norm_fwd(x, w, y)
+    for bad, match in ((dict(mean=None), "mean"), (dict(rms=True), "mean"), (dict(rms=True, mean=None, dbias=_t(64, dtype=torch.float32)), "dbias"), (dict(dweight=_t(64)), "dweight"),
+                       (dict(dres=_t(4, 72)), "dres")):
+        kw = dict(mean=st)
+        kw.update(bad)
+        with pytest.raises(ValueError, match=match):
+            ops.norm_bwd(y, x, w, st, y, **kw)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.norm_bwd(y, x, w, st, y, mean=st)
+
+
+def test_attention_wrapper_refusals():
+    B, H, S = 2, 3, 5
+    mk = lambda: _t(B * S, H * 64)  # noqa: E731
+    base = dict(q=mk(), k=mk(), v=mk(), table=_t(32, H), o=mk(), lse=_t(B, H, S, dtype=torch.float32))
+    for bad, match in ((dict(q=_t(B * S, H * 64 + 8)), "q: expected"), (dict(k=_t(B * S, H * 128)[:, ::2]), "inner stride"), (dict(v=mk().float()), "bf16"),
+                       (dict(table=_t(32, H + 1)), "table"), (dict(table=_t(31, H)), "buckets"), (dict(table=_t(2, H)), "buckets"), (dict(table=_t(130, H)), "buckets"),
+                       (dict(table=_t(32, H, dtype=torch.float32)), "table"), (dict(max_distance=8), "max_distance"), (dict(max_distance=2000), "max_distance"),
+                       (dict(lse=_t(B, H, S)), "lse"), (dict(lse=_t(B, H, S - 1, dtype=torch.float32)), "lse"), (dict(key_mask=torch.ones(B, S)), "key_mask"),
+                       (dict(key_mask=torch.ones(B, S, dtype=torch.int64)), "key_mask"), (dict(key_mask=torch.ones(B, S + 1, dtype=torch.bool)), "key_mask"),
+                       (dict(key_mask=torch.ones(S, B, dtype=torch.bool).t()), "key_mask"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(B=3), "expected"),
+                       (dict(H=0), "B, H, S")):
+        kw = dict(base, B=B, H=H, S=S)
+        kw.update(bad)
+        args = [kw.pop(n) for n in ("q", "k", "v", "table", "o", "lse")]
+        with pytest.raises(ValueError, match=match):
+            ops.attn_relpos_fwd(*args, **kw)
+    args = [base[n] for n in ("q", "k", "v", "table", "o", "lse")]
+    with pytest.raises(ValueError, match="GPU"):
+        ops.attn_relpos_fwd(*args, B=B, H=H, S=S)
+    with pytest.raises(ValueError, match="2 GiB"):
+        ops._attn_relpos_args(*_huge_views(), B=1, H=1, S=600, scale=1.0, key_mask=None, max_distance=128, causal=False)
+    do, dq, dk, dv = mk(), mk(), mk(), mk()
+    for bad, match in ((dict(dtable=_t(32, H, dtype=torch.float16)), "dtable"), (dict(dtable=_t(16, H)), "dtable"), (dict(table=None, dtable=_t(32, H)), "without a table"),
+                       (dict(do=_t(B * S, 64)), "do"), (dict(dv=mk().float()), "dv")):
+        kw = dict(base, do=do, dq=dq, dk=dk, dv=dv, dtable=None)
+        kw.update(bad)
+        with pytest.raises(ValueError, match=match):
+            ops.attn_relpos_bwd(*[kw[n] for n in ("q", "k", "v", "table", "o", "lse", "do", "dq", "dk", "dv", "dtable")], B=B, H=H, S=S)
+
+
+def _huge_views():
+    """[600, 64] views with a row pitch of 2^21 elements without memory behind them: 600 rows span 2.5 GB"""
+    class View:
+        dtype, shape = BF16, torch.Size((600, 64))
+
+        def stride(self):
+            return (1 << 21, 1)
+
+        def data_ptr(self):
+            return 64
+
+    v = View()
+    return v, v, v, None, v, _t(1, 1, 600, dtype=torch.float32)
+
+
+def test_gated_ffn_wrapper_refusals():
+    M, K, F = 4, 64, 128
+    base = dict(x=_t(M, K), w_val=_t(F, K), w_gate=_t(F, K), out=_t(M, F))
+    for bad, match in ((dict(act="relu"), "act"), (dict(x=_t(M, K + 8)), "do not match"), (dict(w_val=_t(F, 60), x=_t(M, 60)), "multiples of 8"), (dict(w_val=_t(12, K)), "multiples of 8"),
+                       (dict(w_gate=_t(F + 8, K)), "w_gate"), (dict(w_gate=_t(F, K + 8)[:, :K]), "one row pitch"), (dict(out=_t(M, F + 8)), "out"), (dict(hg=_t(M, F)), "hg"),
+                       (dict(b_val=_t(F, dtype=torch.float32)), "b_val"), (dict(b_gate=_t(F + 8)), "b_gate"), (dict(x=_t(M, K).float()), "bf16")):
+        kw = dict(base)
+        kw.update(bad)
+        args = [kw.pop(n) for n in ("x", "w_val", "w_gate", "out")]
+        with pytest.raises(ValueError, match=match):
+            ops.gated_ffn_fwd(*args, **kw)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.gated_ffn_fwd(**base)
+    dh, hg = _t(M, F), _t(M, 2 * F)
+    for bad, match in ((dict(dh=_t(M, K)), "dh"), (dict(hg=_t(M, F)), "hg"), (dict(dx=_t(M, F)), "dx"), (dict(dw_val=_t(K, F)), "dw_val"), (dict(db_gate=_t(K)), "db_gate"),
+                       (dict(dw_val=_t(F, K), dw_gate=_t(F, K + 8)[:, :K]), "one row pitch")):
+        kw = dict(dh=dh, x=base["x"], w_val=base["w_val"], w_gate=base["w_gate"], hg=hg)
+        kw.update(bad)
+        args = [kw.pop(n) for n in ("dh", "x", "w_val", "w_gate", "hg")]
+        with pytest.raises(ValueError, match=match):
+            ops.gated_ffn_bwd(*args, **kw)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.gated_ffn_bwd(dh, base["x"], base["w_val"], base["w_gate"], hg, dx=_t(M, K))

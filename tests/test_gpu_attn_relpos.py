@@ -51,6 +51,8 @@ def _near(got, want, tol, name):
     d = (got.double() - want).abs()
     assert torch.isfinite(got).all(), name
     over = d - tol
+    # the bounds above add up absolute values; in the 2-norm at most four roundings (p, o, ds, the result), each below u of its value, reach a result
+    assert float(d.norm()) <= 4 * ref.U * float(want.norm()) + float(tol.min()), f"{name}: relative error {float(d.norm() / want.norm()):.3g}"
     assert (over <= 0).all(), f"{name}: {int((over > 0).sum())} of {d.numel()} elements over their bound, worst by {float(over.max()):.3g} (error {float(d.max()):.3g})"
 
 

@@ -1,0 +1,126 @@
+"""Two text-encoder layers trained through the native operators on the MI355X, as a native encoder would run them — norm, fused q / k / v projection, attention with the relative
+position bias that both layers share, output projection with the residual, norm, gated feed-forward projections, output projection with the residual, and all of it
+backwards — against 64-bit autograd of the published formulas (T5: RMS norm, position bias, no scale; CLIP-like: layer norm, causal, scaled, no bias).
+
+Bound: between an input and any gradient lie at most 2 layers x 16 bf16 tensors (each rounded once, at most u = 2^-8 of its value in the 2-norm) that reach the result through
+residual sums or operators that stretch a relative error by less than 2 on these inputs; independent roundings add up like their squares: 2 u sqrt(32) = 12 u."""
+import pytest
+import torch
+
+from tests import relpos_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+U = 2.0 ** -8
+
+
+def _weights(kind, H, F, seed):
+    C = H * 64
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s, std: (torch.randn(*s, generator=g, device="cuda") * std).to(BF16)  # noqa: E731
+    layers = []
+    for _ in range(2):
+        w = dict(n1=1 + r(C, std=0.2), n2=1 + r(C, std=0.2), qkv=r(3 * C, C, std=C ** -0.5 * 0.6), o=r(C, C, std=C ** -0.5), wv=r(F, C, std=C ** -0.5), wg=r(F, C, std=C ** -0.5),
+                 wo=r(C, F, std=F ** -0.5))
+        if kind == "clip":
+            w.update(b1=r(C, std=0.1), b2=r(C, std=0.1))
+        layers.append(w)
+    return layers, r(32, H, std=0.5) if kind == "t5" else None
+
+
+def _native(x, layers, table, dout, mask, *, kind, B, H, S):
+    from ai_toolkit_amd import ops
+
+    C, M = H * 64, B * S
+    F = layers[0]["wv"].shape[0]
+    rms, act = kind == "t5", "gelu_tanh" if kind == "t5" else "silu"
+    kw = dict(B=B, H=H, S=S, scale=1.0 if kind == "t5" else 0.125, key_mask=mask, causal=kind == "clip")
+    e = lambda *s, dtype=BF16: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+    f32 = torch.float32
+    saved = []
+    for w in layers:
+        s = dict(x=x, n1=e(M, C), qkv=e(M, 3 * C), a=e(M, C), lse=e(B, H, S, dtype=f32), x1=e(M, C), n2=e(M, C), h=e(M, F), hg=e(M, 2 * F), r1=e(M, dtype=f32), r2=e(M, dtype=f32),
+                 m1=None if rms else e(M, dtype=f32), m2=None if rms else e(M, dtype=f32))
+        q, k, v = (s["qkv"][:, i * C:(i + 1) * C] for i in range(3))
+        ops.norm_fwd(x, w["n1"], s["n1"], bias=w.get("b1"), rms=rms, mean=s["m1"], rstd=s["r1"])
+        ops.gemm_nt(s["n1"], w["qkv"], s["qkv"])
+        ops.attn_relpos_fwd(q, k, v, table, s["a"], s["lse"], **kw)
+        ops.gemm_nt(s["a"], w["o"], s["x1"], flags=64, aux_in=x)  # + residual
+        ops.norm_fwd(s["x1"], w["n2"], s["n2"], bias=w.get("b2"), rms=rms, mean=s["m2"], rstd=s["r2"])
+        ops.gated_ffn_fwd(s["n2"], w["wv"], w["wg"], s["h"], act=act, hg=s["hg"])
+        x = e(M, C)
+        ops.gemm_nt(s["h"], w["wo"], x, flags=64, aux_in=s["x1"])
+        saved.append(s)
+    out, grads = x, []
+    dtable = None if table is None else torch.empty(32, H, device="cuda")
+    dx = dout
+    for i, (w, s) in enumerate(zip(layers[::-1], saved[::-1])):
+        q, k, v = (s["qkv"][:, j * C:(j + 1) * C] for j in range(3))
+        g = dict(n1=e(C, dtype=f32), n2=e(C, dtype=f32), wv=e(F, C), wg=e(F, C))
+        if not rms:
+            g.update(b1=e(C, dtype=f32), b2=e(C, dtype=f32))
+        dh, dn2, dx1, da, dqkv, dn1 = e(M, F), e(M, C), e(M, C), e(M, C), e(M, 3 * C), e(M, C)
+        ops.gemm_nt(dx, w["wo"].t().contiguous(), dh)
+        ops.gated_ffn_bwd(dh, s["n2"], w["wv"], w["wg"], s["hg"], act=act, dx=dn2, dw_val=g["wv"], dw_gate=g["wg"])
+        ops.norm_bwd(dn2, s["x1"], w["n2"], s["r2"], dx1, mean=s["m2"], rms=rms, dres=dx, dweight=g["n2"], dbias=g.get("b2"))
+        ops.gemm_nt(dx1, w["o"].t().contiguous(), da)
+        ops.attn_relpos_bwd(q, k, v, table, s["a"], s["lse"], da, dqkv[:, :C], dqkv[:, C:2 * C], dqkv[:, 2 * C:], dtable, accumulate=i > 0, **kw)
+        ops.gemm_nt(dqkv, w["qkv"].t().contiguous(), dn1)
+        dx = e(M, C)
+        ops.norm_bwd(dn1, s["x"], w["n1"], s["r1"], dx, mean=s["m1"], rms=rms, dres=dx1, dweight=g["n1"], dbias=g.get("b1"))
+        grads.append(g)
+    return out, dx, dtable, grads[::-1]
+
+
+def _autograd(x, layers, table, dout, mask, *, kind, B, H, S):
+    C = H * 64
+    F = torch.nn.functional
+    leaf = lambda t: t.double().requires_grad_(True)  # noqa: E731
+    x0, tab = leaf(x), None if table is None else leaf(table)
+    ws = [{k: leaf(v) for k, v in w.items()} for w in layers]
+    idx = None if table is None else ref.bucket_index(S, 32, 128, False, x.device)
+    rms, scale = kind == "t5", 1.0 if kind == "t5" else 0.125
+    norm = lambda t, w, b: t / torch.sqrt((t * t).mean(1, keepdim=True) + 1e-6) * w if rms else F.layer_norm(t, (C,), w, b, 1e-6)  # noqa: E731
+    y = x0
+    for w in ws:
+        q, k, v = ((norm(y, w["n1"], w.get("b1")) @ w["qkv"].t())[:, i * C:(i + 1) * C].reshape(B, S, H, 64).transpose(1, 2) for i in range(3))
+        s = q @ k.transpose(2, 3) * scale
+        if tab is not None:
+            s = s + tab[idx].permute(2, 0, 1)
+        if mask is not None:
+            s = s.masked_fill(~mask[:, None, None, :], float("-inf"))
+        if kind == "clip":
+            s = s.masked_fill(torch.ones(S, S, dtype=torch.bool, device=x.device).triu(1), float("-inf"))
+        y = y + (torch.softmax(s, 3) @ v).transpose(1, 2).reshape(B * S, C) @ w["o"].t()
+        n = norm(y, w["n2"], w.get("b2"))
+        z = n @ w["wg"].t()
+        y = y + (n @ w["wv"].t() * (F.gelu(z, approximate="tanh") if rms else F.silu(z))) @ w["wo"].t()
+    y.backward(dout.double())
+    return y.detach(), x0.grad, None if tab is None else tab.grad, [{k: v.grad for k, v in w.items()} for w in ws]
+
+
+@pytest.mark.parametrize("kind,B,H,F,S", [("t5", 2, 4, 640, 150), ("clip", 3, 2, 512, 77), ("t5", 1, 8, 1024, 512)])
+def test_two_trained_layers(kind, B, H, F, S):
+    layers, table = _weights(kind, H, F, seed=S)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dout = (torch.randn(B * S, H * 64, generator=g, device="cuda").to(BF16) for _ in range(2))
+    mask = None
+    if kind == "t5":
+        mask = torch.arange(S, device="cuda")[None] < torch.tensor([S - 7 * b - 3 for b in range(B)], device="cuda")[:, None]
+    kw = dict(kind=kind, B=B, H=H, S=S)
+    out, dx, dtable, grads = _native(x, layers, table, dout, mask, **kw)
+    torch.cuda.synchronize()
+    want, wdx, wdtable, wgrads = _autograd(x, layers, table, dout, mask, **kw)
+
+    def near(a, b, name):
+        assert torch.isfinite(a).all(), name
+        rel = float((a.double() - b).norm() / b.norm())
+        assert rel <= 12 * U, f"{name}: relative error {rel:.3g}"
+
+    near(out, want, "out")
+    near(dx, wdx, "dx")
+    if table is not None:
+        near(dtable, wdtable, "dtable")
+    for i, (a, b) in enumerate(zip(grads, wgrads)):
+        for n in a:
+            near(a[n], b[n], f"layer {i} {n}")
