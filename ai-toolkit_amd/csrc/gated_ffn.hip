@@ -7,10 +7,10 @@
 // hold gate and value of one output element in the same register slot and h is formed in registers; [u | z] leaves (as bf16) only when a backward pass will want it.
 // Backward: one pass forms [du | dz] (bf16: the operands of the two products; the column sums take the fp32 values), one launch computes dx and both weight gradients.
 //
-// The products share one tile loop (v_mfma_f32_32x32x16_bf16, fp32 accumulators).  K-tiles of 64 go straight from global memory to LDS (buffer loads; rows and K tails outside
-// the buffer arrive as zeros) into a double buffer of 128-byte rows, 16-byte chunks XOR-swizzled by rkey(row).  An operand whose contraction index is contiguous in memory is staged
-// row by row and read as 16-byte row fragments; one whose contraction index is the ROW (W in dx; du and x in dW) is staged the same way, 64 columns by 64 rows, and read with
-// 16-bit transpose reads: no transposed copy of a weight or an activation exists anywhere.
+// The products share one tile loop (v_mfma_f32_32x32x16_bf16, fp32 accumulators).  Stages of 32 contraction elements go straight from global memory to LDS (buffer loads; rows and
+// K tails outside the buffer arrive as zeros), 16-byte chunks XOR-swizzled so that no read meets a bank twice.  An operand whose contraction index is contiguous in memory is
+// read as 16-byte row fragments; one whose contraction index is the ROW (W in dx; du and x in dW) lies in blocks of 64 columns and is read with 16-bit transpose reads: no
+// transposed copy of a weight or an activation exists anywhere.
 #include "common.h"
 #include "aitk_args.h"
 
@@ -73,36 +73,34 @@ __device__ __forceinline__ v4i_t make_srd(const void* base, long bytes) {
 __device__ __forceinline__ void dma16(unsigned dst, unsigned voff, const v4i_t& srd, unsigned soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(srd), "s"(soff) : "memory");
 }
-__device__ __forceinline__ void dma_wait_all() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  asm volatile("" ::: "memory");
-}
 
-// One operand's side of the tile loop: R rows (columns of C's other side) x 64 of the contraction, KC: the contraction index is contiguous in memory.
+constexpr int BK = 32, NST = 4;  // contraction elements of a stage, stages in LDS
+
+// One operand's side of the tile loop: R rows (columns of C's other side) x BK of the contraction, KC: the contraction index is contiguous in memory.
 template <int R, int NT, bool KC>
 struct Operand {
-  static constexpr int BYTES = R * 128, NDMA = R * 8 / NT;
+  static constexpr int BYTES = R * BK * 2, NDMA = BYTES / (NT * 16);
   unsigned voff[KC ? NDMA : 1];
-  int rd[2];  // KC: row fragment address of contraction steps (ks & 1): chunk 2 ks + h; otherwise the transpose reads of row halves lo / hi
-  int rd2;
+  int rd[2];  // KC: the row fragment's address (contraction step ks: ^ 32 ks); otherwise the transpose reads of row halves lo / hi
   const bf16_t* base;
   long ld;
-  long rows;  // rows (KC) or columns (otherwise) of the matrix from the tile's first on
+  int left;  // rows (KC) or columns of the matrix from the tile's first on, at most R
+  int kout;  // KC: first contraction index of this lane's chunk
   __device__ __forceinline__ void init(const bf16_t* p, long ld_, int r0, int count, int tid) {
     ld = ld_;
-    rows = count - r0;
+    left = min(count - r0, R);
     base = KC ? p + (long)r0 * ld : p + r0;
-    const int lane = tid & 63, row = tid >> 3, chunk = (tid & 7) ^ rkey(row);
-    if constexpr (KC) {
+    const int lane = tid & 63, l31 = lane & 31, h = lane >> 5, i = lane & 15, gq = (lane >> 4) & 1;
+    if constexpr (KC) {  // 64-byte rows, four of them per KiB-quarter: chunk ^ (row / 4), so that rows four apart (one bank group) differ
+      const int row = tid >> 2;
+      kout = ((tid & 3) ^ ((row >> 2) & 3)) * 8;
 #pragma unroll
-      for (int i = 0; i < NDMA; ++i) voff[i] = (unsigned)(((row + i * (NT / 8)) * ld + chunk * 8) * 2);
-    } else {
-      voff[0] = (unsigned)((row * ld + chunk * 8) * 2);
-    }
-    const int l31 = lane & 31, h = lane >> 5, i = lane & 15, gq = (lane >> 4) & 1;
-    if constexpr (KC) {
-      rd[0] = l31 * 128 + ((h ^ rkey(l31)) << 4);
-    } else {
+      for (int d = 0; d < NDMA; ++d) voff[d] = (unsigned)(((row + d * (NT / 4)) * ld + kout) * 2);
+      rd[0] = l31 * 64 + ((h ^ ((l31 >> 2) & 3)) << 4);
+    } else {  // blocks of 64 columns: BK rows of 128 bytes, chunk ^ rkey(row)
+      const int row = (tid >> 3) % BK;
+      kout = 0;
+      voff[0] = (unsigned)((row * ld + ((tid & 7) ^ rkey(row)) * 8 + (tid >> 3) / BK * 64) * 2);
 #pragma unroll
       for (int hi = 0; hi < 2; ++hi) {
         const int k = 8 * h + 4 * hi + (i >> 2), c = 2 * gq + ((i & 3) >> 1);
@@ -111,34 +109,19 @@ struct Operand {
     }
   }
   __device__ __forceinline__ void rebase(const bf16_t* p, int r0) { base = KC ? p + (long)r0 * ld : p + r0; }
-  // K-tile [k0, k0 + 64) of a segment of K: tile rows / columns past the matrix and k >= K arrive as zeros (columns past it: the neighbour's, never stored)
-  __device__ __forceinline__ void stage(unsigned dst, int k0, int K, int tid, int wave) const {
-    if constexpr (KC) {
-      const long left = rows < R ? rows : R;
-      const v4i_t srd = make_srd(base, ((left - 1) * ld + K) * 2);
-      const bool tail = k0 + 64 > K;
-      const bool out = tail && k0 + (((tid & 7) ^ rkey(tid >> 3)) * 8) >= K;
-#pragma unroll
-      for (int i = 0; i < NDMA; ++i)
-        dma16(__builtin_amdgcn_readfirstlane(dst + i * (NT * 16) + wave * 1024), out ? 0x80000000u : voff[i], srd, (unsigned)k0 * 2);
-    } else {
-      const int kl = K - k0 < 64 ? K - k0 : 64;
-      const long cols = rows < R ? rows : R;
-      const v4i_t srd = make_srd(base + (long)k0 * ld, ((long)(kl - 1) * ld + cols) * 2);
-#pragma unroll
-      for (int i = 0; i < NDMA; ++i) {
-        // DMA i fills rows [i * NT / 8 % 64, ...) of 64-column block i * NT / 512
-        const int blk = i * NT / 512, k = i * (NT / 8) % 64;
-        dma16(__builtin_amdgcn_readfirstlane(dst + blk * 8192 + k * 128 + wave * 1024), voff[0] + (unsigned)(k * ld * 2) + blk * 128, srd, 0);
-      }
-    }
+  // DMA d of stage [k0, k0 + BK) of a segment of K: rows past the matrix and k >= K arrive as zeros (columns past it: the neighbour's or zeros, never stored)
+  __device__ __forceinline__ void stage(unsigned dst, int k0, int K, int wave, int d) const {
+    const unsigned at = __builtin_amdgcn_readfirstlane(dst + d * (NT * 16) + wave * 1024);
+    if constexpr (KC) dma16(at, k0 + kout >= K ? 0x80000000u : voff[d], make_srd(base, ((long)(left - 1) * ld + K) * 2), (unsigned)k0 * 2);
+    else  // NT / (8 BK) blocks of 64 columns at a time
+      dma16(at, voff[0] + d * (NT / (8 * BK)) * 128, make_srd(base + (long)k0 * ld, ((long)(min(K - k0, BK) - 1) * ld + left) * 2), 0);
   }
-  // fragment of the 32 rows from r on (a multiple of 32), contraction step ks
+  // fragment of the 32 rows from r on (a multiple of 32), contraction step ks of the stage
   __device__ __forceinline__ s16x8_t frag(const lds_char* t, int r, int ks) const {
     if constexpr (KC) {
-      return *reinterpret_cast<const __attribute__((address_space(3))) s16x8_t*>(t + r * 128 + (rd[0] ^ (ks * 32)));
+      return *reinterpret_cast<const __attribute__((address_space(3))) s16x8_t*>(t + r * 64 + (rd[0] ^ (ks * 32)));
     } else {
-      const lds_char* q = t + (r >> 6) * 8192 + ks * 2048;
+      const lds_char* q = t + (r >> 6) * (BK * 128) + ks * 2048;
       const int flip = (r & 32) * 2;  // the second 32 columns of a block: chunk + 4
       const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(q + (rd[0] ^ flip)));
       const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(q + (rd[1] ^ flip)));
@@ -147,61 +130,115 @@ struct Operand {
   }
 };
 
-// The tile loop.  WR x WC waves; a wave owns MB x 32 rows and, of each half of the tile's columns, 32: columns wc * 32 + ni * BN / 2.
+// The tile loop.  WR x WC waves; a wave owns MB x 32 rows and, of each half of the tile's columns, NB / 2 x 32.
+// Four stages of 32 contraction elements: while stage t is multiplied, t + 1 has landed for every wave (its first fragments are read ahead of the barrier that
+// separates the two, so the matrix units go on right behind it), t + 2 and t + 3 are on their way; one barrier a stage.
 template <int BM, int BN, int WR, int WC, bool AK, bool BKC, bool PAIR>
 struct TileLoop {
-  static constexpr int NT = WR * WC * 64, MB = BM / WR / 32;
-  static_assert(BN == WC * 64, "two 32-column blocks per wave");
-  static constexpr int BUF = (BM + BN) * 128;
-  f32x16_t acc[MB][2];
+  static constexpr int NT = WR * WC * 64, MB = BM / WR / 32, NB = BN / WC / 32;
+  static constexpr int STAGE = (BM + BN) * BK * 2, BHALF = BN / 2 * BK * 2, DMAS = STAGE / (NT * 16);
+  typedef Operand<BM, NT, AK> OpA;
+  typedef Operand<PAIR ? BN / 2 : BN, NT, BKC> OpB;
+  static_assert(DMAS == 4 || DMAS == 8, "the counted waits below");
+  f32x16_t acc[MB][NB];
+  // first column, within the half tile, of a wave's block j % (NB / 2)
+  static __device__ __forceinline__ int col(int wc, int j) { return (wc * (NB / 2) + j % (NB / 2)) * 32; }
   __device__ __forceinline__ void run(const Prod& p, int m0, int n0, char* smem) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WC, wc = wave % WC;
     lds_char* const sm = (lds_char*)smem;
-    Operand<BM, NT, AK> A;
-    Operand<PAIR ? BN / 2 : BN, NT, BKC> B, B2;
+    OpA A;
+    OpB B, B2;
     A.init(p.A[0], p.lda, m0, p.M, tid);
     B.init(p.B[0], p.ldb, n0, p.N, tid);
     if constexpr (PAIR) B2.init(p.B[1], p.ldb, n0, p.N, tid);
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int kt_seg = (p.K + 63) / 64, nkt = kt_seg * p.nseg;
-    auto stage = [&](int t, int buf) {
-      const int s = t >= kt_seg ? 1 : 0, k0 = (t - s * kt_seg) * 64;
-      if (!PAIR && t == kt_seg) {
+    const int K = p.K, kt_seg = (K + BK - 1) / BK, nkt = kt_seg * p.nseg;
+    int ts = 0, k0 = 0;  // the stage issued next, its first contraction index within its segment
+    auto issue = [&](int d) {  // DMA d = 0 .. DMAS - 1 of stage ts (ts < nkt), in order
+      if (d == 0 && !PAIR && ts == kt_seg) {
         A.rebase(p.A[1], m0);
         B.rebase(p.B[1], n0);
+        k0 = 0;
       }
-      const unsigned dst = (unsigned)(size_t)sm + buf * BUF;
-      A.stage(dst, k0, p.K, tid, wave);
-      B.stage(dst + BM * 128, k0, p.K, tid, wave);
-      if constexpr (PAIR) B2.stage(dst + BM * 128 + BN * 64, k0, p.K, tid, wave);
+      const unsigned dst = (unsigned)(size_t)sm + (ts & (NST - 1)) * STAGE;
+      if (d < OpA::NDMA) A.stage(dst, k0, K, wave, d);
+      else if (d < OpA::NDMA + OpB::NDMA) B.stage(dst + BM * BK * 2, k0, K, wave, d - OpA::NDMA);
+      else if constexpr (PAIR) B2.stage(dst + BM * BK * 2 + BHALF, k0, K, wave, d - OpA::NDMA - OpB::NDMA);
+      if (d == DMAS - 1) {
+        ++ts;
+        k0 += BK;
+      }
     };
-    stage(0, 0);
-    dma_wait_all();
-    __syncthreads();
-    for (int t = 0; t < nkt; ++t) {
-      const lds_char* at = sm + (t & 1) * BUF;
-      const lds_char* bt = at + BM * 128;
-      if (t + 1 < nkt) stage(t + 1, (t + 1) & 1);
+    s16x8_t af[2][MB], bf[2][NB];
+    auto read_a = [&](int set, int t, int ks, int i) { af[set][i] = A.frag(sm + (t & (NST - 1)) * STAGE, wr * (BM / WR) + i * 32, ks); };
+    auto read_b = [&](int set, int t, int ks, int j) {
+      const lds_char* bt = sm + (t & (NST - 1)) * STAGE + BM * BK * 2;
+      const int half = j / (NB / 2);
+      bf[set][j] = PAIR ? B.frag(bt + half * BHALF, col(wc, j), ks) : B.frag(bt, half * (BN / 2) + col(wc, j), ks);
+    };
+    // One contraction step: the products of `set`, row block by row block.  Behind the first row block go half of a stage's DMAs and the other set's reads: in front of it the
+    // waves, which come from one barrier, would all wait for the address unit with the matrix units idle; later, the wait in front of the next step would find the reads under way
+    // (M 4096, K 4096, F 10240: dx 620 us with the reads behind the second block, 571 us here).
+    auto step = [&](int set, bool rd, int t, int ks, bool more, int d0) {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        s16x8_t af[MB], bf[2];
+      for (int i = 0; i < MB; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) bf[j] = B.frag(bt, j * (BN / 2) + wc * 32, ks);
+        for (int j = 0; j < NB; ++j) acc[i][j] = mfma32(bf[set][j], af[set][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == 0 && more) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) af[i] = A.frag(at, wr * (BM / WR) + i * 32, ks);
+          for (int k = 0; k < DMAS / 2; ++k) issue(d0 + k);
+        }
+        if (i == 0 && rd) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+          for (int j = 0; j < NB; ++j) read_b(set ^ 1, t, ks, j);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) acc[i][j] = mfma32(bf[j], af[i], acc[i][j]);
+          for (int k = 0; k < MB; ++k) read_a(set ^ 1, t, ks, k);
+        }
       }
-      dma_wait_all();
-      __syncthreads();
+    };
+    // a wave's own DMAs are in order: all but the newest n stages' have landed
+    auto landed = [&](int n) {
+      if (n >= 2) {
+        if constexpr (DMAS == 8) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      } else if (n == 1) {
+        if constexpr (DMAS == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+    };
+    auto barrier = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll 1
+    for (int i = 0; i < 3 && i < nkt; ++i) {
+#pragma unroll
+      for (int d = 0; d < DMAS; ++d) issue(d);
+    }
+    landed(nkt - 1);
+    barrier();
+#pragma unroll
+    for (int j = 0; j < NB; ++j) read_b(0, 0, 0, j);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) read_a(0, 0, 0, i);
+#pragma unroll 1
+    for (int t = 0; t < nkt; ++t) {
+      landed(t + 2 < nkt ? 1 : 0);  // stage t + 1 has landed (this wave's part) ...
+      barrier();                    // ... and everybody's; everybody is through with stage t - 1, whose place stage t + 3 takes
+      const bool more = ts < nkt;
+      step(0, true, t, 1, more, 0);
+      step(1, t + 1 < nkt, t + 1, 0, more, DMAS / 2);
     }
   }
 };
@@ -213,8 +250,14 @@ __device__ __forceinline__ void tile_coords(int id, int ntiles, int tm, int tn, 
   m = first + (l % per) % gm;
   n = (l % per) / gm;
 }
-__device__ __forceinline__ void store4(bf16_t* p, float a, float b, float c, float d) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(a, b), pack2bf(c, d));
+
+// Columns 8 h .. 8 h + 7 of a 16-column group, where h is the lane's half of the wave: a lane's registers hold columns 4 h .. + 3 (v) and 8 + 4 h .. + 3 (w); the halves trade
+// so that a lane stores 16 bytes.  All lanes take part.
+__device__ __forceinline__ uint4 trade(const float (&v)[4], const float (&w)[4]) {
+  typedef unsigned u2_t __attribute__((ext_vector_type(2)));
+  const u2_t x = __builtin_amdgcn_permlane32_swap(pack2bf(v[0], v[1]), pack2bf(w[0], w[1]), false, false);
+  const u2_t y = __builtin_amdgcn_permlane32_swap(pack2bf(v[2], v[3]), pack2bf(w[2], w[3]), false, false);
+  return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
 template <int BM, int BN, int WR, int WC>
@@ -224,39 +267,50 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) 
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN / 2 - 1) / (BN / 2);
   int ti, tj;
   tile_coords(blockIdx.x, tm * tn, tm, tn, ti, tj);
-  TileLoop<BM, BN, WR, WC, true, true, true> T;
+  typedef TileLoop<BM, BN, WR, WC, true, true, true> Loop;
+  Loop T;
   T.run(p, ti * BM, tj * (BN / 2), smem);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
-  const int m_w = ti * BM + (wave / WC) * (BM / WR), n_w = tj * (BN / 2) + (wave % WC) * 32 + 4 * h;
+  const int m_w = ti * BM + (wave / WC) * (BM / WR);
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int n = n_w + 8 * g;
-    if (n >= p.N) continue;
-    float bv[4] = {}, bg[4] = {};
-    if (a.bv) {
+  for (int j = 0; j < Loop::NB / 2; ++j) {
+    const int n_w = tj * (BN / 2) + Loop::col(wave % WC, j);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bv[e] = bf2f(a.bv[n + e]);
-    }
-    if (a.bg) {
+    for (int q = 0; q < 2; ++q) {  // 16 columns at a time
+      const int n0 = n_w + 16 * q + 4 * h, n = n_w + 16 * q + 8 * h;
+      float bv[2][4] = {}, bg[2][4] = {};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bg[e] = bf2f(a.bg[n + e]);
-    }
+      for (int k = 0; k < 2; ++k)
+        if (n0 + 8 * k < p.N) {
 #pragma unroll
-    for (int i = 0; i < T.MB; ++i) {
-      const int m = m_w + i * 32 + l31;
-      if (m >= p.M) continue;
-      float z[4], u[4], o[4];
+          for (int e = 0; e < 4; ++e) {
+            if (a.bv) bv[k][e] = bf2f(a.bv[n0 + 8 * k + e]);
+            if (a.bg) bg[k][e] = bf2f(a.bg[n0 + 8 * k + e]);
+          }
+        }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        z[e] = T.acc[i][0][4 * g + e] + bg[e];
-        u[e] = T.acc[i][1][4 * g + e] + bv[e];
-        o[e] = u[e] * act_f(z[e], a.act);
-      }
-      store4(p.C + (long)m * p.ldc + n, o[0], o[1], o[2], o[3]);
-      if (a.hg) {
-        bf16_t* q = a.hg + (long)m * a.ld_hg + n;
-        store4(q, u[0], u[1], u[2], u[3]);
-        store4(q + p.N, z[0], z[1], z[2], z[3]);
+      for (int i = 0; i < Loop::MB; ++i) {
+        const int m = m_w + i * 32 + l31;
+        float z[2][4], u[2][4], o[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            z[k][e] = T.acc[i][j][8 * q + 4 * k + e] + bg[k][e];
+            u[k][e] = T.acc[i][j + Loop::NB / 2][8 * q + 4 * k + e] + bv[k][e];
+            o[k][e] = u[k][e] * act_f(z[k][e], a.act);
+          }
+        const bool in = m < p.M && n < p.N;
+        const uint4 ov = trade(o[0], o[1]);
+        if (in) *reinterpret_cast<uint4*>(p.C + (long)m * p.ldc + n) = ov;
+        if (a.hg) {
+          const uint4 uv = trade(u[0], u[1]), zv = trade(z[0], z[1]);
+          bf16_t* r = a.hg + (long)m * a.ld_hg + n;
+          if (in) {
+            *reinterpret_cast<uint4*>(r) = uv;
+            *reinterpret_cast<uint4*>(r + p.N) = zv;
+          }
+        }
       }
     }
   }
@@ -264,20 +318,24 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) 
 
 template <int BM, int BN, int WR, int WC, bool AK>
 __device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, char* smem) {
-  TileLoop<BM, BN, WR, WC, AK, false, false> T;
+  typedef TileLoop<BM, BN, WR, WC, AK, false, false> Loop;
+  Loop T;
   T.run(p, ti * BM, tj * BN, smem);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
-  const int m_w = ti * BM + (wave / WC) * (BM / WR), n_w = tj * BN + (wave % WC) * 32 + 4 * h;
+  const int m_w = ti * BM + (wave / WC) * (BM / WR);
 #pragma unroll
-  for (int i = 0; i < T.MB; ++i) {
+  for (int i = 0; i < Loop::MB; ++i) {
     const int m = m_w + i * 32 + l31;
-    if (m >= p.M) continue;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < Loop::NB; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n_w + j * (BN / 2) + 8 * g;
-        if (n < p.N) store4(p.C + (long)m * p.ldc + n, T.acc[i][j][4 * g], T.acc[i][j][4 * g + 1], T.acc[i][j][4 * g + 2], T.acc[i][j][4 * g + 3]);
+      for (int q = 0; q < 2; ++q) {
+        const int n = tj * BN + j / (Loop::NB / 2) * (BN / 2) + Loop::col(wave % WC, j) + 16 * q + 8 * h;
+        float v[2][4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e >> 2][e & 3] = T.acc[i][j][8 * q + e];
+        const uint4 c = trade(v[0], v[1]);
+        if (m < p.M && n < p.N) *reinterpret_cast<uint4*>(p.C + (long)m * p.ldc + n) = c;
       }
   }
 }
@@ -394,8 +452,8 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   hipStream_t s = (hipStream_t)stream;
   const int64_t big = tiles(q->M, q->F, 256, 128), small = tiles(q->M, q->F, 128, 64);
   if (small > 0x7fffffff) return AITK_ERR_SHAPE;
-  if (big >= 128) return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)big, 512, 131072, a, s);
-  return launch(gated_ffn_fwd_kernel<128, 128, 2, 2>, (unsigned)small, 256, 65536, a, s);
+  if (big >= 128) return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)big, 512, NST * 512 * BK * 2, a, s);
+  return launch(gated_ffn_fwd_kernel<128, 128, 2, 2>, (unsigned)small, 256, NST * 256 * BK * 2, a, s);
 }
 
 extern "C" int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t F, int32_t bias_grads) {
@@ -436,6 +494,6 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
   }
   if (!small) return AITK_OK;
   if (small > 0x7fffffff) return AITK_ERR_SHAPE;
-  if (big >= 128) return launch(gated_ffn_grads_kernel<256, 256, 2, 4>, (unsigned)big, 512, 131072, a, s);
-  return launch(gated_ffn_grads_kernel<128, 128, 2, 2>, (unsigned)small, 256, 65536, a, s);
+  if (big >= 128) return launch(gated_ffn_grads_kernel<256, 256, 2, 4>, (unsigned)big, 512, NST * 512 * BK * 2, a, s);
+  return launch(gated_ffn_grads_kernel<128, 128, 2, 2>, (unsigned)small, 256, NST * 256 * BK * 2, a, s);
 }
