@@ -320,7 +320,7 @@ def lib():
     L.aitk_attn_relpos_bwd_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.aitk_attn_relpos_buckets.argtypes = [i32, i32, i32, vp]
     L.aitk_gated_ffn_bwd_workspace_bytes.restype = C.c_int64
-    L.aitk_gated_ffn_bwd_workspace_bytes.argtypes = [i32, i32, i32]
+    L.aitk_gated_ffn_bwd_workspace_bytes.argtypes = [i32] * 7
     _lib = L
     return L
 

@@ -19,7 +19,6 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 
 enum { ACT_GELU_TANH = 0, ACT_GELU_ERF = 1, ACT_SILU = 2 };
-enum { FWD = 0, GRADS = 1 };
 
 // one product of the tile loop: C[m][n] = sum over segments s, k of A[s](m, k) B[s](n, k)
 struct Prod {
@@ -27,10 +26,12 @@ struct Prod {
   const bf16_t* B[2];
   bf16_t* C;
   long lda, ldb, ldc;
+  float* part;        // split > 1: [split][M][N] partial sums instead of C
   int M, N, K, nseg;  // K: per segment
+  int split, a_rows;  // pieces of the contraction (workgroups of their own); a_rows: A's contraction index is its row (weight gradients)
 };
 struct FfnArgs {
-  Prod p[3];  // FWD: p[0] (B[0] = Wg, B[1] = Wv); GRADS: dx, dWv, dWg (M = 0: not wanted)
+  Prod p[3];  // forward: p[0] (B[0] = Wg, B[1] = Wv); backward: dx, dWv, dWg, the longest pieces first (M = 0: not wanted)
   const bf16_t* bv;
   const bf16_t* bg;
   bf16_t* hg;  // [M, 2F] = [u | z], may be NULL
@@ -143,7 +144,7 @@ struct TileLoop {
   f32x16_t acc[MB][NB];
   // first column, within the half tile, of a wave's block j % (NB / 2)
   static __device__ __forceinline__ int col(int wc, int j) { return (wc * (NB / 2) + j % (NB / 2)) * 32; }
-  __device__ __forceinline__ void run(const Prod& p, int m0, int n0, char* smem) {
+  __device__ __forceinline__ void run(const Prod& p, int m0, int n0, char* smem, int piece = 0) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WC, wc = wave % WC;
     lds_char* const sm = (lds_char*)smem;
@@ -158,8 +159,14 @@ struct TileLoop {
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int K = p.K, kt_seg = (K + BK - 1) / BK, nkt = kt_seg * p.nseg;
-    int ts = 0, k0 = 0;  // the stage issued next, its first contraction index within its segment
+    const int K = p.K, kt_seg = (K + BK - 1) / BK, all = kt_seg * p.nseg;
+    const int t0 = PAIR ? 0 : (int)((long)all * piece / p.split), nkt = PAIR ? all : (int)((long)all * (piece + 1) / p.split);  // this piece's stages [t0, nkt)
+    int ts = t0, k0 = ts * BK;  // the stage issued next, its first contraction index within its segment
+    if (!PAIR && ts > kt_seg) {
+      A.rebase(p.A[1], m0);
+      B.rebase(p.B[1], n0);
+      k0 -= kt_seg * BK;
+    }
     auto issue = [&](int d) {  // DMA d = 0 .. DMAS - 1 of stage ts (ts < nkt), in order
       if (d == 0 && !PAIR && ts == kt_seg) {
         A.rebase(p.A[1], m0);
@@ -222,18 +229,18 @@ struct TileLoop {
       __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll 1
-    for (int i = 0; i < 3 && i < nkt; ++i) {
+    for (int i = 0; i < 3 && ts < nkt; ++i) {
 #pragma unroll
       for (int d = 0; d < DMAS; ++d) issue(d);
     }
-    landed(nkt - 1);
+    landed(nkt - t0 - 1);
     barrier();
 #pragma unroll
-    for (int j = 0; j < NB; ++j) read_b(0, 0, 0, j);
+    for (int j = 0; j < NB; ++j) read_b(0, t0, 0, j);
 #pragma unroll
-    for (int i = 0; i < MB; ++i) read_a(0, 0, 0, i);
+    for (int i = 0; i < MB; ++i) read_a(0, t0, 0, i);
 #pragma unroll 1
-    for (int t = 0; t < nkt; ++t) {
+    for (int t = t0; t < nkt; ++t) {
       landed(t + 2 < nkt ? 1 : 0);  // stage t + 1 has landed (this wave's part) ...
       barrier();                    // ... and everybody's; everybody is through with stage t - 1, whose place stage t + 3 takes
       const bool more = ts < nkt;
@@ -317,10 +324,10 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) 
 }
 
 template <int BM, int BN, int WR, int WC, bool AK>
-__device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, char* smem) {
+__device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, int piece, char* smem) {
   typedef TileLoop<BM, BN, WR, WC, AK, false, false> Loop;
   Loop T;
-  T.run(p, ti * BM, tj * BN, smem);
+  T.run(p, ti * BM, tj * BN, smem, piece);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
   const int m_w = ti * BM + (wave / WC) * (BM / WR);
 #pragma unroll
@@ -330,7 +337,17 @@ __device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, char* s
     for (int j = 0; j < Loop::NB; ++j)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const int n = tj * BN + j / (Loop::NB / 2) * (BN / 2) + Loop::col(wave % WC, j) + 16 * q + 8 * h;
+        const int n16 = tj * BN + j / (Loop::NB / 2) * (BN / 2) + Loop::col(wave % WC, j) + 16 * q, n = n16 + 8 * h;
+        if (p.split > 1) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int c = n16 + 8 * k + 4 * h;
+            if (m < p.M && c < p.N)
+              *reinterpret_cast<f32x4_t*>(p.part + ((long)piece * p.M + m) * p.N + c) =
+                  f32x4_t{T.acc[i][j][8 * q + 4 * k], T.acc[i][j][8 * q + 4 * k + 1], T.acc[i][j][8 * q + 4 * k + 2], T.acc[i][j][8 * q + 4 * k + 3]};
+          }
+          continue;
+        }
         float v[2][4];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e >> 2][e & 3] = T.acc[i][j][8 * q + e];
@@ -340,7 +357,8 @@ __device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, char* s
   }
 }
 
-// dx and the two weight gradients in one launch: dx's tiles are few and long (a contraction over 2 F), the weights' many and short; the long ones go first
+// dx and the two weight gradients in one launch.  dx contracts over 2 F and has few tiles, the weights contract over M and have many: pieces of a product's contraction
+// (plan() below) make the workgroups alike; the longest go first.
 template <int BM, int BN, int WR, int WC>
 __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_grads_kernel(FfnArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -349,15 +367,37 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_grads_kernel(FfnArgs a
   for (int q = 0; q < 3; ++q) {
     const Prod& p = a.p[q];
     const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, n = tm * tn;
-    if (id >= n) {
-      id -= n;
+    if (id >= n * p.split) {
+      id -= n * p.split;
       continue;
     }
     int ti, tj;
-    tile_coords(id, n, tm, tn, ti, tj);
-    if (q == 0) grad_tile<BM, BN, WR, WC, true>(p, ti, tj, smem);
-    else grad_tile<BM, BN, WR, WC, false>(p, ti, tj, smem);
+    const int piece = id / n;
+    tile_coords(id - piece * n, n, tm, tn, ti, tj);
+    if (p.a_rows) grad_tile<BM, BN, WR, WC, false>(p, ti, tj, piece, smem);
+    else grad_tile<BM, BN, WR, WC, true>(p, ti, tj, piece, smem);
     return;
+  }
+}
+// the pieces' fp32 sums, in their order, rounded once: 8 columns per thread
+__global__ __launch_bounds__(256) void gated_ffn_join_kernel(FfnArgs a) {
+  const Prod& p = a.p[blockIdx.y];
+  if (p.M <= 0 || p.split <= 1) return;
+  const int nc = p.N / 8;
+  const long total = (long)p.M * nc, plane = (long)p.M * p.N;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    const float* q = p.part + i * 8;
+    float v[8] = {};
+    for (int s = 0; s < p.split; ++s) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(q + s * plane), y = *reinterpret_cast<const f32x4_t*>(q + s * plane + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] += x[e];
+        v[4 + e] += y[e];
+      }
+    }
+    const long m = i / nc;
+    *reinterpret_cast<uint4*>(p.C + m * p.ldc + (i - m * nc) * 8) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
   }
 }
 
@@ -435,6 +475,65 @@ int launch(K kernel, unsigned grid, unsigned threads, size_t lds, const FfnArgs&
   return AITK_OK;
 }
 int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return m <= 0 ? 0 : ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
+
+// How a backward pass is cut into workgroups: 256 x 256 tiles (one workgroup per CU) or 128 x 128 (two), and into how many pieces each product's contraction goes.  The time of a
+// plan is estimated from what was measured here: 0.9 us for a stage of a large tile, 0.6 us for one of two small ones side by side, 6 / 3 us for a workgroup's start and end,
+// 8 bytes per element and piece through memory at 4.5 TB/s and 5 us for the launch that joins them; a last round of workgroups is taken as half empty.
+struct Plan {
+  bool big;
+  int split[3];
+};
+Plan plan(int M, int K, int F, bool dx, int ndw) {
+  Plan best = {};
+  double best_us = 1e30;
+  for (int big = 0; big < 2; ++big) {
+    const int b = big ? 256 : 128, slots = big ? 256 : 512;
+    const double stage = big ? 0.9 : 0.6, ends = big ? 6.0 : 3.0;
+    const double n[2] = {dx ? (double)tiles(M, K, b, b) : 0.0, (double)ndw * tiles(F, K, b, b)};
+    const int st[2] = {2 * ((F + BK - 1) / BK), (M + BK - 1) / BK};
+    for (int chunk = 16; chunk <= 16384; chunk += chunk / 2) {
+      int s[2];
+      double work = 0, longest = 0, shortest = 1e30, bytes = 0, count = 0;
+      for (int i = 0; i < 2; ++i) {
+        s[i] = (st[i] + chunk - 1) / chunk;
+        if (s[i] > 16) s[i] = 16;
+        if (n[i] == 0) continue;
+        const double us = ((st[i] + s[i] - 1) / s[i]) * stage + ends;
+        work += n[i] * s[i] * us;
+        count += n[i] * s[i];
+        if (us > longest) longest = us;
+        if (us < shortest) shortest = us;
+        if (s[i] > 1) bytes += (i ? (double)ndw * F : (double)M) * K * 8.0 * s[i];
+      }
+      double us = count <= slots ? longest : work / slots + 0.5 * shortest;
+      if (us < longest) us = longest;
+      if (bytes > 0) us += bytes / 4.5e6 + 5.0;
+      if (us < best_us) {
+        best_us = us;
+        best.big = big;
+        best.split[0] = s[0];
+        best.split[1] = best.split[2] = s[1];
+      }
+    }
+  }
+  return best;
+}
+struct Layout {  // of the backward's workspace, in bytes
+  int64_t sums, part[3], end;
+};
+Layout layout(const Plan& pl, int M, int K, int F, bool dx, bool dwv, bool dwg, bool db) {
+  Layout l;
+  int64_t at = ((int64_t)M * 2 * F * 2 + 255) / 256 * 256;  // [du | dz]
+  l.sums = at;
+  if (db) at += ((int64_t)((M + DU_ROWS - 1) / DU_ROWS) * 2 * F * 4 + 255) / 256 * 256;
+  const bool want[3] = {dx, dwv, dwg};
+  for (int i = 0; i < 3; ++i) {
+    l.part[i] = at;
+    if (want[i] && pl.split[i] > 1) at += (int64_t)pl.split[i] * (i ? F : M) * K * 4;
+  }
+  l.end = at;
+  return l;
+}
 }  // namespace
 
 extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t stream) {
@@ -443,7 +542,7 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   if (bad(q->x, q->ldx, q->K) || bad(q->w_val, q->ldw, q->K) || mis16(q->w_gate) || bad(q->out, q->ld_out, q->F) || (q->hg && bad(q->hg, q->ld_hg, 2 * (int64_t)q->F)))
     return AITK_ERR_ALIGN;
   FfnArgs a = {};
-  a.p[0] = Prod{{q->x, q->x}, {q->w_gate, q->w_val}, q->out, q->ldx, q->ldw, q->ld_out, q->M, q->F, q->K, 1};
+  a.p[0] = Prod{{q->x, q->x}, {q->w_gate, q->w_val}, q->out, q->ldx, q->ldw, q->ld_out, nullptr, q->M, q->F, q->K, 1, 1, 0};
   a.bv = q->b_val;
   a.bg = q->b_gate;
   a.hg = q->hg;
@@ -452,14 +551,15 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   hipStream_t s = (hipStream_t)stream;
   const int64_t big = tiles(q->M, q->F, 256, 128), small = tiles(q->M, q->F, 128, 64);
   if (small > 0x7fffffff) return AITK_ERR_SHAPE;
-  if (big >= 128) return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)big, 512, NST * 512 * BK * 2, a, s);
+  // A round of small tiles (two workgroups per CU) takes 0.55 to 0.75 of a round of large ones: 512 x 4096 x 10240 (1 round against 2) 113 us large, 137 us small;
+  // 4096 x 640 x 2560 (2 against 3) 57.8 and 49.2; 2048 x 2048 x 5120 (2 against 3) 121.5 and 119.8; 256 x 4096 x 10240 (1 against 1) 92 and 74; 2048 x 4096 x 10240 (3 against 5) 366 and 450.
+  if (20 * ((big + 255) / 256) <= 13 * ((small + 511) / 512)) return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)big, 512, NST * 512 * BK * 2, a, s);
   return launch(gated_ffn_fwd_kernel<128, 128, 2, 2>, (unsigned)small, 256, NST * 256 * BK * 2, a, s);
 }
 
-extern "C" int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t F, int32_t bias_grads) {
-  if (M <= 0 || F <= 0) return 0;
-  const int64_t du = ((int64_t)M * 2 * F * 2 + 15) / 16 * 16;
-  return du + (bias_grads ? (int64_t)((M + DU_ROWS - 1) / DU_ROWS) * 2 * F * 4 : 0);
+extern "C" int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t K, int32_t F, int32_t dx, int32_t dw_val, int32_t dw_gate, int32_t bias_grads) {
+  if (M <= 0 || K <= 0 || F <= 0) return 0;
+  return layout(plan(M, K, F, dx != 0, (dw_val != 0) + (dw_gate != 0)), M, K, F, dx != 0, dw_val != 0, dw_gate != 0, bias_grads != 0).end;
 }
 
 extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t stream) {
@@ -471,8 +571,11 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
     return AITK_ERR_ALIGN;
   const int M = q->M, F = q->F, K = q->K;
   if (2 * (int64_t)F > (1 << 20)) return AITK_ERR_SHAPE;
-  bf16_t* du = reinterpret_cast<bf16_t*>(q->ws);
-  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(q->ws) + ((int64_t)M * 2 * F * 2 + 15) / 16 * 16);
+  const Plan pl = plan(M, K, F, q->dx != nullptr, (q->dw_val != nullptr) + (q->dw_gate != nullptr));
+  const Layout l = layout(pl, M, K, F, q->dx != nullptr, q->dw_val != nullptr, q->dw_gate != nullptr, db);
+  char* ws = reinterpret_cast<char*>(q->ws);
+  bf16_t* du = reinterpret_cast<bf16_t*>(ws);
+  float* part = reinterpret_cast<float*>(ws + l.sums);
   hipStream_t s = (hipStream_t)stream;
   const int nchunk = (M + DU_ROWS - 1) / DU_ROWS;
   const dim3 grid((F / 8 + 63) / 64, nchunk);
@@ -484,16 +587,27 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
     AITK_LAUNCH_CHECK();
   }
   FfnArgs a = {};
-  if (q->dx) a.p[0] = Prod{{du, du + F}, {q->w_val, q->w_gate}, q->dx, 2 * (long)F, q->ldw, q->ld_dx, M, K, F, 2};
-  if (q->dw_val) a.p[1] = Prod{{du, du}, {q->x, q->x}, q->dw_val, 2 * (long)F, q->ldx, q->ld_dw, F, K, M, 1};
-  if (q->dw_gate) a.p[2] = Prod{{du + F, du + F}, {q->x, q->x}, q->dw_gate, 2 * (long)F, q->ldx, q->ld_dw, F, K, M, 1};
-  int64_t big = 0, small = 0;
+  const auto partial = [&](int i) { return pl.split[i] > 1 ? reinterpret_cast<float*>(ws + l.part[i]) : nullptr; };
+  const Prod x = {{du, du + F}, {q->w_val, q->w_gate}, q->dx, 2 * (long)F, q->ldw, q->ld_dx, partial(0), q->dx ? M : 0, K, F, 2, pl.split[0], 0};
+  const Prod wv = {{du, du}, {q->x, q->x}, q->dw_val, 2 * (long)F, q->ldx, q->ld_dw, partial(1), q->dw_val ? F : 0, K, M, 1, pl.split[1], 1};
+  const Prod wg = {{du + F, du + F}, {q->x, q->x}, q->dw_gate, 2 * (long)F, q->ldx, q->ld_dw, partial(2), q->dw_gate ? F : 0, K, M, 1, pl.split[2], 1};
+  const bool dx_first = 2 * (int64_t)F * pl.split[1] >= (int64_t)M * pl.split[0];
+  a.p[dx_first ? 0 : 2] = x;
+  a.p[dx_first ? 1 : 0] = wv;
+  a.p[dx_first ? 2 : 1] = wg;
+  int64_t n = 0, joined = 0;
+  const int b = pl.big ? 256 : 128;
   for (const Prod& p : a.p) {
-    big += tiles(p.M, p.N, 256, 256);
-    small += tiles(p.M, p.N, 128, 128);
+    n += tiles(p.M, p.N, b, b) * p.split;
+    if (p.M > 0 && p.split > 1 && (int64_t)p.M * p.N > joined) joined = (int64_t)p.M * p.N;
   }
-  if (!small) return AITK_OK;
-  if (small > 0x7fffffff) return AITK_ERR_SHAPE;
-  if (big >= 128) return launch(gated_ffn_grads_kernel<256, 256, 2, 4>, (unsigned)big, 512, NST * 512 * BK * 2, a, s);
-  return launch(gated_ffn_grads_kernel<128, 128, 2, 2>, (unsigned)small, 256, NST * 256 * BK * 2, a, s);
+  if (!n) return AITK_OK;
+  if (n > 0x7fffffff) return AITK_ERR_SHAPE;
+  const int rc = pl.big ? launch(gated_ffn_grads_kernel<256, 256, 2, 4>, (unsigned)n, 512, NST * 512 * BK * 2, a, s)
+                        : launch(gated_ffn_grads_kernel<128, 128, 2, 2>, (unsigned)n, 256, NST * 256 * BK * 2, a, s);
+  if (rc != AITK_OK || !joined) return rc;
+  const int64_t blocks = (joined / 8 + 255) / 256;
+  hipLaunchKernelGGL(gated_ffn_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048), 3), dim3(256), 0, s, a);
+  AITK_LAUNCH_CHECK();
+  return AITK_OK;
 }

@@ -1449,7 +1449,7 @@ def gated_ffn_bwd(dh, x, w_val, w_gate, hg, *, act="gelu_tanh", dx=None, dw_val=
     if M == 0:
         host_call(lambda: [t.zero_() for t in (dw_val, dw_gate, db_val, db_gate) if t is not None])
         return dx
-    ws = _scratch(_capi.lib().aitk_gated_ffn_bwd_workspace_bytes(M, F, int(db_val is not None or db_gate is not None)), x.device)
+    ws = _scratch(_capi.lib().aitk_gated_ffn_bwd_workspace_bytes(M, K, F, dx is not None, dw_val is not None, dw_gate is not None, db_val is not None or db_gate is not None), x.device)
     a.dh, a.x, a.w_val, a.w_gate, a.hg = _adr(dh), _adr(x), _adr(w_val), _adr(w_gate), _adr(hg)
     a.dx, a.dw_val, a.dw_gate, a.db_val, a.db_gate, a.ws = _adr(dx), _adr(dw_val), _adr(dw_gate), _adr(db_val), _adr(db_gate), _adr(ws)
     a.M, a.K, a.F, a.act = M, K, F, GATED_ACTS[act]

@@ -654,7 +654,8 @@ typedef struct AitkGatedFfnArgs {
 } AitkGatedFfnArgs;
 int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* args, aitk_stream_t stream);
 /* From dh [M, F] and the saved hg: dx [M, K], dw_val / dw_gate [F, K] (one row pitch), db_val / db_gate [F], all bf16, each may be NULL (frozen weights: dx alone).
- * [du | dz] is formed once in bf16 in ws (aitk_gated_ffn_bwd_workspace_bytes); no transposed copy of any operand is made.  Deterministic. */
+ * [du | dz] is formed once in bf16 in ws (aitk_gated_ffn_bwd_workspace_bytes; dx .. bias_grads: which results are asked for); no transposed copy of any operand is made.
+ * Where a product has few tiles and a long contraction, pieces of it are summed in fp32 in a fixed order.  Deterministic. */
 typedef struct AitkGatedFfnBwdArgs {
   const aitk_bf16* dh; int64_t ld_dh;
   const aitk_bf16* x; int64_t ldx;
@@ -666,7 +667,7 @@ typedef struct AitkGatedFfnBwdArgs {
   void* ws;
   int32_t M, K, F, act;
 } AitkGatedFfnBwdArgs;
-int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t F, int32_t bias_grads);
+int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t K, int32_t F, int32_t dx, int32_t dw_val, int32_t dw_gate, int32_t bias_grads);
 int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* args, aitk_stream_t stream);
 
 /* ---- hardware probes (test infrastructure for layout assumptions; not on the product path) ---- */
