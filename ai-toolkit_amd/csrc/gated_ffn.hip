@@ -323,6 +323,72 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) 
   }
 }
 
+// Forward for a few rows (at most 16 TB): bound by the weights' way from memory.  A workgroup takes 16 rows of both weights, its eight waves every eighth 32-wide step of the
+// contraction; weights and x go straight from global memory into the matrix operands (W is the A operand of the 16 x 16 x 32 product, the tokens are its columns), four steps of
+// loads in flight per wave; the waves' sums meet in LDS in a fixed order.
+template <int TB>
+__global__ __launch_bounds__(512) void gated_ffn_few_kernel(FfnArgs a) {
+  constexpr int U = 4;
+  __shared__ f32x4_t box[8][2 * TB][64];
+  const Prod& p = a.p[0];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kg = lane >> 4;
+  const int f0 = blockIdx.x * 16;
+  const bf16_t* w[2];
+#pragma unroll
+  for (int v = 0; v < 2; ++v) w[v] = p.B[v] + (long)min(f0 + r16, p.N - 1) * p.ldb + kg * 8;
+  const bf16_t* x[TB];
+#pragma unroll
+  for (int t = 0; t < TB; ++t) x[t] = p.A[0] + (long)min(t * 16 + r16, p.M - 1) * p.lda + kg * 8;
+  f32x4_t acc[2][TB];
+#pragma unroll
+  for (int t = 0; t < TB; ++t) acc[0][t] = acc[1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int steps = (p.K + 31) / 32;
+  for (int s0 = wave; s0 < steps; s0 += 8 * U) {
+    s16x8_t wf[U][2], xf[U][TB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (s0 + 8 * u) * 32;
+      const bool in = k + kg * 8 < p.K;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) wf[u][v] = in ? *reinterpret_cast<const s16x8_t*>(w[v] + k) : s16x8_t{};
+#pragma unroll
+      for (int t = 0; t < TB; ++t) xf[u][t] = in ? *reinterpret_cast<const s16x8_t*>(x[t] + k) : s16x8_t{};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) acc[v][t] = mfma16(wf[u][v], xf[u][t], acc[v][t]);
+  }
+#pragma unroll
+  for (int v = 0; v < 2; ++v)
+#pragma unroll
+    for (int t = 0; t < TB; ++t) box[wave][2 * t + v][lane] = acc[v][t];
+  __syncthreads();
+  const int m = wave * 16 + r16, n = f0 + 4 * kg;  // wave t finishes token block t: lane -> token r16, rows 4 kg .. + 3 of the weights
+  if (wave >= TB || m >= p.M || n >= p.N) return;
+  f32x4_t z = box[0][2 * wave][lane], u = box[0][2 * wave + 1][lane];
+#pragma unroll
+  for (int q = 1; q < 8; ++q) {
+    z += box[q][2 * wave][lane];
+    u += box[q][2 * wave + 1][lane];
+  }
+  float o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (a.bg) z[e] += bf2f(a.bg[n + e]);
+    if (a.bv) u[e] += bf2f(a.bv[n + e]);
+    o[e] = u[e] * act_f(z[e], a.act);
+  }
+  *reinterpret_cast<uint2*>(p.C + (long)m * p.ldc + n) = make_uint2(pack2bf(o[0], o[1]), pack2bf(o[2], o[3]));
+  if (a.hg) {
+    bf16_t* r = a.hg + (long)m * a.ld_hg + n;
+    *reinterpret_cast<uint2*>(r) = make_uint2(pack2bf(u[0], u[1]), pack2bf(u[2], u[3]));
+    *reinterpret_cast<uint2*>(r + p.N) = make_uint2(pack2bf(z[0], z[1]), pack2bf(z[2], z[3]));
+  }
+}
+
 template <int BM, int BN, int WR, int WC, bool AK>
 __device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, int piece, char* smem) {
   typedef TileLoop<BM, BN, WR, WC, AK, false, false> Loop;
@@ -402,7 +468,7 @@ __global__ __launch_bounds__(256) void gated_ffn_join_kernel(FfnArgs a) {
 }
 
 // [du | dz] from dh and [u | z]; with SUMS the fp32 column sums of the workgroup's rows.  Memory bound: three reads, two writes.  A thread owns 8 columns.
-constexpr int DU_ROWS = 64;  // rows of a workgroup
+constexpr int DU_ROWS = 32;  // rows of a workgroup
 template <bool SUMS>
 __global__ __launch_bounds__(256) void gated_ffn_du_kernel(const bf16_t* dh, long ld_dh, const bf16_t* hg, long ld_hg, bf16_t* du, int M, int F, int act, float* part) {
   const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8, sub = threadIdx.x >> 6;
@@ -451,14 +517,19 @@ __global__ __launch_bounds__(256) void gated_ffn_du_kernel(const bf16_t* dh, lon
     }
   }
 }
+// column sums of the workgroups' partials: 64 columns x 4 slices of the workgroups, joined in a fixed order
 __global__ __launch_bounds__(256) void gated_ffn_db_kernel(const float* part, int nchunk, int F, bf16_t* dbv, bf16_t* dbg) {
-  const int c = blockIdx.x * 256 + threadIdx.x, v = blockIdx.y;
+  __shared__ float box[4][64];
+  const int l = threadIdx.x & 63, sl = threadIdx.x >> 6, c = blockIdx.x * 64 + l, v = blockIdx.y;
   bf16_t* out = v ? dbg : dbv;
-  if (c >= F || !out) return;
   float s = 0.f;
+  if (c < F && out) {
 #pragma unroll 8
-  for (int k = 0; k < nchunk; ++k) s += part[((long)k * 2 + v) * F + c];
-  out[c] = f2bf(s);
+    for (int k = sl; k < nchunk; k += 4) s += part[((long)k * 2 + v) * F + c];
+  }
+  box[sl][l] = s;
+  __syncthreads();
+  if (sl == 0 && c < F && out) out[c] = f2bf(box[0][l] + box[1][l] + box[2][l] + box[3][l]);
 }
 
 bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
@@ -551,6 +622,14 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   hipStream_t s = (hipStream_t)stream;
   const int64_t big = tiles(q->M, q->F, 256, 128), small = tiles(q->M, q->F, 128, 64);
   if (small > 0x7fffffff) return AITK_ERR_SHAPE;
+  const unsigned strips = (unsigned)((q->F + 15) / 16);
+  // up to 32 rows the weights' way bounds both forms: 4096 x 10240 16 rows 36 us against 48 us of the small tiles, 32 rows 45 against 48, 512 x 1024 3.8 / 4.5 against 11 us.  Up to 64
+  // rows the waves read x more often than W: 64 rows 69 us against 48 for 4096 x 10240 (168 MB), but 8.5 against 16.5 for 1024 x 2816 (12 MB): there the tiles' start-up decides.
+  if (q->M <= 32 || (q->M <= 64 && (int64_t)q->F * q->K <= (8 << 20))) {
+    if (q->M <= 16) return launch(gated_ffn_few_kernel<1>, strips, 512, 0, a, s);
+    if (q->M <= 32) return launch(gated_ffn_few_kernel<2>, strips, 512, 0, a, s);
+    return launch(gated_ffn_few_kernel<4>, strips, 512, 0, a, s);
+  }
   // A round of small tiles (two workgroups per CU) takes 0.55 to 0.75 of a round of large ones: 512 x 4096 x 10240 (1 round against 2) 113 us large, 137 us small;
   // 4096 x 640 x 2560 (2 against 3) 57.8 and 49.2; 2048 x 2048 x 5120 (2 against 3) 121.5 and 119.8; 256 x 4096 x 10240 (1 against 1) 92 and 74; 2048 x 4096 x 10240 (3 against 5) 366 and 450.
   if (20 * ((big + 255) / 256) <= 13 * ((small + 511) / 512)) return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)big, 512, NST * 512 * BK * 2, a, s);
@@ -583,7 +662,7 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
   else hipLaunchKernelGGL(gated_ffn_du_kernel<false>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, part);
   AITK_LAUNCH_CHECK();
   if (db) {
-    hipLaunchKernelGGL(gated_ffn_db_kernel, dim3((F + 255) / 256, 2), dim3(256), 0, s, part, nchunk, F, q->db_val, q->db_gate);
+    hipLaunchKernelGGL(gated_ffn_db_kernel, dim3((F + 63) / 64, 2), dim3(256), 0, s, part, nchunk, F, q->db_val, q->db_gate);
     AITK_LAUNCH_CHECK();
   }
   FfnArgs a = {};
