@@ -97,6 +97,19 @@ __device__ __forceinline__ s16x8_t frag_tr(const lds_char* tile, const TileLane&
   const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(tile + kk * 2048 + L.tr[d][1]));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
+// A lane's 32 x 2 columns of one output row (registers of o^T: column 32 d + 8 g + 4 h + e): the two halves of the wave trade so that a lane stores 16 bytes, columns
+// 16 c + 8 h .. + 7 of its row.  All lanes take part; `in`: the row exists.
+__device__ __forceinline__ void store_row(bf16_t* row, const f32x16_t (&o)[2], float mul, int h, bool in) {
+  typedef unsigned u2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int d = 0; d < 2; ++d)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const u2_t x = __builtin_amdgcn_permlane32_swap(pack2bf(o[d][8 * q] * mul, o[d][8 * q + 1] * mul), pack2bf(o[d][8 * q + 4] * mul, o[d][8 * q + 5] * mul), false, false);
+      const u2_t y = __builtin_amdgcn_permlane32_swap(pack2bf(o[d][8 * q + 2] * mul, o[d][8 * q + 3] * mul), pack2bf(o[d][8 * q + 6] * mul, o[d][8 * q + 7] * mul), false, false);
+      if (in) *reinterpret_cast<uint4*>(row + 32 * d + 16 * q + 8 * h) = make_uint4(x[0], y[0], x[1], y[1]);
+    }
+}
 // one 64-row tile of a [rows][64] slice: two DMAs per wave; rows whose bit of `keep` is 0 arrive as zeros
 __device__ __forceinline__ void stage(lds_char* tile, const TileLane& L, long ld, int row0, const v4i_t& srd, int wave, unsigned long long keep) {
 #pragma unroll
@@ -353,17 +366,8 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
   }
   const float inv = l_tot > 0.f ? 1.0f / l_tot : l_tot != l_tot ? l_tot : 0.f;
   const int q = q0 + l31;
-  if (q < S) {
-    bf16_t* op = a.O + ((long)b * S + q) * a.ldo + hd * 64;
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint2 u = make_uint2(pack2bf(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), pack2bf(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
-        *reinterpret_cast<uint2*>(op + 32 * d + 8 * g + 4 * h) = u;
-      }
-    if (h == 0) a.LSE[((long)b * a.H + hd) * S + q] = l_tot == 0.f ? -INFINITY : m_run + log2f(l_tot);
-  }
+  store_row(a.O + ((long)b * S + min(q, S - 1)) * a.ldo + hd * 64, o, inv, h, q < S);
+  if (q < S && h == 0) a.LSE[((long)b * a.H + hd) * S + q] = l_tot == 0.f ? -INFINITY : m_run + log2f(l_tot);
 }
 
 // ============================================================================================ backward
@@ -425,7 +429,9 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   lds_float* const acc = line + 4 * r.line_p + wave * n_line;
   lds_float* const skew = line + 4 * r.line_p + (4 * n_line + 3) / 4 * 4 + wave * (32 * SKEW_P);
   lds_float* const skew_w = skew + l31 * SKEW_P + 31 - l31 + ((l31 + 1) & 3) + 4 * h;
-  float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f;
+  // The rows of ds add up to 0; what they add up to here is the error of delta (o is rounded to bf16), spread over the row in proportion to p.  A narrow bucket hardly sees it, the last
+  // bucket of a sign, which takes a row's far keys all with one sign, does: its sum is corrected by (row sum of ds) x (row's p in the bucket).
+  float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f, fp_past = 0.f, fp_ahead = 0.f, row_ds = 0.f;
   const int ib = E + 4 * h - q0 - l31;
   if constexpr (BIAS) {
     build_line(line, r, hd, 1);
@@ -467,7 +473,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
           else if (kv0 - q0 - 31 >= r.sat) side = 2, tb = far_ahead;
         }
         const float sub = tb - l2;
-        float fs = 0.f;
+        float fs = 0.f, fp = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           f32x16_t s, dp = zero16();
@@ -488,7 +494,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) dp = mfma32(frag_rm(vt, L, j, ks), gf[ks], dp);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, sub)) * (dp[e] - delta);
+          for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, sub));
           if (~keep) {
             const unsigned mj = (unsigned)(keep >> (32 * j)) >> (4 * h);
 #pragma unroll
@@ -501,7 +507,15 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
             for (int e = 0; e < 16; ++e)
               if ((e & 3) + 8 * (e >> 2) > lim) s[e] = 0.f;
           }
+          if (sums && side != 0) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) fp += s[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] *= dp[e] - delta;
           if (sums) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) fs += s[e];
             if (side == 0) {
 #pragma unroll
               for (int g = 0; g < 4; ++g)
@@ -512,9 +526,6 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
               for (int q = 0; q < 32; ++q) v += skew[q * SKEW_P + ((q + 1) & 3) + lane];
               acc[E + kv0 + 32 * j - q0 - 31 + lane] += v;
               __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) fs += s[e];
             }
           }
 #pragma unroll
@@ -524,8 +535,9 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
             for (int d = 0; d < 2; ++d) dq[d] = mfma32(frag_tr(kt, L, 2 * j + kk, d), df, dq[d]);
           }
         }
-        if (side == 1) fs_past += fs;
-        else fs_ahead += fs;
+        row_ds += fs;
+        if (side == 1) fs_past += fs, fp_past += fp;
+        if (side == 2) fs_ahead += fs, fp_ahead += fp;
       }
       dma_wait_all();
       __syncthreads();
@@ -535,20 +547,12 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       cur ^= 1;
     }
   }
-  if (live) {
-    bf16_t* op = a.dQ + ((long)b * S + q0 + l31) * a.lddq + hd * 64;
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint2 u = make_uint2(pack2bf(dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale), pack2bf(dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale));
-        *reinterpret_cast<uint2*>(op + 32 * d + 8 * g + 4 * h) = u;
-      }
-  }
+  store_row(a.dQ + ((long)b * S + qc) * a.lddq + hd * 64, dq, a.scale, h, live);
   if (sums) {
     lds_float* const fars = (lds_float*)smem;  // the tiles are done with (the loop ends behind a barrier; so does the set-up when no tile was visited)
-    fs_past = wave_sum(fs_past);
-    fs_ahead = wave_sum(fs_ahead);
+    row_ds += __shfl_xor(row_ds, 32, 64);  // the row's two lanes
+    fs_past = wave_sum(fs_past - row_ds * fp_past);
+    fs_ahead = wave_sum(fs_ahead - row_ds * fp_ahead);
     if (lane == 0) {
       fars[wave] = fs_past;
       fars[4 + wave] = fs_ahead;
@@ -679,21 +683,12 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
       __syncthreads();
     }
   }
-  if (inside) {
-    bf16_t* kp = a.dK + ((long)b * S + key) * a.lddk + hd * 64;
-    bf16_t* vp = a.dV + ((long)b * S + key) * a.lddv + hd * 64;
-    const float sc = a.scale;
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint2 u = make_uint2(pack2bf(dk[d][4 * g] * sc, dk[d][4 * g + 1] * sc), pack2bf(dk[d][4 * g + 2] * sc, dk[d][4 * g + 3] * sc));
-        uint2 w = make_uint2(pack2bf(dv[d][4 * g], dv[d][4 * g + 1]), pack2bf(dv[d][4 * g + 2], dv[d][4 * g + 3]));
-        if (!kept) u = w = make_uint2(0u, 0u);
-        *reinterpret_cast<uint2*>(kp + 32 * d + 8 * g + 4 * h) = u;
-        *reinterpret_cast<uint2*>(vp + 32 * d + 8 * g + 4 * h) = w;
-      }
+  if (!kept) {  // a masked key's lane may hold anything
+    dk[0] = dk[1] = dv[0] = dv[1] = zero16();
   }
+  const long row = (long)b * S + (inside ? key : 0);
+  store_row(a.dK + row * a.lddk + hd * 64, dk, a.scale, h, inside);
+  store_row(a.dV + row * a.lddv + hd * 64, dv, 1.0f, h, inside);
 }
 
 // both gradients in one launch (they share nothing but their inputs): twice the workgroups, so that a single prompt fills the chip
