@@ -24,7 +24,7 @@ typedef int v4i_t __attribute__((ext_vector_type(4)));
 
 constexpr int TILE = 8192;          // bytes of a [64][64] bf16 tile
 constexpr int BAND_PAD = 96;        // a wave's 32 rows x 64 columns span 95 distances
-constexpr int SKEW_P = 68;          // floats per row of a skewed 32 x 32 block (63 diagonals + 3 of slack)
+constexpr int SKEW_P = 44;          // floats per row of a skewed 8 x 32 block (39 diagonals + 3 of slack)
 constexpr int MAX_HALF = 64;        // buckets of one sign
 constexpr float M_NONE = -3.0e38f;  // running maximum of a row that has met no key yet (finite: differences with it are never NaN)
 constexpr float DEFER = 8.0f;       // the accumulators are rescaled only when a row's maximum grew by more than 2^8 (p stays below 2^8: exact in fp32 sums)
@@ -33,7 +33,7 @@ struct RelposArgs {
   AitkAttnRelposArgs a;
   int half, sat, line_p, _pad;  // buckets per sign, first distance of the last one, floats per shifted copy of the line
   int first[MAX_HALF];          // first distance of every bucket of one sign
-  float* delta;                 // backward: [2][B][H][S]: dO.o, and lse with +inf for rows without a key
+  float* delta;                 // backward: [2][B][H][S]: dO.o, and -lse (-inf for rows without a key)
   float* part;                  // backward: [B * row tiles][H][num_buckets] bucket sums
 };
 
@@ -119,6 +119,19 @@ __device__ __forceinline__ void stage(lds_char* tile, const TileLane& L, long ld
     if (~keep) off = (keep >> r) & 1 ? off : 0x80000000u;
     dma16(__builtin_amdgcn_readfirstlane((unsigned)(size_t)tile + (wave + 4 * p) * 1024), off, srd);
   }
+}
+
+// 16 start values from the line: entries i0 + 8 g .. + 3 of every lane
+__device__ __forceinline__ f32x16_t load_line(const lds_float* line, int line_p, int i0) {
+  const lds_float* lp = line + (i0 & 3) * line_p + (i0 & ~3);
+  f32x16_t s;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(lp + 8 * g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
+  }
+  return s;
 }
 
 // bucket of a distance n >= 0 within its sign
@@ -268,14 +281,7 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) kf[ks] = frag_rm(kt, L, j, ks);
           if (BIAS && near) {
-            const int i0 = ib + kv0;
-            const lds_float* lp = line + (i0 & 3) * r.line_p + (i0 & ~3) + 32 * j;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const f32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(lp + 8 * g);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[j][4 * g + e] = v[e];
-            }
+            s[j] = load_line(line, r.line_p, ib + kv0 + 32 * j);
           } else {
             s[j] = zero16();
           }
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
 }
 
 // ============================================================================================ backward
-// delta[q] = dO[q].o[q], and the row statistic with +inf for rows without a key (2^(s - inf) = 0: their probabilities vanish).  A wave takes 8 rows of one head.
+// delta[q] = dO[q].o[q], and minus the row statistic, -inf for rows without a key (2^(s - inf) = 0: their probabilities vanish).  A wave takes 8 rows of one head.
 __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
   const AitkAttnRelposArgs& a = r.a;
   const int s = blockIdx.x * 32 + (threadIdx.x >> 3), hd = blockIdx.y, b = blockIdx.z, c = (threadIdx.x & 7) * 8;
@@ -387,7 +393,7 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
     const long i = ((long)b * a.H + hd) * a.S + s;
     const float l = a.LSE[i];
     r.delta[i] = v;
-    r.delta[(long)a.B * a.H * a.S + i] = l == -INFINITY ? INFINITY : l;
+    r.delta[(long)a.B * a.H * a.S + i] = l == -INFINITY ? -INFINITY : -l;
   }
 }
 
@@ -419,16 +425,17 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   }
   const long stat = ((long)b * a.H + hd) * S + qc;
   const float delta = r.delta[stat];
-  const float l2 = live ? r.delta[(long)a.B * a.H * S + stat] : INFINITY;  // rows past the end: p = 0, ds = 0
+  const float l2 = live ? -r.delta[(long)a.B * a.H * S + stat] : INFINITY;  // rows past the end: p = 0, ds = 0
   const float c2 = a.scale * 1.4426950408889634f;
   const int E = r.sat + BAND_PAD, n_line = 2 * E + 1;
   const bool sums = BIAS && a.dtable != nullptr;
-  // Bucket sums.  A 32 x 32 block's diagonals (one relative position each) become columns of a wave-private LDS patch: row q is written q places to the left (with up to
-  // three places of slack so that its 16-byte stores are aligned; what a row never writes stays zero), a lane then adds up one column and joins it to the wave's
-  // accumulator of that distance.  Fixed order, no atomics (an LDS float add per element: 330 us for 4 x 64 heads x 512 against 137 us).
+  // Bucket sums.  The diagonals of a 32 x 32 block (one relative position each) become columns of a wave-private LDS patch, eight query rows at a time: row q is written q mod 8
+  // places to the left (with up to three places of slack so that its 16-byte stores are aligned; what a row never writes stays zero), a lane then adds up one column and
+  // joins it to the wave's accumulator of that distance.  Fixed order, no atomics (an LDS float add per element: 330 us for 4 x 64 heads x 512 against 137 us).  Eight rows and not all 32: the
+  // workgroup's LDS then lets three of them share a CU.
   lds_float* const acc = line + 4 * r.line_p + wave * n_line;
-  lds_float* const skew = line + 4 * r.line_p + (4 * n_line + 3) / 4 * 4 + wave * (32 * SKEW_P);
-  lds_float* const skew_w = skew + l31 * SKEW_P + 31 - l31 + ((l31 + 1) & 3) + 4 * h;
+  lds_float* const skew = line + 4 * r.line_p + (4 * n_line + 3) / 4 * 4 + wave * (8 * SKEW_P);
+  lds_float* const skew_w = skew + (l31 & 7) * SKEW_P + 7 - (l31 & 7) + ((l31 + 1) & 3) + 4 * h;
   // The rows of ds add up to 0; what they add up to here is the error of delta (o is rounded to bf16), spread over the row in proportion to p.  A narrow bucket hardly sees it, the last
   // bucket of a sign, which takes a row's far keys all with one sign, does: its sum is corrected by (row sum of ds) x (row's p in the bucket).
   float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f, fp_past = 0.f, fp_ahead = 0.f, row_ds = 0.f;
@@ -438,7 +445,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
     far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
     far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
     if (sums)
-      for (int i = tid; i < (4 * n_line + 3) / 4 * 4 + 4 * 32 * SKEW_P; i += 256) (line + 4 * r.line_p)[i] = 0.f;
+      for (int i = tid; i < (4 * n_line + 3) / 4 * 4 + 4 * 8 * SKEW_P; i += 256) (line + 4 * r.line_p)[i] = 0.f;
     __syncthreads();
   }
   f32x16_t dq[2] = {zero16(), zero16()};
@@ -477,15 +484,8 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           f32x16_t s, dp = zero16();
-          const int i0 = ib + kv0;
           if (BIAS && side == 0) {
-            const lds_float* lp = line + (i0 & 3) * r.line_p + (i0 & ~3) + 32 * j;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const f32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(lp + 8 * g);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
-            }
+            s = load_line(line, r.line_p, ib + kv0 + 32 * j);
           } else {
             s = zero16();
           }
@@ -518,14 +518,21 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
             for (int e = 0; e < 16; ++e) fs += s[e];
             if (side == 0) {
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(skew_w + 8 * g) = f32x4_t{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
-              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' stores: LDS keeps a wave's accesses in order
-              float v = 0.f;
+              for (int p8 = 0; p8 < 4; ++p8) {
+                if (l31 >> 3 == p8) {
 #pragma unroll
-              for (int q = 0; q < 32; ++q) v += skew[q * SKEW_P + ((q + 1) & 3) + lane];
-              acc[E + kv0 + 32 * j - q0 - 31 + lane] += v;
-              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                  for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(skew_w + 8 * g) = f32x4_t{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' stores: LDS keeps a wave's accesses in order
+                if (lane < 39) {
+                  float v[2] = {0.f, 0.f};
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) v[q & 1] += skew[q * SKEW_P + ((q + 1) & 3) + lane];
+                  acc[E + kv0 + 32 * j - q0 - 7 - 8 * p8 + lane] += v[0] + v[1];
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+              }
             }
           }
 #pragma unroll
@@ -579,7 +586,7 @@ template <bool BIAS, bool CAUSAL>
 __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int tile_x, int hd, int b) {
   const AitkAttnRelposArgs& a = r.a;
   lds_char* const sm = (lds_char*)smem;                        // 2 x (Q tile, dO tile)
-  lds_float* const st = (lds_float*)(smem + 4 * TILE);         // 2 x (64 lse, 64 delta)
+  lds_float* const st = (lds_float*)(smem + 4 * TILE);         // 2 x (64 -lse, 64 delta)
   lds_float* const line = (lds_float*)(smem + 4 * TILE + 1024);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5, S = a.S;
@@ -610,11 +617,11 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
     const float c2 = a.scale * 1.4426950408889634f;
     const int E = r.sat + BAND_PAD;
     const int ib = E + 4 * h - key;  // line index of query 0 of this lane's first register: entry i is the bias of key - query = E - i
-    float far_past = 0.f, far_ahead = 0.f;
+    float far_past = 0.f, far_ahead = 0.f;  // not in the log2 domain here: start values like the line's
     if constexpr (BIAS) {
       build_line(line, r, hd, -1);
-      far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
-      far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
+      far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale);
+      far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale);
     }
     // rows past the end arrive as zeros: dO = 0 and delta = 0, so they add nothing to either gradient
     auto stage_all = [&](int t, int buf) {
@@ -631,27 +638,16 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
       const lds_char* qt = sm + cur * 2 * TILE;
       const lds_char* gt = qt + TILE;
       const int qt0 = t * 64;
-      float tb = 0.f;
-      bool near = false;
-      if constexpr (BIAS) {
-        near = true;
-        if (k0 + 31 - qt0 <= -r.sat) near = false, tb = far_past;
-        else if (k0 - qt0 - 63 >= r.sat) near = false, tb = far_ahead;
-      }
+      const bool past = BIAS && k0 + 31 - qt0 <= -r.sat, ahead = BIAS && k0 - qt0 - 63 >= r.sat;
+      const float far = past ? far_past : ahead ? far_ahead : 0.f;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         f32x16_t s, dp = zero16();
-        if (BIAS && near) {
-          const int i0 = ib + qt0;
-          const lds_float* lp = line + (i0 & 3) * r.line_p + (i0 & ~3) + 32 * j;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(lp + 8 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
-          }
+        if (BIAS && !past && !ahead) {
+          s = load_line(line, r.line_p, ib + qt0 + 32 * j);
         } else {
-          s = zero16();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = far;
         }
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) s = mfma32(frag_rm(qt, L, j, ks), kf[ks], s);
@@ -659,11 +655,11 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
         for (int ks = 0; ks < 4; ++ks) dp = mfma32(frag_rm(gt, L, j, ks), vf[ks], dp);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4_t l2 = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 32 * j + 8 * g + 4 * h);
+          const f32x4_t nl = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 32 * j + 8 * g + 4 * h);
           const f32x4_t de = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 64 + 32 * j + 8 * g + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], c2, tb - l2[e]));
+            float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], c2, nl[e]));
             if (CAUSAL && qt0 + 32 * j + 8 * g + 4 * h + e < key) p = 0.f;
             s[4 * g + e] = p;
             dp[4 * g + e] = p * (dp[4 * g + e] - de[e]);
@@ -693,7 +689,7 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
 
 // both gradients in one launch (they share nothing but their inputs): twice the workgroups, so that a single prompt fills the chip
 template <bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void attn_relpos_bwd_kernel(RelposArgs r) {
+__global__ __launch_bounds__(256, 3) void attn_relpos_bwd_kernel(RelposArgs r) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int nt = (r.a.S + 127) / 128;
   int tile_x, hd, b;
@@ -824,7 +820,7 @@ extern "C" int aitk_attn_relpos_bwd(const AitkAttnRelposArgs* a, aitk_stream_t s
   hipLaunchKernelGGL(attn_relpos_delta_kernel, dim3((a->S + 31) / 32, a->H, a->B), dim3(256), 0, s, r);
   AITK_LAUNCH_CHECK();
   const unsigned grid = (unsigned)((a->S + 127) / 128) * a->H * a->B * 2;
-  const size_t lds = 4 * TILE + 1024 + (size_t)4 * r.line_p * 4 + (a->dtable ? ((size_t)4 * (2 * (r.sat + BAND_PAD) + 1) + 3 + 4 * 32 * SKEW_P) * 4 : 0);
+  const size_t lds = 4 * TILE + 1024 + (size_t)4 * r.line_p * 4 + (a->dtable ? ((size_t)4 * (2 * (r.sat + BAND_PAD) + 1) + 3 + 4 * 8 * SKEW_P) * 4 : 0);
   if (a->table) rc = a->causal ? launch(attn_relpos_bwd_kernel<true, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<true, false>, grid, lds, r, s);
   else rc = a->causal ? launch(attn_relpos_bwd_kernel<false, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<false, false>, grid, lds, r, s);
   if (rc != AITK_OK) return rc;
