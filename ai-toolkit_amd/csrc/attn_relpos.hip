@@ -180,13 +180,15 @@ __device__ __forceinline__ unsigned long long lane64(unsigned long long m, int t
   const unsigned lo = __builtin_amdgcn_readlane((unsigned)m, t), hi = __builtin_amdgcn_readlane((unsigned)(m >> 32), t);
   return (unsigned long long)hi << 32 | lo;
 }
-// workgroup -> (row tile, head, sample): the tiles of one (head, sample) stay on one XCD, whose L2 then holds their slices (block i runs on XCD i % 8)
-__device__ __forceinline__ void wg_coords(int ntiles, int H, int& tile, int& hd, int& b) {
+// workgroup -> (row tile, head, sample): the tiles of one (head, sample) stay on one XCD, whose L2 then holds their slices (block i runs on XCD i % 8), and an XCD gets all the
+// samples of its heads: with a key mask the samples differ in length, and whole samples per XCD left the XCDs of the
+// short ones idle (4 x 64 heads x 512 with lengths 24 .. 512: backward 126 -> 105 us, forward 37 -> 32 us)
+__device__ __forceinline__ void wg_coords(int ntiles, int B, int& tile, int& hd, int& b) {
   const int n = gridDim.x, id = blockIdx.x, x = id & 7, per = n >> 3, rem = n & 7;
   const int l = x * per + min(x, rem) + (id >> 3);
   tile = l % ntiles;
-  hd = (l / ntiles) % H;
-  b = (l / ntiles) / H;
+  b = (l / ntiles) % B;
+  hd = (l / ntiles) / B;
 }
 
 // ============================================================================================ forward
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
   const int l31 = lane & 31, h = lane >> 5, S = a.S;
   const int qg = wave / KVS, part = wave % KVS;
   int tile_x, hd, b;
-  wg_coords((S + ROWS - 1) / ROWS, a.H, tile_x, hd, b);
+  wg_coords((S + ROWS - 1) / ROWS, a.B, tile_x, hd, b);
   const int q0 = tile_x * ROWS + qg * 32;
   const v4i_t srdK = make_srd(a.K + (long)b * S * a.ldk + hd * 64, ((long)(S - 1) * a.ldk + 64) * 2);
   const v4i_t srdV = make_srd(a.V + (long)b * S * a.ldv + hd * 64, ((long)(S - 1) * a.ldv + 64) * 2);
@@ -693,7 +695,7 @@ __global__ __launch_bounds__(256, 3) void attn_relpos_bwd_kernel(RelposArgs r) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int nt = (r.a.S + 127) / 128;
   int tile_x, hd, b;
-  wg_coords(2 * nt, r.a.H, tile_x, hd, b);
+  wg_coords(2 * nt, r.a.B, tile_x, hd, b);
   if (tile_x < nt) dq_role<BIAS, CAUSAL>(r, smem, tile_x, hd, b);
   else dkv_role<BIAS, CAUSAL>(r, smem, tile_x - nt, hd, b);
 }
