@@ -492,9 +492,11 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
             s = zero16();
           }
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) s = mfma32(frag_rm(kt, L, j, ks), qf[ks], s);
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) dp = mfma32(frag_rm(vt, L, j, ks), gf[ks], dp);
+          for (int ks = 0; ks < 4; ++ks) {
+            s = mfma32(frag_rm(kt, L, j, ks), qf[ks], s);
+            dp = mfma32(frag_rm(vt, L, j, ks), gf[ks], dp);
+          }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, sub));
           if (~keep) {
@@ -652,9 +654,11 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
           for (int e = 0; e < 16; ++e) s[e] = far;
         }
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) s = mfma32(frag_rm(qt, L, j, ks), kf[ks], s);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) dp = mfma32(frag_rm(gt, L, j, ks), vf[ks], dp);
+        for (int ks = 0; ks < 4; ++ks) {
+          s = mfma32(frag_rm(qt, L, j, ks), kf[ks], s);
+          dp = mfma32(frag_rm(gt, L, j, ks), vf[ks], dp);
+        }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const f32x4_t nl = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 32 * j + 8 * g + 4 * h);
