@@ -331,6 +331,7 @@ def check(rc, what):
 
 
 def stream_ptr():
+    """the current stream's handle, without the Stream object: 1 us of a small call's 10"""
     import torch
 
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))  # the current stream's handle without the Stream object: 1 us of a small call's 10
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))

@@ -51,6 +51,9 @@ def _emit(name, args):
     if name == "_wgrad_defer":
         _emit_wgrad_defer(*args)
         return
+    if _gemm_hook is None and _attn_hook is None:
+        _capi.check(getattr(_capi.lib(), name)(*args, _capi.stream_ptr()), name)
+        return
     timed = _gemm_hook is not None and name in ("aitk_gemm_nt", "aitk_gemm_nt_grouped")
     timed_attn = _attn_hook is not None and name in ("aitk_attn_fwd", "aitk_attn_bwd")
     if timed or timed_attn:
@@ -1200,47 +1203,59 @@ def attn_small_bwd(q, k, v, o, lse, do, dq, dk, dv, *, B, H, S, D, scale, Skv=0)
 # ---------------------------------------------------------------------------------------------------------- text-encoder block
 # Norms with a learned weight, attention with a learned relative position bias, the gated feed-forward projections.  Arguments that the kernels cannot take raise
 # ValueError before anything is launched; scratch is a torch allocation of the call (current stream's, and a capturing graph's own pool), never a buffer that two
-# streams or two captured graphs would share.
-def _rows(t, name, rows, cols):
-    """bf16 [rows, cols] view with unit inner stride, a row pitch of whole 16-byte chunks and a 16-byte aligned start -> the row pitch"""
-    st = t.stride()
-    if t.dtype == BF16 and t.shape == (rows, cols) and (st[1] == 1 or cols == 1):
-        ld = st[0] if rows > 1 else max(st[0], (cols + 7) & -8)  # the pitch of a single row is nobody's
-        if ld >= cols and ld % 8 == 0 and t.data_ptr() % 16 == 0:
-            return ld
+# streams or two captured graphs would share.  The checks format nothing until one fails and the argument blocks are filled in field order: a small call costs its user
+# more on the host than on the GPU.
+def _rows(t, name, shape):
+    """bf16 view of that shape with unit inner stride, a row pitch of whole 16-byte chunks and a 16-byte aligned start -> (address, row pitch)"""
+    if t.dtype is BF16 and t.shape == shape:
+        ld, inner = t.stride()
+        p = t.data_ptr()
+        rows, cols = shape
+        if rows <= 1 or cols <= 1:  # a stride that nothing steps over is nobody's
+            if rows <= 1:
+                ld = (cols + 7) & -8
+            inner = 1 if cols <= 1 else inner
+        if inner == 1 and ld >= cols and not ld & 7 and not p & 15:
+            return p, ld
     if t.dtype != BF16:
         raise ValueError(f"{name}: expected bf16, got {t.dtype}")
-    if t.shape != (rows, cols):
-        raise ValueError(f"{name}: expected [{rows}, {cols}], got {tuple(t.shape)}")
-    raise ValueError(f"{name}: rows must have unit inner stride, be 16-byte aligned and not overlap (strides {st}, address mod 16 = {t.data_ptr() % 16})")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected {list(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name}: rows must have unit inner stride, be 16-byte aligned and not overlap (strides {t.stride()}, address mod 16 = {t.data_ptr() % 16})")
 
 
 def _vec(t, name, n, dtypes):
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.shape != (n,) or not t.is_contiguous() or t.data_ptr() % 16:
-        raise ValueError(f"{name}: expected a contiguous, 16-byte aligned [{n}], got {tuple(t.shape)} strides {t.stride()}")
-
-
-def _on_device(**tensors):
-    """every operand lives on the current GPU: the launch goes to its current stream"""
-    cur = torch.cuda.current_device() if torch.cuda.is_available() else -2
-    for name, t in tensors.items():
-        if t is not None and t.get_device() != cur:
-            raise ValueError(f"{name} is on {t.device}; the call launches on the current GPU" + (f", cuda:{cur}" if cur >= 0 else ", and there is none"))
-
-
-def _adr(t):
-    """device address for a pointer field (kept alive like _ptr while launches are recorded)"""
     if t is None:
         return None
+    p = t.data_ptr()
+    if t.dtype in dtypes and t.shape == (n,) and t.is_contiguous() and not p & 15:
+        return p
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    raise ValueError(f"{name}: expected a contiguous, 16-byte aligned [{n}], got {tuple(t.shape)} strides {t.stride()}")
+
+
+def _on_device(names, tensors):
+    """every operand lives on the current GPU (the launch goes to its current stream), and as long as a launch list that is being recorded"""
+    dev = None
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if dev is None:
+                dev = d
+            if d < 0 or d != dev:
+                raise ValueError(f"{names}: expected tensors of one GPU, got {[str(t.device) for t in tensors if t is not None]}")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"{names} are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    if _REC is not None:
+        _REC.append(("_keepalive", tensors))
+
+
+def _scratch(nbytes, like):
+    t = torch.empty(max(1, (nbytes + 3) // 4), dtype=torch.float32, device=like.device)
     if _REC is not None:
         _REC.append(("_keepalive", (t,)))
-    return t.data_ptr()
-
-
-def _scratch(nbytes, device):
-    return torch.empty(max(1, (nbytes + 3) // 4), dtype=torch.float32, device=device)
+    return t
 
 
 def _norm_shape(x):
@@ -1250,94 +1265,90 @@ def _norm_shape(x):
 
 
 def _norm_stat(t, name, M):
-    if t is not None and (t.dtype != torch.float32 or t.shape != (M,) or not t.is_contiguous()):
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or t.shape != (M,) or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous fp32 [{M}], got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+_F32 = (torch.float32,)
+_W_TYPES = (BF16, torch.float32)
 
 
 def norm_fwd(x, weight, y, *, bias=None, rms=False, mean=None, rstd=None, eps=1e-6):
     """y = xh * weight (+ bias) per row of x [M, C] bf16: xh = (x - mean) / sqrt(var + eps) (layer norm) or x / sqrt(mean(x^2) + eps) (rms: no mean, no bias).
     weight / bias [C] bf16 or fp32 (both the same); mean / rstd: fp32 [M], written for norm_bwd (mean: layer norm only).  y may be x.  C % 8 == 0, C <= 8192."""
-    M, Cc = _norm_shape(x)
+    shape = _norm_shape(x)
+    M, Cc = shape
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
     if rms and (bias is not None or mean is not None):
         raise ValueError("an RMS norm has neither bias nor mean")
-    a = _capi.NormArgs()
-    a.ldx, a.ldy = _rows(x, "x", M, Cc), _rows(y, "y", M, Cc)
-    _vec(weight, "weight", Cc, (BF16, torch.float32))
-    if bias is not None:
-        _vec(bias, "bias", Cc, (weight.dtype,))
-    _norm_stat(mean, "mean", M)
-    _norm_stat(rstd, "rstd", M)
-    _on_device(x=x, weight=weight, y=y, bias=bias, mean=mean, rstd=rstd)
-    if M == 0:
-        return y
-    a.x, a.weight, a.bias, a.y, a.mean, a.rstd = _adr(x), _adr(weight), _adr(bias), _adr(y), _adr(mean), _adr(rstd)
-    a.eps, a.rms, a.w_f32, a.M, a.C = eps, int(rms), int(weight.dtype == torch.float32), M, Cc
-    _call("aitk_norm_fwd", C.byref(a))
+    px, ldx = _rows(x, "x", shape)
+    py, ldy = _rows(y, "y", shape)
+    a = _capi.NormArgs(px, ldx, _vec(weight, "weight", Cc, _W_TYPES), _vec(bias, "bias", Cc, (weight.dtype,)), py, ldy, _norm_stat(mean, "mean", M),
+                       _norm_stat(rstd, "rstd", M), eps, 1 if rms else 0, 1 if weight.dtype is torch.float32 else 0, M, Cc)
+    _on_device("x, weight, y, bias, mean, rstd", (x, weight, y, bias, mean, rstd))
+    if M:
+        _call("aitk_norm_fwd", C.byref(a))
     return y
 
 
 def norm_bwd(dy, x, weight, rstd, dx, *, mean=None, rms=False, dres=None, dweight=None, dbias=None, accumulate=False):
     """dx = norm_fwd's gradient . dy (+ dres) from the saved rstd (and, layer norm, mean); dweight / dbias (fp32 [C], either may be left out) = the gradients of weight
     and bias, added to what they hold with `accumulate`.  dx may be dy, x or dres.  Deterministic."""
-    M, Cc = _norm_shape(x)
+    shape = _norm_shape(x)
+    M, Cc = shape
     if (mean is None) != bool(rms):
         raise ValueError("mean: a layer norm needs the saved mean, an RMS norm has none")
     if rms and dbias is not None:
         raise ValueError("dbias: an RMS norm has no bias")
-    a = _capi.NormBwdArgs()
-    a.ld_dy, a.ldx, a.ld_dx = _rows(dy, "dy", M, Cc), _rows(x, "x", M, Cc), _rows(dx, "dx", M, Cc)
-    if dres is not None:
-        a.ld_dres = _rows(dres, "dres", M, Cc)
-    _vec(weight, "weight", Cc, (BF16, torch.float32))
-    _norm_stat(mean, "mean", M)
-    _norm_stat(rstd, "rstd", M)
-    for t, name in ((dweight, "dweight"), (dbias, "dbias")):
-        if t is not None:
-            _vec(t, name, Cc, (torch.float32,))
-    _on_device(dy=dy, x=x, weight=weight, rstd=rstd, dx=dx, mean=mean, dres=dres, dweight=dweight, dbias=dbias)
+    pdy, ld_dy = _rows(dy, "dy", shape)
+    px, ldx = _rows(x, "x", shape)
+    pdx, ld_dx = _rows(dx, "dx", shape)
+    pres, ld_dres = (None, 0) if dres is None else _rows(dres, "dres", shape)
+    a = _capi.NormBwdArgs(pdy, ld_dy, px, ldx, _vec(weight, "weight", Cc, _W_TYPES), _norm_stat(mean, "mean", M), _norm_stat(rstd, "rstd", M), pres, ld_dres, pdx, ld_dx,
+                          _vec(dweight, "dweight", Cc, _F32), _vec(dbias, "dbias", Cc, _F32), None, 1 if rms else 0, 1 if weight.dtype is torch.float32 else 0,
+                          1 if accumulate else 0, M, Cc)
+    _on_device("dy, x, weight, rstd, dx, mean, dres, dweight, dbias", (dy, x, weight, rstd, dx, mean, dres, dweight, dbias))
     if M == 0:
         if not accumulate:
             host_call(lambda: [t.zero_() for t in (dweight, dbias) if t is not None])
         return dx
-    part = None
     if dweight is not None or dbias is not None:
-        part = _scratch(_capi.lib().aitk_norm_bwd_workspace_bytes(M, Cc, int(rms)), x.device)
-    a.dy, a.x, a.weight, a.mean, a.rstd, a.dres, a.dx = _adr(dy), _adr(x), _adr(weight), _adr(mean), _adr(rstd), _adr(dres), _adr(dx)
-    a.dweight, a.dbias, a.partial = _adr(dweight), _adr(dbias), _adr(part)
-    a.rms, a.w_f32, a.accumulate, a.M, a.C = int(rms), int(weight.dtype == torch.float32), int(accumulate), M, Cc
+        part = _scratch(_capi.lib().aitk_norm_bwd_workspace_bytes(M, Cc, 1 if rms else 0), x)
+        a.partial = part.data_ptr()
     _call("aitk_norm_bwd", C.byref(a))
     return dx
 
 
-def _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal):
+def _attn_relpos_check(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal):
     if not (B >= 0 and H > 0 and S >= 0 and 0.0 < scale < 1e30):
         raise ValueError(f"B, H, S, scale: got {B}, {H}, {S}, {scale} (scale must be positive and finite)")
-    a = _capi.AttnRelposArgs()
-    n, w = B * S, H * 64
-    a.ldq, a.ldk, a.ldv, a.ldo = _rows(q, "q", n, w), _rows(k, "k", n, w), _rows(v, "v", n, w), _rows(o, "o", n, w)
-    if lse.dtype != torch.float32 or lse.numel() != n * H or not lse.is_contiguous():
+    shape = (B * S, H * 64)
+    pq, ldq = _rows(q, "q", shape)
+    pk, ldk = _rows(k, "k", shape)
+    pv, ldv = _rows(v, "v", shape)
+    po, ldo = _rows(o, "o", shape)
+    if lse.dtype is not torch.float32 or lse.numel() != B * H * S or not lse.is_contiguous():
         raise ValueError(f"lse: expected a contiguous fp32 [{B}, {H}, {S}], got {lse.dtype} {tuple(lse.shape)}")
+    nb, pt, pm = 0, None, None
     if table is not None:
-        if table.dtype != BF16 or table.dim() != 2 or table.shape[1] != H or not table.is_contiguous():
+        if table.dtype is not BF16 or table.dim() != 2 or table.shape[1] != H or not table.is_contiguous():
             raise ValueError(f"table: expected a contiguous bf16 [num_buckets, {H}], got {table.dtype} {tuple(table.shape)}")
-        a.num_buckets, a.max_distance = table.shape[0], max_distance
-        half = a.num_buckets if causal else a.num_buckets // 2
-        if not 2 <= half <= 64 or (not causal and a.num_buckets % 2) or not half // 2 < max_distance <= 1024:
-            raise ValueError(f"table: {a.num_buckets} buckets up to distance {max_distance} (causal={bool(causal)}): 2 to 64 buckets of each sign, the exact half of them "
+        nb, pt = table.shape[0], table.data_ptr()
+        half = nb if causal else nb // 2
+        if not 2 <= half <= 64 or (not causal and nb % 2) or not half // 2 < max_distance <= 1024:
+            raise ValueError(f"table: {nb} buckets up to distance {max_distance} (causal={bool(causal)}): 2 to 64 buckets of each sign, the exact half of them "
                              "below max_distance <= 1024")
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, S) or not key_mask.is_contiguous():
             raise ValueError(f"key_mask: expected a contiguous bool or uint8 [{B}, {S}] (non-zero = attend), got {key_mask.dtype} {tuple(key_mask.shape)}")
-    if (S + 64) * max(a.ldq, a.ldk, a.ldv) * 2 >= 2 ** 31 - 1 or n * H >= 2 ** 31:
+        pm = key_mask.data_ptr()
+    if (S + 64) * max(ldq, ldk, ldv) * 2 >= 2 ** 31 - 1 or B * H * S >= 2 ** 31:
         raise ValueError(f"a head's slice of q, k and v must stay below 2 GiB and B S H below 2^31 (B, H, S = {B}, {H}, {S})")
-    a.scale, a.B, a.H, a.S, a.causal = scale, B, H, S, int(causal)
-    return a
-
-
-def _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask):
-    a.Q, a.K, a.V, a.O, a.LSE, a.table, a.key_mask = _adr(q), _adr(k), _adr(v), _adr(o), _adr(lse), _adr(table), _adr(key_mask)
+    return shape, nb, (pq, pk, pv, ldq, ldk, ldv, po, ldo, lse.data_ptr(), pt, pm)
 
 
 def attn_relpos_fwd(q, k, v, table, o, lse, *, B, H, S, scale=1.0, key_mask=None, max_distance=128, causal=False):
@@ -1345,12 +1356,11 @@ def attn_relpos_fwd(q, k, v, table, o, lse, *, B, H, S, scale=1.0, key_mask=None
     (row pitch = token pitch); table: bf16 [num_buckets, H] (T5's relative_attention_bias.weight) or None (no bias: CLIP); lse: fp32 [B, H, S], written for the backward.
     key_mask: bool / uint8 [B, S], non-zero = attend; causal: keys up to the query, all buckets for the past.  A row that the masks leave empty gives 0 (lse = -inf);
     what masked keys hold reaches nothing, NaN and infinities too."""
-    a = _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
-    _on_device(q=q, k=k, v=v, table=table, o=o, lse=lse, key_mask=key_mask)
-    if B * S == 0:
-        return o
-    _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask)
-    _call("aitk_attn_relpos_fwd", C.byref(a))
+    _, nb, head = _attn_relpos_check(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
+    a = _capi.AttnRelposArgs(*head, None, 0, None, None, None, 0, 0, 0, None, None, scale, B, H, S, nb, max_distance, 1 if causal else 0)
+    _on_device("q, k, v, table, o, lse, key_mask", (q, k, v, table, o, lse, key_mask))
+    if B * S:
+        _call("aitk_attn_relpos_fwd", C.byref(a))
     return o
 
 
@@ -1358,29 +1368,33 @@ def attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable=None, *, B, H
     """dq, dk, dv ([B*S, H*64] bf16 views) and, if given, dtable ([num_buckets, H] bf16 or fp32: the table's gradient, added to what it holds with `accumulate` — T5's layers
     share one table) from attn_relpos_fwd's operands, o and lse.  The probabilities are recomputed; every sum has a fixed order.  dtable's fp32 form is as exact as the
     bf16 operands o and do it is formed from, not more."""
-    a = _attn_relpos_args(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
-    n, w = B * S, H * 64
-    a.lddo, a.lddq, a.lddk, a.lddv = _rows(do, "do", n, w), _rows(dq, "dq", n, w), _rows(dk, "dk", n, w), _rows(dv, "dv", n, w)
-    if (S + 64) * a.lddo * 2 >= 2 ** 31 - 1:
+    shape, nb, head = _attn_relpos_check(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
+    pdo, lddo = _rows(do, "do", shape)
+    pdq, lddq = _rows(dq, "dq", shape)
+    pdk, lddk = _rows(dk, "dk", shape)
+    pdv, lddv = _rows(dv, "dv", shape)
+    if (S + 64) * lddo * 2 >= 2 ** 31 - 1:
         raise ValueError("a head's slice of do must stay below 2 GiB")
-    if dtable is not None and (table is None or dtable.dtype not in (BF16, torch.float32) or dtable.shape != table.shape or not dtable.is_contiguous()):
-        raise ValueError(f"dtable: expected the table's shape, contiguous, in bf16 or fp32, got {dtable.dtype} {tuple(dtable.shape)}" + (" without a table" if table is None else ""))
-    _on_device(q=q, k=k, v=v, table=table, o=o, lse=lse, do=do, dq=dq, dk=dk, dv=dv, dtable=dtable, key_mask=key_mask)
+    pdt, f32 = None, 0
+    if dtable is not None:
+        if table is None or dtable.dtype not in _W_TYPES or dtable.shape != table.shape or not dtable.is_contiguous():
+            raise ValueError(f"dtable: expected the table's shape, contiguous, in bf16 or fp32, got {dtable.dtype} {tuple(dtable.shape)}" + (" without a table" if table is None else ""))
+        pdt, f32 = dtable.data_ptr(), 1 if dtable.dtype is torch.float32 else 0
+    _on_device("q, k, v, table, o, lse, do, dq, dk, dv, dtable, key_mask", (q, k, v, table, o, lse, do, dq, dk, dv, dtable, key_mask))
     if B * S == 0:
         if dtable is not None and not accumulate:
             host_call(lambda: dtable.zero_())
         return
-    ws = _scratch(_capi.lib().aitk_attn_relpos_bwd_workspace_bytes(B, H, S, a.num_buckets if dtable is not None else 0), q.device)
-    _attn_relpos_ptrs(a, q, k, v, table, o, lse, key_mask)
-    a.dO, a.dQ, a.dK, a.dV, a.dtable, a.ws = _adr(do), _adr(dq), _adr(dk), _adr(dv), _adr(dtable), _adr(ws)
-    a.dtable_f32, a.accumulate = int(dtable is not None and dtable.dtype == torch.float32), int(accumulate)
+    ws = _scratch(_capi.lib().aitk_attn_relpos_bwd_workspace_bytes(B, H, S, nb if dtable is not None else 0), q)
+    a = _capi.AttnRelposArgs(*head, pdo, lddo, pdq, pdk, pdv, lddq, lddk, lddv, pdt, ws.data_ptr(), scale, B, H, S, nb, max_distance, 1 if causal else 0, f32,
+                             1 if accumulate else 0)
     _call("aitk_attn_relpos_bwd", C.byref(a))
 
 
 GATED_ACTS = {"gelu_tanh": 0, "gelu": 1, "silu": 2}
 
 
-def _ffn_shape(x, w_val, w_gate, act):
+def _ffn_check(x, w_val, w_gate, act):
     if act not in GATED_ACTS:
         raise ValueError(f"act: expected one of {sorted(GATED_ACTS)}, got {act!r}")
     if x.dim() != 2 or w_val.dim() != 2 or x.shape[1] != w_val.shape[1]:
@@ -1389,10 +1403,12 @@ def _ffn_shape(x, w_val, w_gate, act):
     F = w_val.shape[0]
     if K <= 0 or F <= 0 or K % 8 or F % 8 or 2 * F > 1 << 20:
         raise ValueError(f"K and F must be positive multiples of 8 (2 F up to 2^20), got K = {K}, F = {F}")
-    ldw = _rows(w_val, "w_val", F, K)
-    if _rows(w_gate, "w_gate", F, K) != ldw:
-        raise ValueError(f"w_val and w_gate must share one row pitch, got {w_val.stride(0)} and {w_gate.stride(0)}")
-    return M, K, F, ldw
+    pv, ldw = _rows(w_val, "w_val", (F, K))
+    pg, ldg = _rows(w_gate, "w_gate", (F, K))
+    if ldg != ldw:
+        raise ValueError(f"w_val and w_gate must share one row pitch, got {ldw} and {ldg}")
+    px, ldx = _rows(x, "x", (M, K))
+    return M, K, F, px, ldx, pv, pg, ldw
 
 
 def _pitches(*lds):
@@ -1404,54 +1420,40 @@ def gated_ffn_fwd(x, w_val, w_gate, out, *, act="gelu_tanh", b_val=None, b_gate=
     """out = (x w_val^T + b_val) * act(x w_gate^T + b_gate) in one launch: x [M, K], weights [F, K] (one row pitch: two views of a fused [2F, K] matrix, or two matrices),
     biases [F] or None, out [M, F], all bf16.  act: "gelu_tanh" (T5 / UMT5), "gelu" (erf: GEGLU) or "silu".  hg [M, 2F]: also leaves [value | gate] before the
     activation, which gated_ffn_bwd needs (geglu_fwd's layout).  K % 8 == F % 8 == 0."""
-    M, K, F, ldw = _ffn_shape(x, w_val, w_gate, act)
-    a = _capi.GatedFfnArgs()
-    a.ldx, a.ld_out, a.ldw = _rows(x, "x", M, K), _rows(out, "out", M, F), ldw
-    if hg is not None:
-        a.ld_hg = _rows(hg, "hg", M, 2 * F)
-    if b_val is not None:
-        _vec(b_val, "b_val", F, (BF16,))
-    if b_gate is not None:
-        _vec(b_gate, "b_gate", F, (BF16,))
-    _pitches(a.ldx, a.ld_out, a.ld_hg, ldw)
-    _on_device(x=x, w_val=w_val, w_gate=w_gate, out=out, b_val=b_val, b_gate=b_gate, hg=hg)
-    if M == 0:
-        return out
-    a.x, a.w_val, a.w_gate, a.b_val, a.b_gate, a.out, a.hg = _adr(x), _adr(w_val), _adr(w_gate), _adr(b_val), _adr(b_gate), _adr(out), _adr(hg)
-    a.M, a.K, a.F, a.act = M, K, F, GATED_ACTS[act]
-    _call("aitk_gated_ffn_fwd", C.byref(a))
+    M, K, F, px, ldx, pv, pg, ldw = _ffn_check(x, w_val, w_gate, act)
+    po, ld_out = _rows(out, "out", (M, F))
+    ph, ld_hg = (None, 0) if hg is None else _rows(hg, "hg", (M, 2 * F))
+    _pitches(ldx, ld_out, ld_hg, ldw)
+    a = _capi.GatedFfnArgs(px, ldx, pv, pg, ldw, _vec(b_val, "b_val", F, (BF16,)), _vec(b_gate, "b_gate", F, (BF16,)), po, ld_out, ph, ld_hg, M, K, F, GATED_ACTS[act])
+    _on_device("x, w_val, w_gate, out, b_val, b_gate, hg", (x, w_val, w_gate, out, b_val, b_gate, hg))
+    if M:
+        _call("aitk_gated_ffn_fwd", C.byref(a))
     return out
 
 
 def gated_ffn_bwd(dh, x, w_val, w_gate, hg, *, act="gelu_tanh", dx=None, dw_val=None, dw_gate=None, db_val=None, db_gate=None):
     """gated_ffn_fwd's gradients from dh [M, F] and the saved hg: dx [M, K], dw_val / dw_gate [F, K] (one row pitch), db_val / db_gate [F], all bf16; only what is
     given is computed (frozen weights: dx alone).  Nothing is transposed or copied beyond the one [M, 2F] gradient of hg.  Deterministic."""
-    M, K, F, ldw = _ffn_shape(x, w_val, w_gate, act)
-    a = _capi.GatedFfnBwdArgs()
-    a.ld_dh, a.ldx, a.ld_hg, a.ldw = _rows(dh, "dh", M, F), _rows(x, "x", M, K), _rows(hg, "hg", M, 2 * F), ldw
-    if dx is not None:
-        a.ld_dx = _rows(dx, "dx", M, K)
-    if dw_val is not None:
-        a.ld_dw = _rows(dw_val, "dw_val", F, K)
+    M, K, F, px, ldx, pv, pg, ldw = _ffn_check(x, w_val, w_gate, act)
+    pdh, ld_dh = _rows(dh, "dh", (M, F))
+    phg, ld_hg = _rows(hg, "hg", (M, 2 * F))
+    pdx, ld_dx = (None, 0) if dx is None else _rows(dx, "dx", (M, K))
+    pdv, ld_dw = (None, 0) if dw_val is None else _rows(dw_val, "dw_val", (F, K))
+    pdg = None
     if dw_gate is not None:
-        ld = _rows(dw_gate, "dw_gate", F, K)
-        if dw_val is not None and ld != a.ld_dw:
-            raise ValueError(f"dw_val and dw_gate must share one row pitch, got {a.ld_dw} and {ld}")
-        a.ld_dw = ld
-    if db_val is not None:
-        _vec(db_val, "db_val", F, (BF16,))
-    if db_gate is not None:
-        _vec(db_gate, "db_gate", F, (BF16,))
-    _pitches(a.ld_dh, a.ldx, a.ld_hg, ldw, a.ld_dx, a.ld_dw)
-    if M > 64 * 65535:
-        raise ValueError(f"at most {64 * 65535} rows, got {M}")
-    _on_device(dh=dh, x=x, w_val=w_val, w_gate=w_gate, hg=hg, dx=dx, dw_val=dw_val, dw_gate=dw_gate, db_val=db_val, db_gate=db_gate)
+        pdg, ld = _rows(dw_gate, "dw_gate", (F, K))
+        if dw_val is not None and ld != ld_dw:
+            raise ValueError(f"dw_val and dw_gate must share one row pitch, got {ld_dw} and {ld}")
+        ld_dw = ld
+    pbv, pbg = _vec(db_val, "db_val", F, (BF16,)), _vec(db_gate, "db_gate", F, (BF16,))
+    _pitches(ld_dh, ldx, ld_hg, ldw, ld_dx, ld_dw)
+    if M > 32 * 65535:
+        raise ValueError(f"at most {32 * 65535} rows, got {M}")
+    _on_device("dh, x, w_val, w_gate, hg, dx, dw_val, dw_gate, db_val, db_gate", (dh, x, w_val, w_gate, hg, dx, dw_val, dw_gate, db_val, db_gate))
     if M == 0:
         host_call(lambda: [t.zero_() for t in (dw_val, dw_gate, db_val, db_gate) if t is not None])
         return dx
-    ws = _scratch(_capi.lib().aitk_gated_ffn_bwd_workspace_bytes(M, K, F, dx is not None, dw_val is not None, dw_gate is not None, db_val is not None or db_gate is not None), x.device)
-    a.dh, a.x, a.w_val, a.w_gate, a.hg = _adr(dh), _adr(x), _adr(w_val), _adr(w_gate), _adr(hg)
-    a.dx, a.dw_val, a.dw_gate, a.db_val, a.db_gate, a.ws = _adr(dx), _adr(dw_val), _adr(dw_gate), _adr(db_val), _adr(db_gate), _adr(ws)
-    a.M, a.K, a.F, a.act = M, K, F, GATED_ACTS[act]
+    ws = _scratch(_capi.lib().aitk_gated_ffn_bwd_workspace_bytes(M, K, F, dx is not None, dw_val is not None, dw_gate is not None, db_val is not None or db_gate is not None), x)
+    a = _capi.GatedFfnBwdArgs(pdh, ld_dh, px, ldx, pv, pg, ldw, phg, ld_hg, pdx, ld_dx, pdv, pdg, ld_dw, pbv, pbg, ws.data_ptr(), M, K, F, GATED_ACTS[act])
     _call("aitk_gated_ffn_bwd", C.byref(a))
     return dx

@@ -181,7 +181,7 @@ def test_attention_wrapper_refusals():
     with pytest.raises(ValueError, match="GPU"):
         ops.attn_relpos_fwd(*args, B=B, H=H, S=S)
     with pytest.raises(ValueError, match="2 GiB"):
-        ops._attn_relpos_args(*_huge_views(), B=1, H=1, S=600, scale=1.0, key_mask=None, max_distance=128, causal=False)
+        ops.attn_relpos_fwd(*_huge_views(), B=1, H=1, S=600)
     do, dq, dk, dv = mk(), mk(), mk(), mk()
     for bad, match in ((dict(dtable=_t(32, H, dtype=torch.float16)), "dtable"), (dict(dtable=_t(16, H)), "dtable"), (dict(table=None, dtable=_t(32, H)), "without a table"),
                        (dict(do=_t(B * S, 64)), "do"), (dict(dv=mk().float()), "dv")):
