@@ -569,17 +569,23 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       fars[4 + wave] = fs_ahead;
     }
     __syncthreads();
-    const lds_float* all = line + 4 * r.line_p;
-    if (tid < a.num_buckets) {
-      const bool ahead = tid >= r.half;
-      const int j = ahead ? tid - r.half : tid;
+    lds_float* const all = line + 4 * r.line_p;
+    for (int i = tid; i < n_line; i += 256) all[i] = (all[i] + all[n_line + i]) + (all[2 * n_line + i] + all[3 * n_line + i]);
+    __syncthreads();
+    // eight lanes to a bucket: one lane's walk over the last bucket's distances is a chain of LDS reads as long as two key tiles
+    for (int i = tid; i < a.num_buckets * 8; i += 256) {
+      const int bucket = i >> 3;
+      const bool ahead = bucket >= r.half;
+      const int j = ahead ? bucket - r.half : bucket;
       const bool last = j == r.half - 1;
-      const int n0 = r.first[j], n1 = last ? E + 1 : r.first[j + 1];
+      const int n0 = ahead && j == 0 ? 1 : r.first[j], n1 = last ? E + 1 : r.first[j + 1];
       float v = 0.f;
-      if (last) v = ahead ? fars[4] + fars[5] + fars[6] + fars[7] : fars[0] + fars[1] + fars[2] + fars[3];
-      for (int n = n0 > 0 || !ahead ? n0 : 1; n < n1; ++n)
-        for (int w = 0; w < 4; ++w) v += all[w * n_line + E + (ahead ? n : -n)];
-      r.part[(((long)b * ((S + 127) / 128) + tile_x) * a.H + hd) * a.num_buckets + tid] = v;
+      for (int n = n0 + (i & 7); n < n1; n += 8) v += all[E + (ahead ? n : -n)];
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+      const int f = ahead ? 4 : 0;
+      if (last) v += (fars[f] + fars[f + 1]) + (fars[f + 2] + fars[f + 3]);
+      if ((i & 7) == 0) r.part[(((long)b * ((S + 127) / 128) + tile_x) * a.H + hd) * a.num_buckets + bucket] = v;
     }
   }
 }
@@ -658,7 +664,7 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
           s = mfma32(frag_rm(qt, L, j, ks), kf[ks], s);
           dp = mfma32(frag_rm(gt, L, j, ks), vf[ks], dp);
         }
-          __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const f32x4_t nl = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 32 * j + 8 * g + 4 * h);
