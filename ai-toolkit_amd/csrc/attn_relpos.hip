@@ -134,27 +134,26 @@ __device__ __forceinline__ f32x16_t load_line(const lds_float* line, int line_p,
   return s;
 }
 
-// bucket of a distance n >= 0 within its sign
-__device__ __forceinline__ int bucket_of(const RelposArgs& r, int n) {
-  int j = 0;
-  for (int i = 1; i < r.half; ++i) j += r.first[i] <= n;
-  return j;
-}
-// bias of relative position d = key - query, divided by the softmax scale (it joins the scores before they are multiplied by it)
-__device__ __forceinline__ float bias_of(const RelposArgs& r, int d, int hd, float inv_scale) {
-  const int n = d > 0 ? (r.a.causal ? 0 : d) : -d;
-  const int j = bucket_of(r, n) + (d > 0 && !r.a.causal ? r.half : 0);
-  return bf2f(r.a.table[(long)j * r.a.H + hd]) * inv_scale;
-}
-// the four shifted copies: copy c, entry i = bias of distance sign * (i + c - E)
+// The four shifted copies of the line: copy c, entry i = the bias of distance sign * (i + c - E), divided by the softmax scale (it joins the scores before they are multiplied by
+// it).  Eight lanes to a bucket walk its distances: one load of the table per lane, where a search of the bucket per distance cost every workgroup 1 us more.  Causal: what lies ahead
+// is masked and takes bucket 0.
 __device__ __forceinline__ void build_line(lds_float* line, const RelposArgs& r, int hd, int sign) {
   const int E = r.sat + BAND_PAD;
   const float inv = 1.0f / r.a.scale;
-  for (int i = threadIdx.x; i < 2 * E + 1; i += 256) {
-    const float b = bias_of(r, sign * (i - E), hd, inv);
+  const bool causal = r.a.causal != 0;
+  for (int i = threadIdx.x; i < (causal ? r.half + 1 : 2 * r.half) * 8; i += 256) {
+    const int k = i >> 3;
+    const bool ahead = k >= r.half;
+    const int j = ahead ? (causal ? 0 : k - r.half) : k;
+    const float b = bf2f(r.a.table[(long)(causal ? j : k) * r.a.H + hd]) * inv;
+    const int n0 = j || !ahead ? r.first[j] : 1, n1 = j == r.half - 1 || (causal && ahead) ? E + 1 : r.first[j + 1];
+    const int dir = ahead == (sign > 0) ? 1 : -1;
+    for (int n = n0 + (i & 7); n < n1; n += 8) {
+      const int at = E + dir * n;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (i - c >= 0) line[c * r.line_p + i - c] = b;
+      for (int c = 0; c < 4; ++c)
+        if (at - c >= 0) line[c * r.line_p + at - c] = b;
+    }
   }
 }
 // keep-bits of 64 key tiles [t0, t0 + 64) of one sample: lane t gets tile t0 + t.  `box`: 64 x 8 bytes of LDS, rewritten here; ends behind a barrier.
@@ -255,11 +254,13 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
     if (more) fetch(sm, t, keep);
     if (BIAS && t0 == 0) {  // with the first tiles on their way
       build_line(line, r, hd, 1);
-      far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
-      far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
     }
     dma_wait_all();
     __syncthreads();
+    if (BIAS && t0 == 0) {
+      far_past = line[E - r.sat] * c2;
+      far_ahead = line[E + r.sat] * c2;
+    }
     while (more) {
       more = todo != 0;
       int tn = 0;
@@ -442,27 +443,29 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   // bucket of a sign, which takes a row's far keys all with one sign, does: its sum is corrected by (row sum of ds) x (row's p in the bucket).
   float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f, fp_past = 0.f, fp_ahead = 0.f, row_ds = 0.f;
   const int ib = E + 4 * h - q0 - l31;
-  if constexpr (BIAS) {
-    build_line(line, r, hd, 1);
-    far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale) * c2;
-    far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale) * c2;
-    if (sums)
-      for (int i = tid; i < (4 * n_line + 3) / 4 * 4 + 4 * 8 * SKEW_P; i += 256) (line + 4 * r.line_p)[i] = 0.f;
-    __syncthreads();
-  }
   f32x16_t dq[2] = {zero16(), zero16()};
   const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * 128 + 127) / 64 + 1) : (S + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += 64) {
     const unsigned long long masks = tile_masks(a, b, t0, ntiles, box, lane, wave);
     unsigned long long todo = __ballot(masks != 0);
-    if (!todo) continue;
-    int t = __builtin_ctzll(todo), cur = 0;
+    int t = todo ? __builtin_ctzll(todo) : 0, cur = 0;
     unsigned long long keep = lane64(masks, t);
-    stage(sm, L, a.ldk, (t0 + t) * 64, srdK, wave, keep);
-    stage(sm + TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, keep);
+    if (todo) {
+      stage(sm, L, a.ldk, (t0 + t) * 64, srdK, wave, keep);
+      stage(sm + TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, keep);
+    }
+    if (BIAS && t0 == 0) {  // with the first tiles on their way
+      build_line(line, r, hd, 1);
+      if (sums)
+        for (int i = tid; i < (4 * n_line + 3) / 4 * 4 + 4 * 8 * SKEW_P; i += 256) (line + 4 * r.line_p)[i] = 0.f;
+    }
     dma_wait_all();
     __syncthreads();
-    while (true) {
+    if (BIAS && t0 == 0) {
+      far_past = line[E - r.sat] * c2;
+      far_ahead = line[E + r.sat] * c2;
+    }
+    while (todo) {
       todo &= todo - 1;
       const int tn = todo ? __builtin_ctzll(todo) : 0;
       const unsigned long long keep_n = lane64(masks, tn);
@@ -552,7 +555,6 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       }
       dma_wait_all();
       __syncthreads();
-      if (!todo) break;
       t = tn;
       keep = keep_n;
       cur ^= 1;
@@ -628,11 +630,6 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
     const int E = r.sat + BAND_PAD;
     const int ib = E + 4 * h - key;  // line index of query 0 of this lane's first register: entry i is the bias of key - query = E - i
     float far_past = 0.f, far_ahead = 0.f;  // not in the log2 domain here: start values like the line's
-    if constexpr (BIAS) {
-      build_line(line, r, hd, -1);
-      far_past = bias_of(r, -r.sat, hd, 1.0f / a.scale);
-      far_ahead = bias_of(r, r.sat, hd, 1.0f / a.scale);
-    }
     // rows past the end arrive as zeros: dO = 0 and delta = 0, so they add nothing to either gradient
     auto stage_all = [&](int t, int buf) {
       stage(sm + buf * 2 * TILE, L, a.ldq, t * 64, srdQ, wave, ~0ull);
@@ -641,8 +638,13 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
         dma4(__builtin_amdgcn_readfirstlane((unsigned)(size_t)(st + buf * 128 + wave * 64)), (unsigned)((t * 64 + lane) * 4), wave ? srdD : srdL);
     };
     stage_all(first_tile, 0);
+    if (BIAS) build_line(line, r, hd, -1);
     dma_wait_all();
     __syncthreads();
+    if constexpr (BIAS) {
+      far_past = line[E + r.sat];
+      far_ahead = line[E - r.sat];
+    }
     for (int t = first_tile, cur = 0; t < ntiles; ++t, cur ^= 1) {
       if (t + 1 < ntiles) stage_all(t + 1, cur ^ 1);
       const lds_char* qt = sm + cur * 2 * TILE;
