@@ -524,6 +524,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
 #pragma unroll
             for (int e = 0; e < 16; ++e) fs += s[e];
             if (side == 0) {
+              float v[2] = {0.f, 0.f};
 #pragma unroll
               for (int p8 = 0; p8 < 4; ++p8) {
                 if (l31 >> 3 == p8) {
@@ -532,14 +533,13 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
                     *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(skew_w + 8 * g) = f32x4_t{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' stores: LDS keeps a wave's accesses in order
-                if (lane < 39) {
-                  float v[2] = {0.f, 0.f};
+                const int c = lane - 24 + 8 * p8;
+                const lds_float* const col = skew + ((unsigned)c < 39u ? c : 39);
 #pragma unroll
-                  for (int q = 0; q < 8; ++q) v[q & 1] += skew[q * SKEW_P + ((q + 1) & 3) + lane];
-                  acc[E + kv0 + 32 * j - q0 - 7 - 8 * p8 + lane] += v[0] + v[1];
-                }
+                for (int q = 0; q < 8; ++q) v[q & 1] += col[q * SKEW_P + ((q + 1) & 3)];
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
               }
+              acc[E + kv0 + 32 * j - q0 - 31 + lane] += v[0] + v[1];
             }
           }
 #pragma unroll
