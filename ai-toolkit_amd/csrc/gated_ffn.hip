@@ -3,8 +3,8 @@
 //   u = x Wv^T + bv,  z = x Wg^T + bg,  h = u act(z)                                                   x [M, K], Wv / Wg [F, K], h [M, F]
 //   du = dh act(z),  dz = dh u act'(z);   dx = du Wv + dz Wg,  dWv = du^T x,  dWg = dz^T x,  dbv / dbg = column sums of du / dz
 //
-// Forward: one launch for both projections, the activation and the product.  A workgroup's B tile is BN / 2 rows of Wg next to the SAME BN / 2 rows of Wv, so a wave's accumulators
-// hold gate and value of one output element in the same register slot and h is formed in registers; [u | z] leaves (as bf16) only when a backward pass will want it.
+// Forward: one launch for both projections, the activation and the product.  Every 32 rows of a workgroup's B tile are 16 rows of Wg next to the SAME 16 rows of Wv, so an accumulator
+// holds gate and value of one output element eight registers apart and h is formed in registers; [u | z] leaves (as bf16) only when a backward pass will want it.
 // Backward: one pass forms [du | dz] (bf16: the operands of the two products; the column sums take the fp32 values), one launch computes dx and both weight gradients.
 //
 // The products share one tile loop (v_mfma_f32_32x32x16_bf16, fp32 accumulators).  Stages of 32 contraction elements go straight from global memory to LDS (buffer loads; rows and
@@ -39,10 +39,28 @@ struct FfnArgs {
   int act, _pad;
 };
 
+// The normal distribution's Phi(z), and e = exp(-z^2 / 2), for the erf GELU: Phi(-x) = e P(1 / (1 + x / 4)) for x >= 0, where P is a polynomial of degree 7 fitted here to
+// exp(x^2 / 2) Phi(-x) (relative error 1.6e-7 up to x = 10, where Phi(-x) = 8e-24; with the roundings below 1e-6 up to 3, 5e-6 up to 10).  One exp and one reciprocal, where the library's erff has two
+// branches that a wave takes both (4096 x 640 x 2560 forward 57 us with it, 47 us so).
+__device__ __forceinline__ float phi_f(float z, float& e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.25f, fabsf(z), 1.0f));
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  float p = -0.09756391730033673f;
+  p = fmaf(p, t, 0.37102050773583856f);
+  p = fmaf(p, t, -0.32741976101566833f);
+  p = fmaf(p, t, 0.34794113047610714f);
+  p = fmaf(p, t, -0.017855954230578303f);
+  p = fmaf(p, t, 0.127858177201618f);
+  p = fmaf(p, t, 0.09578246310144875f);
+  p = fmaf(p, t, 0.00023743313234458844f);
+  const float q = e * p;
+  return z < 0.f ? q : 1.0f - q;
+}
 __device__ __forceinline__ float act_f(float z, int act) {
   if (act == ACT_GELU_TANH) return gelu_tanh_f(z);
-  if (act == ACT_GELU_ERF) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-  return z / (1.0f + __expf(-z));
+  float e;
+  if (act == ACT_GELU_ERF) return z * phi_f(z, e);
+  return z * sigmoid_fast_f(z);
 }
 // act'(z) next to act(z)
 __device__ __forceinline__ void act_grad_f(float z, int act, float& f, float& d) {
@@ -50,11 +68,12 @@ __device__ __forceinline__ void act_grad_f(float z, int act, float& f, float& d)
     f = gelu_tanh_f(z);
     d = gelu_tanh_grad_f(z);
   } else if (act == ACT_GELU_ERF) {
-    const float c = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+    float e;
+    const float c = phi_f(z, e);
     f = z * c;
-    d = c + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    d = fmaf(z * 0.3989422804014327f, e, c);
   } else {
-    const float s = 1.0f / (1.0f + __expf(-z));
+    const float s = sigmoid_fast_f(z);
     f = z * s;
     d = s * (1.0f + z * (1.0f - s));
   }
@@ -77,26 +96,31 @@ __device__ __forceinline__ void dma16(unsigned dst, unsigned voff, const v4i_t& 
 
 constexpr int BK = 32, NST = 4;  // contraction elements of a stage, stages in LDS
 
-// One operand's side of the tile loop: R rows (columns of C's other side) x BK of the contraction, KC: the contraction index is contiguous in memory.
-template <int R, int NT, bool KC>
+// One operand's side of the tile loop: R rows (columns of C's other side) x BK of the contraction, KC: the contraction index is contiguous in memory.  PAIR: blocks of 32 rows, 16 of
+// one matrix and the same 16 of another: a wave stages 16 rows at a time, so odd waves work on the second matrix.
+template <int R, int NT, bool KC, bool PAIR>
 struct Operand {
-  static constexpr int BYTES = R * BK * 2, NDMA = BYTES / (NT * 16);
+  static constexpr int BYTES = R * BK * 2, NDMA = BYTES / (NT * 16), COUNT = PAIR ? R / 2 : R;
   unsigned voff[KC ? NDMA : 1];
   int rd[2];  // KC: the row fragment's address (contraction step ks: ^ 32 ks); otherwise the transpose reads of row halves lo / hi
   const bf16_t* base;
   long ld;
-  int left;  // rows (KC) or columns of the matrix from the tile's first on, at most R
+  int left;  // rows (KC) or columns of the matrix from the tile's first on, at most COUNT
   int kout;  // KC: first contraction index of this lane's chunk
-  __device__ __forceinline__ void init(const bf16_t* p, long ld_, int r0, int count, int tid) {
+  __device__ __forceinline__ void init(const bf16_t* const (&seg)[2], long ld_, int r0, int count, int tid) {
     ld = ld_;
-    left = min(count - r0, R);
+    left = min(count - r0, COUNT);
+    const bf16_t* p = seg[PAIR ? __builtin_amdgcn_readfirstlane(tid >> 6) & 1 : 0];
     base = KC ? p + (long)r0 * ld : p + r0;
     const int lane = tid & 63, l31 = lane & 31, h = lane >> 5, i = lane & 15, gq = (lane >> 4) & 1;
     if constexpr (KC) {  // 64-byte rows, four of them per KiB-quarter: chunk ^ (row / 4), so that rows four apart (one bank group) differ
       const int row = tid >> 2;
       kout = ((tid & 3) ^ ((row >> 2) & 3)) * 8;
 #pragma unroll
-      for (int d = 0; d < NDMA; ++d) voff[d] = (unsigned)(((row + d * (NT / 4)) * ld + kout) * 2);
+      for (int d = 0; d < NDMA; ++d) {
+        const int r = row + d * (NT / 4);
+        voff[d] = (unsigned)(((PAIR ? (r >> 5) * 16 + (r & 15) : r) * ld + kout) * 2);
+      }
       rd[0] = l31 * 64 + ((h ^ ((l31 >> 2) & 3)) << 4);
     } else {  // blocks of 64 columns: BK rows of 128 bytes, chunk ^ rkey(row)
       const int row = (tid >> 3) % BK;
@@ -131,34 +155,46 @@ struct Operand {
   }
 };
 
-// The tile loop.  WR x WC waves; a wave owns MB x 32 rows and, of each half of the tile's columns, NB / 2 x 32.
+// The tile loop.  WR x WC waves; a wave owns MB x 32 rows and NB blocks of 32 columns of the tile.  PAIR: a block of 32 columns is 16 of p.B[0] (registers 0 .. 7 of the
+// accumulator) next to the same 16 of p.B[1] (registers 8 .. 15); the accumulators start from the biases.
 // Four stages of 32 contraction elements: while stage t is multiplied, t + 1 has landed for every wave (its first fragments are read ahead of the barrier that
 // separates the two, so the matrix units go on right behind it), t + 2 and t + 3 are on their way; one barrier a stage.
 template <int BM, int BN, int WR, int WC, bool AK, bool BKC, bool PAIR>
 struct TileLoop {
   static constexpr int NT = WR * WC * 64, MB = BM / WR / 32, NB = BN / WC / 32;
-  static constexpr int STAGE = (BM + BN) * BK * 2, BHALF = BN / 2 * BK * 2, DMAS = STAGE / (NT * 16);
-  typedef Operand<BM, NT, AK> OpA;
-  typedef Operand<PAIR ? BN / 2 : BN, NT, BKC> OpB;
-  static_assert(DMAS == 4 || DMAS == 8, "the counted waits below");
+  typedef Operand<BM, NT, AK, false> OpA;
+  typedef Operand<BN, NT, BKC, PAIR> OpB;
+  static constexpr int STAGE = OpA::BYTES + OpB::BYTES, DMAS = OpA::NDMA + OpB::NDMA;
+  static_assert(DMAS == 4 && NB % 2 == 0, "the counted waits below; stores of pairs of blocks");
   f32x16_t acc[MB][NB];
-  // first column, within the half tile, of a wave's block j % (NB / 2)
-  static __device__ __forceinline__ int col(int wc, int j) { return (wc * (NB / 2) + j % (NB / 2)) * 32; }
-  __device__ __forceinline__ void run(const Prod& p, int m0, int n0, char* smem, int piece = 0) {
+  // a wave's j-th block of 32 columns within the tile: neighbours where a store joins two of them; otherwise one of either half of the tile (4096 x 640 x 2560, both gradients: 83 us
+  // with neighbours, 80 us so)
+  static __device__ __forceinline__ int block(int wc, int j) { return PAIR ? wc * NB + j : j / (NB / 2) * (BN / 64) + wc * (NB / 2) + j % (NB / 2); }
+  __device__ __forceinline__ void run(const Prod& p, int m0, int n0, char* smem, int piece = 0, const bf16_t* b0 = nullptr, const bf16_t* b1 = nullptr) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WC, wc = wave % WC;
     lds_char* const sm = (lds_char*)smem;
     OpA A;
-    OpB B, B2;
-    A.init(p.A[0], p.lda, m0, p.M, tid);
-    B.init(p.B[0], p.ldb, n0, p.N, tid);
-    if constexpr (PAIR) B2.init(p.B[1], p.ldb, n0, p.N, tid);
+    OpB B;
+    A.init(p.A, p.lda, m0, p.M, tid);
+    B.init(p.B, p.ldb, n0, p.N, tid);
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    uint2 bias[NB][4] = {};  // four columns each: b0's 4 h and 8 + 4 h, b1's
+    if constexpr (PAIR) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int n = n0 + block(wc, j) * 16 + 8 * (k & 1) + 4 * ((tid >> 5) & 1);
+          const bf16_t* b = k < 2 ? b0 : b1;
+          if (b && n < p.N) bias[j][k] = *reinterpret_cast<const uint2*>(b + n);
+        }
+    }
     const int K = p.K, kt_seg = (K + BK - 1) / BK, all = kt_seg * p.nseg;
     const int t0 = PAIR ? 0 : (int)((long)all * piece / p.split), nkt = PAIR ? all : (int)((long)all * (piece + 1) / p.split);  // this piece's stages [t0, nkt)
     int ts = t0, k0 = ts * BK;  // the stage issued next, its first contraction index within its segment
@@ -175,8 +211,7 @@ struct TileLoop {
       }
       const unsigned dst = (unsigned)(size_t)sm + (ts & (NST - 1)) * STAGE;
       if (d < OpA::NDMA) A.stage(dst, k0, K, wave, d);
-      else if (d < OpA::NDMA + OpB::NDMA) B.stage(dst + BM * BK * 2, k0, K, wave, d - OpA::NDMA);
-      else if constexpr (PAIR) B2.stage(dst + BM * BK * 2 + BHALF, k0, K, wave, d - OpA::NDMA - OpB::NDMA);
+      else B.stage(dst + OpA::BYTES, k0, K, wave, d - OpA::NDMA);
       if (d == DMAS - 1) {
         ++ts;
         k0 += BK;
@@ -185,9 +220,7 @@ struct TileLoop {
     s16x8_t af[2][MB], bf[2][NB];
     auto read_a = [&](int set, int t, int ks, int i) { af[set][i] = A.frag(sm + (t & (NST - 1)) * STAGE, wr * (BM / WR) + i * 32, ks); };
     auto read_b = [&](int set, int t, int ks, int j) {
-      const lds_char* bt = sm + (t & (NST - 1)) * STAGE + BM * BK * 2;
-      const int half = j / (NB / 2);
-      bf[set][j] = PAIR ? B.frag(bt + half * BHALF, col(wc, j), ks) : B.frag(bt, half * (BN / 2) + col(wc, j), ks);
+      bf[set][j] = B.frag(sm + (t & (NST - 1)) * STAGE + OpA::BYTES, block(wc, j) * 32, ks);
     };
     // One contraction step: the products of `set`, row block by row block.  Behind the first row block go half of a stage's DMAs and the other set's reads: in front of it the
     // waves, which come from one barrier, would all wait for the address unit with the matrix units idle; later, the wait in front of the next step would find the reads under way
@@ -213,15 +246,9 @@ struct TileLoop {
     };
     // a wave's own DMAs are in order: all but the newest n stages' have landed
     auto landed = [&](int n) {
-      if (n >= 2) {
-        if constexpr (DMAS == 8) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-      } else if (n == 1) {
-        if constexpr (DMAS == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
+      if (n >= 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      else if (n == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
     auto barrier = [&]() {
       __builtin_amdgcn_sched_barrier(0);
@@ -232,6 +259,17 @@ struct TileLoop {
     for (int i = 0; i < 3 && ts < nkt; ++i) {
 #pragma unroll
       for (int d = 0; d < DMAS; ++d) issue(d);
+    }
+    if (PAIR && (b0 || b1)) {
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const uint32_t x = r & 2 ? bias[j][r >> 2].y : bias[j][r >> 2].x;
+            acc[i][j][r] = r & 1 ? bf_hi(x) : bf_lo(x);
+          }
     }
     landed(nkt - t0 - 1);
     barrier();
@@ -267,6 +305,23 @@ __device__ __forceinline__ uint4 trade(const float (&v)[4], const float (&w)[4])
   return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
+// Two neighbouring 16-column groups of 32 rows, as trade() leaves them (lane: row l31, columns 8 h .. + 7 of either group): rows 16 apart trade once more, so that a store covers 16 rows
+// x 64 bytes and not 32 x 32 (L2 takes a request per segment: the forward of 2048 x 4096 x 10240 with hg 407 -> 389 us).  All lanes take part.
+struct Out {
+  bf16_t* C;
+  long ld;
+  int M, N;
+};
+__device__ __forceinline__ void store_two(const Out& o, int m0, int n0, int lane, const uint4& a, const uint4& b) {
+  typedef unsigned u2_t __attribute__((ext_vector_type(2)));
+  const u2_t x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+  const u2_t z = __builtin_amdgcn_permlane16_swap(a.z, b.z, false, false), w = __builtin_amdgcn_permlane16_swap(a.w, b.w, false, false);
+  const int m = m0 + (lane & 15), n = n0 + (lane & 16) + 8 * (lane >> 5);
+  bf16_t* p = o.C + (long)m * o.ld + n;
+  if (m < o.M && n < o.N) *reinterpret_cast<uint4*>(p) = make_uint4(x[0], y[0], z[0], w[0]);
+  if (m + 16 < o.M && n < o.N) *reinterpret_cast<uint4*>(p + 16 * o.ld) = make_uint4(x[1], y[1], z[1], w[1]);
+}
+
 template <int BM, int BN, int WR, int WC>
 __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -276,48 +331,34 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) 
   tile_coords(blockIdx.x, tm * tn, tm, tn, ti, tj);
   typedef TileLoop<BM, BN, WR, WC, true, true, true> Loop;
   Loop T;
-  T.run(p, ti * BM, tj * (BN / 2), smem);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
-  const int m_w = ti * BM + (wave / WC) * (BM / WR);
+  T.run(p, ti * BM, tj * (BN / 2), smem, 0, a.bg, a.bv);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int j = 0; j < Loop::NB / 2; ++j) {
-    const int n_w = tj * (BN / 2) + Loop::col(wave % WC, j);
+  for (int j = 0; j < Loop::NB; j += 2) {
+    const int n = tj * (BN / 2) + Loop::block(wave % WC, j) * 16;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {  // 16 columns at a time
-      const int n0 = n_w + 16 * q + 4 * h, n = n_w + 16 * q + 8 * h;
-      float bv[2][4] = {}, bg[2][4] = {};
+    for (int i = 0; i < Loop::MB; ++i) {
+      const int m = ti * BM + (wave / WC) * (BM / WR) + i * 32;
+      uint4 ov[2], uv[2], zv[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (n0 + 8 * k < p.N) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (a.bv) bv[k][e] = bf2f(a.bv[n0 + 8 * k + e]);
-            if (a.bg) bg[k][e] = bf2f(a.bg[n0 + 8 * k + e]);
-          }
-        }
-#pragma unroll
-      for (int i = 0; i < Loop::MB; ++i) {
-        const int m = m_w + i * 32 + l31;
+      for (int b = 0; b < 2; ++b) {
         float z[2][4], u[2][4], o[2][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            z[k][e] = T.acc[i][j][8 * q + 4 * k + e] + bg[k][e];
-            u[k][e] = T.acc[i][j + Loop::NB / 2][8 * q + 4 * k + e] + bv[k][e];
+            z[k][e] = T.acc[i][j + b][4 * k + e];
+            u[k][e] = T.acc[i][j + b][8 + 4 * k + e];
             o[k][e] = u[k][e] * act_f(z[k][e], a.act);
           }
-        const bool in = m < p.M && n < p.N;
-        const uint4 ov = trade(o[0], o[1]);
-        if (in) *reinterpret_cast<uint4*>(p.C + (long)m * p.ldc + n) = ov;
-        if (a.hg) {
-          const uint4 uv = trade(u[0], u[1]), zv = trade(z[0], z[1]);
-          bf16_t* r = a.hg + (long)m * a.ld_hg + n;
-          if (in) {
-            *reinterpret_cast<uint4*>(r) = uv;
-            *reinterpret_cast<uint4*>(r + p.N) = zv;
-          }
-        }
+        ov[b] = trade(o[0], o[1]);
+        uv[b] = trade(u[0], u[1]);
+        zv[b] = trade(z[0], z[1]);
+      }
+      store_two(Out{p.C, p.ldc, p.M, p.N}, m, n, lane, ov[0], ov[1]);
+      if (a.hg) {
+        store_two(Out{a.hg, a.ld_hg, p.M, p.N}, m, n, lane, uv[0], uv[1]);
+        store_two(Out{a.hg + p.N, a.ld_hg, p.M, p.N}, m, n, lane, zv[0], zv[1]);
       }
     }
   }
@@ -394,32 +435,32 @@ __device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, int pie
   typedef TileLoop<BM, BN, WR, WC, AK, false, false> Loop;
   Loop T;
   T.run(p, ti * BM, tj * BN, smem, piece);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
-  const int m_w = ti * BM + (wave / WC) * (BM / WR);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < Loop::MB; ++i) {
-    const int m = m_w + i * 32 + l31;
+    const int m0 = ti * BM + (wave / WC) * (BM / WR) + i * 32;
 #pragma unroll
-    for (int j = 0; j < Loop::NB; ++j)
+    for (int j = 0; j < Loop::NB; ++j) {
+      const int n0 = tj * BN + Loop::block(wave % WC, j) * 32;
+      if (p.split > 1) {
+        const int m = m0 + (lane & 31), n = n0 + 4 * (lane >> 5);
+        float* const out = p.part + ((long)piece * p.M + m) * p.N + n;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (m < p.M && n + 8 * k < p.N)
+            *reinterpret_cast<f32x4_t*>(out + 8 * k) = f32x4_t{T.acc[i][j][4 * k], T.acc[i][j][4 * k + 1], T.acc[i][j][4 * k + 2], T.acc[i][j][4 * k + 3]};
+        continue;
+      }
+      uint4 c[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const int n16 = tj * BN + j / (Loop::NB / 2) * (BN / 2) + Loop::col(wave % WC, j) + 16 * q, n = n16 + 8 * h;
-        if (p.split > 1) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int c = n16 + 8 * k + 4 * h;
-            if (m < p.M && c < p.N)
-              *reinterpret_cast<f32x4_t*>(p.part + ((long)piece * p.M + m) * p.N + c) =
-                  f32x4_t{T.acc[i][j][8 * q + 4 * k], T.acc[i][j][8 * q + 4 * k + 1], T.acc[i][j][8 * q + 4 * k + 2], T.acc[i][j][8 * q + 4 * k + 3]};
-          }
-          continue;
-        }
         float v[2][4];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e >> 2][e & 3] = T.acc[i][j][8 * q + e];
-        const uint4 c = trade(v[0], v[1]);
-        if (m < p.M && n < p.N) *reinterpret_cast<uint4*>(p.C + (long)m * p.ldc + n) = c;
+        c[q] = trade(v[0], v[1]);
       }
+      store_two(Out{p.C, p.ldc, p.M, p.N}, m0, n0, lane, c[0], c[1]);
+    }
   }
 }
 
@@ -610,7 +651,8 @@ Layout layout(const Plan& pl, int M, int K, int F, bool dx, bool dwv, bool dwg, 
 extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t stream) {
   if (!q || q->M <= 0 || q->K <= 0 || q->F <= 0 || (q->K % 8) || (q->F % 8)) return AITK_ERR_SHAPE;
   if (!q->x || !q->w_val || !q->w_gate || !q->out || q->act < 0 || q->act > 2) return AITK_ERR_ARG;
-  if (bad(q->x, q->ldx, q->K) || bad(q->w_val, q->ldw, q->K) || mis16(q->w_gate) || bad(q->out, q->ld_out, q->F) || (q->hg && bad(q->hg, q->ld_hg, 2 * (int64_t)q->F)))
+  if (bad(q->x, q->ldx, q->K) || bad(q->w_val, q->ldw, q->K) || mis16(q->w_gate) || bad(q->out, q->ld_out, q->F) || (q->hg && bad(q->hg, q->ld_hg, 2 * (int64_t)q->F)) ||
+      mis16(q->b_val) || mis16(q->b_gate))
     return AITK_ERR_ALIGN;
   FfnArgs a = {};
   a.p[0] = Prod{{q->x, q->x}, {q->w_gate, q->w_val}, q->out, q->ldx, q->ldw, q->ld_out, nullptr, q->M, q->F, q->K, 1, 1, 0};
