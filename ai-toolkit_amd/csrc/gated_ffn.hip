@@ -165,7 +165,7 @@ struct TileLoop {
   typedef Operand<BM, NT, AK, false> OpA;
   typedef Operand<BN, NT, BKC, PAIR> OpB;
   static constexpr int STAGE = OpA::BYTES + OpB::BYTES, DMAS = OpA::NDMA + OpB::NDMA;
-  static_assert(DMAS == 4 && NB % 2 == 0, "the counted waits below; stores of pairs of blocks");
+  static_assert((DMAS == 3 || DMAS == 4) && NB % 2 == 0, "the counted waits below; stores of pairs of blocks");
   f32x16_t acc[MB][NB];
   // a wave's j-th block of 32 columns within the tile: neighbours where a store joins two of them; otherwise one of either half of the tile (4096 x 640 x 2560, both gradients: 83 us
   // with neighbours, 80 us so)
@@ -234,7 +234,7 @@ struct TileLoop {
         __builtin_amdgcn_sched_barrier(0);
         if (i == 0 && more) {
 #pragma unroll
-          for (int k = 0; k < DMAS / 2; ++k) issue(d0 + k);
+          for (int d = d0; d < (d0 ? DMAS : DMAS / 2); ++d) issue(d);
         }
         if (i == 0 && rd) {
 #pragma unroll
@@ -246,9 +246,15 @@ struct TileLoop {
     };
     // a wave's own DMAs are in order: all but the newest n stages' have landed
     auto landed = [&](int n) {
-      if (n >= 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-      else if (n == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (n >= 2) {
+        if constexpr (DMAS == 4) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+      } else if (n == 1) {
+        if constexpr (DMAS == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
     };
     auto barrier = [&]() {
       __builtin_amdgcn_sched_barrier(0);
@@ -288,9 +294,8 @@ struct TileLoop {
   }
 };
 
-// tile order: XCD k works on a contiguous range of tiles, 8 row tiles of a column group at a time, so that its L2 sees few panels
-__device__ __forceinline__ void tile_coords(int id, int ntiles, int tm, int tn, int& m, int& n) {
-  const int l = xcd_remap(id, ntiles);
+// tile order: 8 row tiles of a column group at a time; XCD k works on a contiguous range of l (xcd_remap), so that its L2 sees few panels
+__device__ __forceinline__ void tile_coords(int l, int tm, int tn, int& m, int& n) {
   const int per = 8 * tn, g = l / per, first = g * 8, gm = min(tm - first, 8);
   m = first + (l % per) % gm;
   n = (l % per) / gm;
@@ -323,22 +328,18 @@ __device__ __forceinline__ void store_two(const Out& o, int m0, int n0, int lane
 }
 
 template <int BM, int BN, int WR, int WC>
-__global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+__device__ __forceinline__ void fwd_tile(const FfnArgs& a, int m0, int f0, char* smem) {
   const Prod& p = a.p[0];
-  const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN / 2 - 1) / (BN / 2);
-  int ti, tj;
-  tile_coords(blockIdx.x, tm * tn, tm, tn, ti, tj);
   typedef TileLoop<BM, BN, WR, WC, true, true, true> Loop;
   Loop T;
-  T.run(p, ti * BM, tj * (BN / 2), smem, 0, a.bg, a.bv);
+  T.run(p, m0, f0, smem, 0, a.bg, a.bv);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < Loop::NB; j += 2) {
-    const int n = tj * (BN / 2) + Loop::block(wave % WC, j) * 16;
+    const int n = f0 + Loop::block(wave % WC, j) * 16;
 #pragma unroll
     for (int i = 0; i < Loop::MB; ++i) {
-      const int m = ti * BM + (wave / WC) * (BM / WR) + i * 32;
+      const int m = m0 + (wave / WC) * (BM / WR) + i * 32;
       uint4 ov[2], uv[2], zv[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -361,6 +362,24 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a) 
         store_two(Out{a.hg + p.N, a.ld_hg, p.M, p.N}, m, n, lane, zv[0], zv[1]);
       }
     }
+  }
+}
+
+// The first `whole` workgroups take a tile each, the others half a tile (BM / 2 rows): with one large tile per CU at a time, a last round of at most half as many tiles as CUs runs as
+// twice as many halves.
+template <int BM, int BN, int WR, int WC>
+__global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a, int whole) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tm = (a.p[0].M + BM - 1) / BM, tn = (a.p[0].N + BN / 2 - 1) / (BN / 2), id = blockIdx.x;
+  int ti, tj;
+  if (id < whole) {
+    tile_coords(xcd_remap(id, whole), tm, tn, ti, tj);
+    fwd_tile<BM, BN, WR, WC>(a, ti * BM, tj * (BN / 2), smem);
+  } else if constexpr (BM == 256) {
+    const int l = xcd_remap(id - whole, gridDim.x - whole);
+    tile_coords(whole + (l >> 1), tm, tn, ti, tj);
+    const int m0 = ti * BM + (l & 1) * (BM / 2);
+    if (m0 < a.p[0].M) fwd_tile<BM / 2, BN, WR, WC>(a, m0, tj * (BN / 2), smem);
   }
 }
 
@@ -480,7 +499,7 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_grads_kernel(FfnArgs a
     }
     int ti, tj;
     const int piece = id / n;
-    tile_coords(id - piece * n, n, tm, tn, ti, tj);
+    tile_coords(xcd_remap(id - piece * n, n), tm, tn, ti, tj);
     if (p.a_rows) grad_tile<BM, BN, WR, WC, false>(p, ti, tj, piece, smem);
     else grad_tile<BM, BN, WR, WC, true>(p, ti, tj, piece, smem);
     return;
@@ -576,13 +595,13 @@ __global__ __launch_bounds__(256) void gated_ffn_db_kernel(const float* part, in
 bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
 bool bad(const void* p, int64_t ld, int64_t width) { return mis16(p) || (ld % 8) || ld < width || ld > (1 << 20); }
 
-template <typename K>
-int launch(K kernel, unsigned grid, unsigned threads, size_t lds, const FfnArgs& a, hipStream_t s) {
+template <typename K, typename... More>
+int launch(K kernel, unsigned grid, unsigned threads, size_t lds, hipStream_t s, const FfnArgs& a, More... more) {
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, s, a);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, s, a, more...);
   AITK_LAUNCH_CHECK();
   return AITK_OK;
 }
@@ -668,14 +687,16 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   // up to 32 rows the weights' way bounds both forms: 4096 x 10240 16 rows 36 us against 48 us of the small tiles, 32 rows 45 against 48, 512 x 1024 3.8 / 4.5 against 11 us.  Up to 64
   // rows the waves read x more often than W: 64 rows 69 us against 48 for 4096 x 10240 (168 MB), but 8.5 against 16.5 for 1024 x 2816 (12 MB): there the tiles' start-up decides.
   if (q->M <= 32 || (q->M <= 64 && (int64_t)q->F * q->K <= (8 << 20))) {
-    if (q->M <= 16) return launch(gated_ffn_few_kernel<1>, strips, 512, 0, a, s);
-    if (q->M <= 32) return launch(gated_ffn_few_kernel<2>, strips, 512, 0, a, s);
-    return launch(gated_ffn_few_kernel<4>, strips, 512, 0, a, s);
+    if (q->M <= 16) return launch(gated_ffn_few_kernel<1>, strips, 512, 0, s, a);
+    if (q->M <= 32) return launch(gated_ffn_few_kernel<2>, strips, 512, 0, s, a);
+    return launch(gated_ffn_few_kernel<4>, strips, 512, 0, s, a);
   }
-  // A round of small tiles (two workgroups per CU) takes 0.55 to 0.75 of a round of large ones: 512 x 4096 x 10240 (1 round against 2) 113 us large, 137 us small;
-  // 4096 x 640 x 2560 (2 against 3) 57.8 and 49.2; 2048 x 2048 x 5120 (2 against 3) 121.5 and 119.8; 256 x 4096 x 10240 (1 against 1) 92 and 74; 2048 x 4096 x 10240 (3 against 5) 366 and 450.
-  if (20 * ((big + 255) / 256) <= 13 * ((small + 511) / 512)) return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)big, 512, NST * 512 * BK * 2, a, s);
-  return launch(gated_ffn_fwd_kernel<128, 128, 2, 2>, (unsigned)small, 256, NST * 256 * BK * 2, a, s);
+  // Large tiles (one workgroup per CU), the last round in halves if they all find a CU; 128 x 128 tiles (two workgroups per CU) only while every one of them has a CU to itself.  Large
+  // with halves / large / small, us: 4096 x 640 x 2560 (320 tiles) 44 / 50 / 50; 2048 x 4096 x 10240 (640) 301 / 316 / 397; 512 x 4096 x 10240 (160) 92 / 92 / 120; 1024 x 640 x 2560
+  // (80 large, 320 small) 17.2 / 24 / 17.7; 1000 x 768 x 2048 (64, 256) 17.6 / 25 / 16.1; 77 x 4096 x 10240 (80, 160) 58 / 84 / 48.
+  if (small <= 256) return launch(gated_ffn_fwd_kernel<128, 128, 2, 2>, (unsigned)small, 256, NST * 256 * BK * 2, s, a, (int)small);
+  const int64_t rest = big % 256, halves = rest <= 128 ? rest : 0;
+  return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)(big + halves), 512, NST * 512 * BK * 2, s, a, (int)(big - halves));
 }
 
 extern "C" int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t K, int32_t F, int32_t dx, int32_t dw_val, int32_t dw_gate, int32_t bias_grads) {
@@ -724,8 +745,8 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
   }
   if (!n) return AITK_OK;
   if (n > 0x7fffffff) return AITK_ERR_SHAPE;
-  const int rc = pl.big ? launch(gated_ffn_grads_kernel<256, 256, 2, 4>, (unsigned)n, 512, NST * 512 * BK * 2, a, s)
-                        : launch(gated_ffn_grads_kernel<128, 128, 2, 2>, (unsigned)n, 256, NST * 256 * BK * 2, a, s);
+  const int rc = pl.big ? launch(gated_ffn_grads_kernel<256, 256, 2, 4>, (unsigned)n, 512, NST * 512 * BK * 2, s, a)
+                        : launch(gated_ffn_grads_kernel<128, 128, 2, 2>, (unsigned)n, 256, NST * 256 * BK * 2, s, a);
   if (rc != AITK_OK || !joined) return rc;
   const int64_t blocks = (joined / 8 + 255) / 256;
   hipLaunchKernelGGL(gated_ffn_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048), 3), dim3(256), 0, s, a);

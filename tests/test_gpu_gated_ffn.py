@@ -112,7 +112,8 @@ def test_sizes(M, K, F):
     _case(M, K, F, seed=M)
 
 
-@pytest.mark.parametrize("M,K,F", [(2048, 512, 4096), (4096, 640, 2560), (2300, 328, 4104), (600, 1000, 10240)])
+# the last three: a last round of half tiles, some of them with a few rows or none
+@pytest.mark.parametrize("M,K,F", [(2048, 512, 4096), (4096, 640, 2560), (600, 1000, 10240), (2300, 328, 4104), (2100, 136, 4104), (900, 72, 2560)])
 @pytest.mark.parametrize("act", ["gelu_tanh", "gelu", "silu"])
 def test_large_tiles(M, K, F, act):
     _case(M, K, F, act=act, bias=act == "gelu")
