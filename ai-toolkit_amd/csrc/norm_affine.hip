@@ -33,12 +33,30 @@ __device__ __forceinline__ void load_w8(const void* w, int f32, int c, float* f)
   }
 }
 
-// sum over the LPR lanes of a row; rows of more than one wave meet in `slot` (one float per wave of the workgroup), which the caller alternates so that one
+// v plus the value of the lane that DPP control `CTRL` names
+template <int CTRL>
+__device__ __forceinline__ float plus_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// v plus the value of the neighbouring row of 16 lanes (of the other half of the wave)
+template <int ROWS>
+__device__ __forceinline__ float plus_swapped(float v) {
+  typedef unsigned u2_t __attribute__((ext_vector_type(2)));
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  const u2_t s = ROWS == 16 ? __builtin_amdgcn_permlane16_swap(a, a, false, false) : __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const unsigned lo = s[0], hi = s[1];  // __builtin_bit_cast of a vector's element takes element 0
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+// sum over the LPR lanes of a row, in every one of them: neighbours, pairs, quads (mirrored halves of 8), eights (mirrored 16), then the two swaps between rows of lanes; rows of more than one wave meet in `slot` (one float per wave of the workgroup), which the caller alternates so that one
 // barrier per sum is enough.  Every lane of the workgroup calls it the same number of times.
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v, float* slot) {
-#pragma unroll
-  for (int o = (LPR > 64 ? 64 : LPR) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = plus_dpp<0xB1>(v);
+  v = plus_dpp<0x4E>(v);
+  v = plus_dpp<0x141>(v);
+  v = plus_dpp<0x140>(v);
+  if constexpr (LPR >= 32) v = plus_swapped<16>(v);
+  if constexpr (LPR >= 64) v = plus_swapped<32>(v);
   if constexpr (LPR > 64) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) slot[wave] = v;
@@ -113,14 +131,14 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(AitkNormArgs p) {
   }
 }
 
-// Backward.  A workgroup of 512 threads walks its rows with the next row's x and dy in flight; each thread owns fixed columns and sums dy xh and dy over its rows in
-// registers; the column sums of all its rows leave the workgroup as ONE row of partials (one workgroup per CU above 2048 columns, two below).
-#define NB_THREADS 512
+// Backward.  A workgroup walks its rows with the next row's x and dy in flight; each thread owns fixed columns and sums dy xh and dy over its rows in registers; the column
+// sums of all its rows leave the workgroup as ONE row of partials.  A CU's registers hold 16 waves with 2 vectors per lane (two workgroups of 512 threads), 12 with 3 (one of 768), 8 with
+// 4 (one of 512): see bwd_form().
 #define NB_SLOTS(LPR) ((LPR) == 256 ? 1 : 4)  // column sums of so many row groups meet in LDS at a time (at most 32 KiB)
-template <int LPR, int NV, bool RMS, bool GRADS>
-__global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p) {
-  constexpr int RPW = NB_THREADS / LPR;
-  __shared__ float red[2][2][NB_THREADS / 64];
+template <int TH, int LPR, int NV, bool RMS, bool GRADS>
+__global__ __launch_bounds__(TH) void norm_bwd_kernel(AitkNormBwdArgs p) {
+  constexpr int RPW = TH / LPR;
+  __shared__ float red[2][2][TH / 64];
   extern __shared__ __attribute__((aligned(16))) float colsum[];  // [SLOTS][C] when GRADS
   const int t = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   const float inv_c = 1.0f / (float)p.C;
@@ -145,7 +163,7 @@ __global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p)
     const long m = base + grp;
     const bool live = m < p.M;
     const long mr = live ? m : 0;
-    const float mean = RMS ? 0.f : p.mean[mr], rstd = p.rstd[mr];
+    const float rstd = p.rstd[mr], shift = RMS ? 0.f : -p.mean[mr] * rstd;  // xh = x rstd + shift
     uint4 xn[NV], gn[NV], rv[NV];
     if (base + step < p.M) fetch(m + step, xn, gn);
     if (p.dres) {
@@ -166,7 +184,7 @@ __global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p)
         load_w8(p.weight, p.w_f32, c, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float xh = (x[e] - mean) * rstd, gw = g[e] * w[e];
+          const float xh = fmaf(x[e], rstd, shift), gw = g[e] * w[e];
           s1 += gw;
           s2 = fmaf(gw, xh, s2);
           if (GRADS && live) {
@@ -178,6 +196,7 @@ __global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p)
     }
     const float c1 = RMS ? 0.f : row_sum<LPR>(s1, red[par][0]) * inv_c;
     const float c2 = row_sum<LPR>(s2, red[par][1]) * inv_c;
+    const float kx = -rstd * rstd * c2, k0 = -rstd * fmaf(shift, c2, c1);  // rstd (g w - c1 - xh c2) = rstd g w + kx x + k0
     if (live) {
       bf16_t* dr = p.dx + m * p.ld_dx;
 #pragma unroll
@@ -190,10 +209,7 @@ __global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p)
           if (p.dres) up8(rv[i], r);
           load_w8(p.weight, p.w_f32, c, w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float xh = (x[e] - mean) * rstd;
-            r[e] = fmaf(rstd, g[e] * w[e] - c1 - xh * c2, r[e]);
-          }
+          for (int e = 0; e < 8; ++e) r[e] += fmaf(g[e] * w[e], rstd, fmaf(x[e], kx, k0));
           *reinterpret_cast<uint4*>(dr + c) = dn8(r);
         }
       }
@@ -217,7 +233,7 @@ __global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p)
           }
     }
     // the row groups of the workgroup meet in LDS in a fixed order, one vector after the other
-    constexpr int G = LPR < 64 ? NB_THREADS / 64 : RPW, SLOTS = NB_SLOTS(LPR);
+    constexpr int G = LPR < 64 ? TH / 64 : RPW, SLOTS = NB_SLOTS(LPR);
     const int g = LPR < 64 ? threadIdx.x >> 6 : grp;
     const bool holds = LPR >= 64 || (threadIdx.x & 63) < LPR;
     for (int v = 0; v < (RMS ? 1 : 2); ++v) {
@@ -240,7 +256,7 @@ __global__ __launch_bounds__(NB_THREADS) void norm_bwd_kernel(AitkNormBwdArgs p)
       }
       __syncthreads();
       float* out = p.partial + ((long)blockIdx.x * (RMS ? 1 : 2) + v) * p.C;
-      for (int c = threadIdx.x; c < p.C; c += NB_THREADS) {
+      for (int c = threadIdx.x; c < p.C; c += TH) {
         float a = colsum[c];
         for (int k = 1; k < SLOTS; ++k) a += colsum[k * p.C + c];
         out[c] = a;
@@ -277,11 +293,23 @@ __global__ __launch_bounds__(256) void norm_wgrad_finish_kernel(const float* par
 
 bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
 
+// form of the backward: threads and lanes per row, and the workgroups that the CUs hold at a time
+struct BwdForm {
+  int threads, lanes, most;
+};
+BwdForm bwd_form(int C) {
+  if (C <= 256) return {512, 16, 512};
+  if (C <= 512) return {512, 32, 512};
+  if (C <= 768) return {768, 32, 256};
+  if (C <= 1024) return {512, 64, 512};
+  if (C <= 1536) return {768, 64, 256};
+  if (C <= 2048) return {512, 64, 256};
+  return {512, 256, 256};
+}
 int bwd_grid(int M, int C) {
-  const int rpw = C <= 512 ? NB_THREADS / 16 : C <= 2048 ? NB_THREADS / 64 : NB_THREADS / 256;
-  const int n = (M + rpw - 1) / rpw;
-  const int most = C <= 2048 ? 512 : 256;
-  return n < most ? n : most;
+  const BwdForm f = bwd_form(C);
+  const int rpw = f.threads / f.lanes, n = M / rpw + (M % rpw != 0);
+  return n < f.most ? n : f.most;
 }
 
 template <int LPR, int NV>
@@ -291,17 +319,18 @@ void launch_fwd(const AitkNormArgs& a, hipStream_t s) {
   if (a.rms) hipLaunchKernelGGL((norm_fwd_kernel<LPR, NV, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((norm_fwd_kernel<LPR, NV, false>), grid, dim3(256), 0, s, a);
 }
-template <int LPR, int NV>
+template <int TH, int LPR, int NV>
 void launch_bwd(const AitkNormBwdArgs& a, hipStream_t s) {
-  const bool grads = a.dweight || a.dbias;
   const dim3 grid(bwd_grid(a.M, a.C));
-  const size_t lds = grads ? (size_t)NB_SLOTS(LPR) * a.C * 4 : 0;
-  if (a.rms) {
-    if (grads) hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, true, true>), grid, dim3(NB_THREADS), lds, s, a);
-    else hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, true, false>), grid, dim3(NB_THREADS), lds, s, a);
-  } else {
-    if (grads) hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, false, true>), grid, dim3(NB_THREADS), lds, s, a);
-    else hipLaunchKernelGGL((norm_bwd_kernel<LPR, NV, false, false>), grid, dim3(NB_THREADS), lds, s, a);
+  if (a.dweight || a.dbias) {
+    const size_t lds = (size_t)NB_SLOTS(LPR) * a.C * 4;
+    if (a.rms) hipLaunchKernelGGL((norm_bwd_kernel<TH, LPR, NV, true, true>), grid, dim3(TH), lds, s, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<TH, LPR, NV, false, true>), grid, dim3(TH), lds, s, a);
+  } else {  // without the sums' registers
+    const int n = a.M / (512 / LPR) + (a.M % (512 / LPR) != 0);
+    const dim3 wide(n < 512 ? n : 512);
+    if (a.rms) hipLaunchKernelGGL((norm_bwd_kernel<512, LPR, NV, true, false>), wide, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<512, LPR, NV, false, false>), wide, dim3(512), 0, s, a);
   }
 }
 }  // namespace
@@ -338,14 +367,15 @@ extern "C" int aitk_norm_bwd(const AitkNormBwdArgs* a, aitk_stream_t stream) {
     return AITK_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   const int C = a->C;
-  if (C <= 128) launch_bwd<16, 1>(*a, s);
-  else if (C <= 256) launch_bwd<16, 2>(*a, s);
-  else if (C <= 512) launch_bwd<16, 4>(*a, s);
-  else if (C <= 1024) launch_bwd<64, 2>(*a, s);
-  else if (C <= 1536) launch_bwd<64, 3>(*a, s);
-  else if (C <= 2048) launch_bwd<64, 4>(*a, s);
-  else if (C <= 4096) launch_bwd<256, 2>(*a, s);
-  else launch_bwd<256, 4>(*a, s);
+  if (C <= 128) launch_bwd<512, 16, 1>(*a, s);
+  else if (C <= 256) launch_bwd<512, 16, 2>(*a, s);
+  else if (C <= 512) launch_bwd<512, 32, 2>(*a, s);
+  else if (C <= 768) launch_bwd<768, 32, 3>(*a, s);
+  else if (C <= 1024) launch_bwd<512, 64, 2>(*a, s);
+  else if (C <= 1536) launch_bwd<768, 64, 3>(*a, s);
+  else if (C <= 2048) launch_bwd<512, 64, 4>(*a, s);
+  else if (C <= 4096) launch_bwd<512, 256, 2>(*a, s);
+  else launch_bwd<512, 256, 4>(*a, s);
   AITK_LAUNCH_CHECK();
   if (grads) {
     const int V = a->rms ? 1 : 2;
