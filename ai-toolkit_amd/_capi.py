@@ -334,4 +334,4 @@ def stream_ptr():
     """the current stream's handle, without the Stream object: 1 us of a small call's 10"""
     import torch
 
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))

@@ -1211,11 +1211,9 @@ def _rows(t, name, shape):
         ld, inner = t.stride()
         p = t.data_ptr()
         rows, cols = shape
-        if rows <= 1 or cols <= 1:  # a stride that nothing steps over is nobody's
-            if rows <= 1:
-                ld = (cols + 7) & -8
-            inner = 1 if cols <= 1 else inner
-        if inner == 1 and ld >= cols and not ld & 7 and not p & 15:
+        if rows <= 1:  # a stride that nothing steps over is nobody's
+            ld = (cols + 7) & -8
+        if (inner == 1 or cols <= 1) and ld >= cols and not ld & 7 and not p & 15:
             return p, ld
     if t.dtype != BF16:
         raise ValueError(f"{name}: expected bf16, got {t.dtype}")
@@ -1237,15 +1235,11 @@ def _vec(t, name, n, dtypes):
 
 def _on_device(names, tensors):
     """every operand lives on the current GPU (the launch goes to its current stream), and as long as a launch list that is being recorded"""
-    dev = None
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None:
-            d = t.get_device()
-            if dev is None:
-                dev = d
-            if d < 0 or d != dev:
-                raise ValueError(f"{names}: expected tensors of one GPU, got {[str(t.device) for t in tensors if t is not None]}")
-    if dev != torch.cuda.current_device():
+        if t is not None and t.get_device() != dev or dev < 0:
+            raise ValueError(f"{names}: expected tensors of one GPU, got {[str(t.device) for t in tensors if t is not None]}")
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"{names} are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     if _REC is not None:
         _REC.append(("_keepalive", tensors))
@@ -1259,9 +1253,10 @@ def _scratch(nbytes, like):
 
 
 def _norm_shape(x):
-    if x.dim() != 2 or x.shape[1] <= 0 or x.shape[1] % 8 or x.shape[1] > 8192:
-        raise ValueError(f"x: expected [M, C] with C a multiple of 8 up to 8192, got {tuple(x.shape)}")
-    return x.shape
+    shape = x.shape
+    if len(shape) != 2 or not 0 < shape[1] <= 8192 or shape[1] % 8:
+        raise ValueError(f"x: expected [M, C] with C a multiple of 8 up to 8192, got {tuple(shape)}")
+    return shape
 
 
 def _norm_stat(t, name, M):
@@ -1397,17 +1392,18 @@ GATED_ACTS = {"gelu_tanh": 0, "gelu": 1, "silu": 2}
 def _ffn_check(x, w_val, w_gate, act):
     if act not in GATED_ACTS:
         raise ValueError(f"act: expected one of {sorted(GATED_ACTS)}, got {act!r}")
-    if x.dim() != 2 or w_val.dim() != 2 or x.shape[1] != w_val.shape[1]:
-        raise ValueError(f"x [M, K] and w_val [F, K] do not match: {tuple(x.shape)}, {tuple(w_val.shape)}")
-    M, K = x.shape
-    F = w_val.shape[0]
+    xs, ws = x.shape, w_val.shape
+    if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[1]:
+        raise ValueError(f"x [M, K] and w_val [F, K] do not match: {tuple(xs)}, {tuple(ws)}")
+    M, K = xs
+    F = ws[0]
     if K <= 0 or F <= 0 or K % 8 or F % 8 or 2 * F > 1 << 20:
         raise ValueError(f"K and F must be positive multiples of 8 (2 F up to 2^20), got K = {K}, F = {F}")
-    pv, ldw = _rows(w_val, "w_val", (F, K))
-    pg, ldg = _rows(w_gate, "w_gate", (F, K))
+    pv, ldw = _rows(w_val, "w_val", ws)
+    pg, ldg = _rows(w_gate, "w_gate", ws)
     if ldg != ldw:
         raise ValueError(f"w_val and w_gate must share one row pitch, got {ldw} and {ldg}")
-    px, ldx = _rows(x, "x", (M, K))
+    px, ldx = _rows(x, "x", xs)
     return M, K, F, px, ldx, pv, pg, ldw
 
 
