@@ -31,7 +31,8 @@ constexpr float DEFER = 8.0f;       // the accumulators are rescaled only when a
 
 struct RelposArgs {
   AitkAttnRelposArgs a;
-  int half, sat, line_p, _pad;  // buckets per sign, first distance of the last one, floats per shifted copy of the line
+  int half, sat, line_p;        // buckets per sign, first distance of the last one, floats per shifted copy of the line
+  int tiles;                    // backward: row tiles of a workgroup's height
   int first[MAX_HALF];          // first distance of every bucket of one sign
   float* delta;                 // backward: [2][B][H][S]: dO.o, and -lse (-inf for rows without a key)
   float* part;                  // backward: [B * row tiles][H][num_buckets] bucket sums
@@ -179,6 +180,27 @@ __device__ __forceinline__ unsigned long long lane64(unsigned long long m, int t
   const unsigned lo = __builtin_amdgcn_readlane((unsigned)m, t), hi = __builtin_amdgcn_readlane((unsigned)(m >> 32), t);
   return (unsigned long long)hi << 32 | lo;
 }
+// The next KVS tiles of two operands (A, B) that `todo` names into one stage of KVS x (A tile, B tile); wave part `part`'s own tile and its keep-bits (0: nothing for it in this step).
+template <int KVS>
+__device__ __forceinline__ void fetch(lds_char* dst, const TileLane& L, long lda, const v4i_t& srdA, long ldb, const v4i_t& srdB, int wave, int part, int t0, unsigned long long masks,
+                                      unsigned long long& todo, int& mine, unsigned long long& keep) {
+  mine = 0;
+  keep = 0;
+#pragma unroll
+  for (int i = 0; i < KVS; ++i) {
+    if (todo) {
+      const int t = __builtin_ctzll(todo);
+      const unsigned long long k = lane64(masks, t);
+      stage(dst + 2 * i * TILE, L, lda, (t0 + t) * 64, srdA, wave, k);
+      stage(dst + (2 * i + 1) * TILE, L, ldb, (t0 + t) * 64, srdB, wave, k);
+      if (KVS == 1 || part == i) {
+        mine = t;
+        keep = k;
+      }
+      todo &= todo - 1;
+    }
+  }
+}
 // workgroup -> (row tile, head, sample): the tiles of one (head, sample) stay on one XCD, whose L2 then holds their slices (block i runs on XCD i % 8), and an XCD gets all the
 // samples of its heads: with a key mask the samples differ in length, and whole samples per XCD left the XCDs of the
 // short ones idle (4 x 64 heads x 512 with lengths 24 .. 512: backward 126 -> 105 us, forward 37 -> 32 us)
@@ -229,29 +251,10 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
   for (int t0 = 0; t0 < ntiles; t0 += 64) {
     const unsigned long long masks = tile_masks(a, b, t0, ntiles, box, lane, wave);
     unsigned long long todo = __ballot(masks != 0);
-    // the next KVS tiles of the group into one stage; this wave's own tile and its keep-bits (0: nothing for it in this step)
-    auto fetch = [&](lds_char* dst, int& mine, unsigned long long& keep) {
-      mine = 0;
-      keep = 0;
-#pragma unroll
-      for (int i = 0; i < KVS; ++i) {
-        if (todo) {
-          const int t = __builtin_ctzll(todo);
-          const unsigned long long k = lane64(masks, t);
-          stage(dst + 2 * i * TILE, L, a.ldk, (t0 + t) * 64, srdK, wave, k);
-          stage(dst + (2 * i + 1) * TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, k);
-          if (KVS == 1 || part == i) {
-            mine = t;
-            keep = k;
-          }
-          todo &= todo - 1;
-        }
-      }
-    };
     int t, cur = 0;
     unsigned long long keep;
     bool more = todo != 0;
-    if (more) fetch(sm, t, keep);
+    if (more) fetch<KVS>(sm, L, a.ldk, srdK, a.ldv, srdV, wave, part, t0, masks, todo, t, keep);
     if (BIAS && t0 == 0) {  // with the first tiles on their way
       build_line(line, r, hd, 1);
     }
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
       more = todo != 0;
       int tn = 0;
       unsigned long long keep_n = 0;
-      if (more) fetch(sm + (cur ^ 1) * STEP, tn, keep_n);
+      if (more) fetch<KVS>(sm + (cur ^ 1) * STEP, L, a.ldk, srdK, a.ldv, srdV, wave, part, t0, masks, todo, tn, keep_n);
       const lds_char* kt = sm + cur * STEP + part * 2 * TILE;
       const lds_char* vt = kt + TILE;
       const int kv0 = (t0 + t) * 64;
@@ -400,16 +403,18 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
   }
 }
 
-// dQ (and the bucket sums of ds): 4 waves x 32 query rows over the key tiles
-template <bool BIAS, bool CAUSAL>
+// dQ (and the bucket sums of ds): 4 waves over the key tiles, 32 query rows each (KVS = 1) or two waves to 32 rows, every other tile each (KVS = 2), as in the forward
+template <bool BIAS, bool CAUSAL, int KVS>
 __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int tile_x, int hd, int b) {
   const AitkAttnRelposArgs& a = r.a;
+  constexpr int ROWS = 128 / KVS, STEP = 2 * KVS * TILE;
   lds_char* const sm = (lds_char*)smem;
-  unsigned long long* const box = reinterpret_cast<unsigned long long*>(smem + 4 * TILE);
-  lds_float* const line = (lds_float*)(smem + 4 * TILE + 512);
+  unsigned long long* const box = reinterpret_cast<unsigned long long*>(smem + 2 * STEP);
+  lds_float* const line = (lds_float*)(smem + 2 * STEP + 512);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5, S = a.S;
-  const int q0 = tile_x * 128 + wave * 32;
+  const int qg = wave / KVS, part = wave % KVS;
+  const int q0 = tile_x * ROWS + qg * 32;
   const v4i_t srdK = make_srd(a.K + (long)b * S * a.ldk + hd * 64, ((long)(S - 1) * a.ldk + 64) * 2);
   const v4i_t srdV = make_srd(a.V + (long)b * S * a.ldv + hd * 64, ((long)(S - 1) * a.ldv + 64) * 2);
   TileLane L;
@@ -444,16 +449,14 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f, fp_past = 0.f, fp_ahead = 0.f, row_ds = 0.f;
   const int ib = E + 4 * h - q0 - l31;
   f32x16_t dq[2] = {zero16(), zero16()};
-  const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * 128 + 127) / 64 + 1) : (S + 63) / 64;
+  const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * ROWS + ROWS - 1) / 64 + 1) : (S + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += 64) {
     const unsigned long long masks = tile_masks(a, b, t0, ntiles, box, lane, wave);
     unsigned long long todo = __ballot(masks != 0);
-    int t = todo ? __builtin_ctzll(todo) : 0, cur = 0;
-    unsigned long long keep = lane64(masks, t);
-    if (todo) {
-      stage(sm, L, a.ldk, (t0 + t) * 64, srdK, wave, keep);
-      stage(sm + TILE, L, a.ldv, (t0 + t) * 64, srdV, wave, keep);
-    }
+    int t = 0, cur = 0;
+    unsigned long long keep = 0;
+    bool more = todo != 0;
+    if (more) fetch<KVS>(sm, L, a.ldk, srdK, a.ldv, srdV, wave, part, t0, masks, todo, t, keep);
     if (BIAS && t0 == 0) {  // with the first tiles on their way
       build_line(line, r, hd, 1);
       if (sums)
@@ -465,19 +468,15 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       far_past = line[E - r.sat] * c2;
       far_ahead = line[E + r.sat] * c2;
     }
-    while (todo) {
-      todo &= todo - 1;
-      const int tn = todo ? __builtin_ctzll(todo) : 0;
-      const unsigned long long keep_n = lane64(masks, tn);
-      if (todo) {
-        lds_char* nx = sm + (cur ^ 1) * 2 * TILE;
-        stage(nx, L, a.ldk, (t0 + tn) * 64, srdK, wave, keep_n);
-        stage(nx + TILE, L, a.ldv, (t0 + tn) * 64, srdV, wave, keep_n);
-      }
-      const lds_char* kt = sm + cur * 2 * TILE;
+    while (more) {
+      more = todo != 0;
+      int tn = 0;
+      unsigned long long keep_n = 0;
+      if (more) fetch<KVS>(sm + (cur ^ 1) * STEP, L, a.ldk, srdK, a.ldv, srdV, wave, part, t0, masks, todo, tn, keep_n);
+      const lds_char* kt = sm + cur * STEP + part * 2 * TILE;
       const lds_char* vt = kt + TILE;
       const int kv0 = (t0 + t) * 64;
-      if (!CAUSAL || kv0 <= q0 + 31) {
+      if ((KVS == 1 || keep) && (!CAUSAL || kv0 <= q0 + 31)) {
         float tb = 0.f;
         int side = 0;  // 0: the band, 1: past, 2: ahead
         if constexpr (BIAS) {
@@ -560,9 +559,38 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       cur ^= 1;
     }
   }
-  store_row(a.dQ + ((long)b * S + qc) * a.lddq + hd * 64, dq, a.scale, h, live);
+  if constexpr (KVS == 2) {
+    lds_float* const mine = (lds_float*)smem + qg * (37 * 64) + lane;  // the tiles are done with: every loop ends behind a barrier
+    if (part) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        mine[e * 64] = dq[0][e];
+        mine[(16 + e) * 64] = dq[1][e];
+      }
+      mine[32 * 64] = row_ds;
+      mine[33 * 64] = fs_past;
+      mine[34 * 64] = fs_ahead;
+      mine[35 * 64] = fp_past;
+      mine[36 * 64] = fp_ahead;
+      fs_past = fs_ahead = fp_past = fp_ahead = 0.f;
+    }
+    __syncthreads();
+    if (!part) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        dq[0][e] += mine[e * 64];
+        dq[1][e] += mine[(16 + e) * 64];
+      }
+      row_ds += mine[32 * 64];
+      fs_past += mine[33 * 64];
+      fs_ahead += mine[34 * 64];
+      fp_past += mine[35 * 64];
+      fp_ahead += mine[36 * 64];
+    }
+  }
+  if (KVS == 1 || !part) store_row(a.dQ + ((long)b * S + qc) * a.lddq + hd * 64, dq, a.scale, h, live);
   if (sums) {
-    lds_float* const fars = (lds_float*)smem;  // the tiles are done with (the loop ends behind a barrier; so does the set-up when no tile was visited)
+    lds_float* const fars = (lds_float*)box;  // the tile masks are done with
     row_ds += __shfl_xor(row_ds, 32, 64);  // the row's two lanes
     fs_past = wave_sum(fs_past - row_ds * fp_past);
     fs_ahead = wave_sum(fs_ahead - row_ds * fp_ahead);
@@ -587,27 +615,28 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       for (int o = 4; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
       const int f = ahead ? 4 : 0;
       if (last) v += (fars[f] + fars[f + 1]) + (fars[f + 2] + fars[f + 3]);
-      if ((i & 7) == 0) r.part[(((long)b * ((S + 127) / 128) + tile_x) * a.H + hd) * a.num_buckets + bucket] = v;
+      if ((i & 7) == 0) r.part[(((long)b * r.tiles + tile_x) * a.H + hd) * a.num_buckets + bucket] = v;
     }
   }
 }
 
-// dK and dV: 4 waves x 32 keys over the query tiles.  S = Q K^T: a lane owns one key (column), its registers hold query rows, so the line of the bias runs backwards and
+// dK and dV: 4 waves over the query tiles, 32 keys each (KVS = 2: two waves to 32 keys).  S = Q K^T: a lane owns one key (column), its registers hold query rows, so the line of the bias runs backwards and
 // the row statistics come from LDS.  What a masked key computes stays in its own lane, which writes zeros.
-template <bool BIAS, bool CAUSAL>
+template <bool BIAS, bool CAUSAL, int KVS>
 __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int tile_x, int hd, int b) {
   const AitkAttnRelposArgs& a = r.a;
-  lds_char* const sm = (lds_char*)smem;                        // 2 x (Q tile, dO tile)
-  lds_float* const st = (lds_float*)(smem + 4 * TILE);         // 2 x (64 -lse, 64 delta)
-  lds_float* const line = (lds_float*)(smem + 4 * TILE + 1024);
+  constexpr int ROWS = 128 / KVS, STEP = 2 * KVS * TILE;
+  lds_char* const sm = (lds_char*)smem;                                // 2 x KVS x (Q tile, dO tile)
+  lds_float* const st = (lds_float*)(smem + 2 * STEP);                 // 2 x KVS x (64 -lse, 64 delta)
+  lds_float* const line = (lds_float*)(smem + 2 * STEP + KVS * 1024);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5, S = a.S;
-  const int k0 = tile_x * 128 + wave * 32;
+  const int part = wave % KVS, k0 = tile_x * ROWS + wave / KVS * 32;
   const int key = k0 + l31;
   const bool inside = key < S;
   const bool kept = inside && (!a.key_mask || a.key_mask[(long)b * S + (inside ? key : 0)] != 0);
   f32x16_t dk[2] = {zero16(), zero16()}, dv[2] = {zero16(), zero16()};
-  const int ntiles = (S + 63) / 64, first_tile = CAUSAL ? tile_x * 2 : 0;
+  const int ntiles = (S + 63) / 64, first_tile = CAUSAL ? tile_x * (ROWS / 64) : 0;
   if (__syncthreads_or(kept)) {  // a block of keys that are all masked has zero gradients
     const v4i_t srdQ = make_srd(a.Q + (long)b * S * a.ldq + hd * 64, ((long)(S - 1) * a.ldq + 64) * 2);
     const v4i_t srdG = make_srd(a.dO + (long)b * S * a.lddo + hd * 64, ((long)(S - 1) * a.lddo + 64) * 2);
@@ -632,10 +661,15 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
     float far_past = 0.f, far_ahead = 0.f;  // not in the log2 domain here: start values like the line's
     // rows past the end arrive as zeros: dO = 0 and delta = 0, so they add nothing to either gradient
     auto stage_all = [&](int t, int buf) {
-      stage(sm + buf * 2 * TILE, L, a.ldq, t * 64, srdQ, wave, ~0ull);
-      stage(sm + buf * 2 * TILE + TILE, L, a.lddo, t * 64, srdG, wave, ~0ull);
-      if (wave < 2)
-        dma4(__builtin_amdgcn_readfirstlane((unsigned)(size_t)(st + buf * 128 + wave * 64)), (unsigned)((t * 64 + lane) * 4), wave ? srdD : srdL);
+#pragma unroll
+      for (int i = 0; i < KVS; ++i) {
+        if (i && t + i >= ntiles) break;
+        lds_char* const dst = sm + buf * STEP + i * 2 * TILE;
+        stage(dst, L, a.ldq, (t + i) * 64, srdQ, wave, ~0ull);
+        stage(dst + TILE, L, a.lddo, (t + i) * 64, srdG, wave, ~0ull);
+        if (wave < 2)
+          dma4(__builtin_amdgcn_readfirstlane((unsigned)(size_t)(st + (buf * KVS + i) * 128 + wave * 64)), (unsigned)(((t + i) * 64 + lane) * 4), wave ? srdD : srdL);
+      }
     };
     stage_all(first_tile, 0);
     if (BIAS) build_line(line, r, hd, -1);
@@ -645,54 +679,82 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
       far_past = line[E + r.sat];
       far_ahead = line[E - r.sat];
     }
-    for (int t = first_tile, cur = 0; t < ntiles; ++t, cur ^= 1) {
-      if (t + 1 < ntiles) stage_all(t + 1, cur ^ 1);
-      const lds_char* qt = sm + cur * 2 * TILE;
+    for (int t = first_tile, cur = 0; t < ntiles; t += KVS, cur ^= 1) {
+      if (t + KVS < ntiles) stage_all(t + KVS, cur ^ 1);
+      const lds_char* qt = sm + cur * STEP + part * 2 * TILE;
       const lds_char* gt = qt + TILE;
-      const int qt0 = t * 64;
-      const bool past = BIAS && k0 + 31 - qt0 <= -r.sat, ahead = BIAS && k0 - qt0 - 63 >= r.sat;
-      const float far = past ? far_past : ahead ? far_ahead : 0.f;
+      const lds_float* const row = st + (cur * KVS + part) * 128;
+      const int qt0 = (t + part) * 64;
+      if (KVS == 1 || t + part < ntiles) {
+        const bool past = BIAS && k0 + 31 - qt0 <= -r.sat, ahead = BIAS && k0 - qt0 - 63 >= r.sat;
+        const float far = past ? far_past : ahead ? far_ahead : 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f32x16_t s, dp = zero16();
-        if (BIAS && !past && !ahead) {
-          s = load_line(line, r.line_p, ib + qt0 + 32 * j);
-        } else {
+        for (int j = 0; j < 2; ++j) {
+          f32x16_t s, dp = zero16();
+          if (BIAS && !past && !ahead) {
+            s = load_line(line, r.line_p, ib + qt0 + 32 * j);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[e] = far;
-        }
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          s = mfma32(frag_rm(qt, L, j, ks), kf[ks], s);
-          dp = mfma32(frag_rm(gt, L, j, ks), vf[ks], dp);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4_t nl = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 32 * j + 8 * g + 4 * h);
-          const f32x4_t de = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(st + cur * 128 + 64 + 32 * j + 8 * g + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], c2, nl[e]));
-            if (CAUSAL && qt0 + 32 * j + 8 * g + 4 * h + e < key) p = 0.f;
-            s[4 * g + e] = p;
-            dp[4 * g + e] = p * (dp[4 * g + e] - de[e]);
+            for (int e = 0; e < 16; ++e) s[e] = far;
           }
-        }
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          const s16x8_t pf = pack8r(s, 8 * kk), df = pack8r(dp, 8 * kk);
+          for (int ks = 0; ks < 4; ++ks) {
+            s = mfma32(frag_rm(qt, L, j, ks), kf[ks], s);
+            dp = mfma32(frag_rm(gt, L, j, ks), vf[ks], dp);
+          }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            dv[d] = mfma32(frag_tr(gt, L, 2 * j + kk, d), pf, dv[d]);
-            dk[d] = mfma32(frag_tr(qt, L, 2 * j + kk, d), df, dk[d]);
+          for (int g = 0; g < 4; ++g) {
+            const f32x4_t nl = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(row + 32 * j + 8 * g + 4 * h);
+            const f32x4_t de = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(row + 64 + 32 * j + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], c2, nl[e]));
+              if (CAUSAL && qt0 + 32 * j + 8 * g + 4 * h + e < key) p = 0.f;
+              s[4 * g + e] = p;
+              dp[4 * g + e] = p * (dp[4 * g + e] - de[e]);
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) {
+            const s16x8_t pf = pack8r(s, 8 * kk), df = pack8r(dp, 8 * kk);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              dv[d] = mfma32(frag_tr(gt, L, 2 * j + kk, d), pf, dv[d]);
+              dk[d] = mfma32(frag_tr(qt, L, 2 * j + kk, d), df, dk[d]);
+            }
           }
         }
       }
       dma_wait_all();
       __syncthreads();
     }
+    if constexpr (KVS == 2) {  // the tiles are done with
+      lds_float* const mine = (lds_float*)smem + wave / 2 * (64 * 64) + lane;
+      if (part) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            mine[(16 * d + e) * 64] = dk[d][e];
+            mine[(32 + 16 * d + e) * 64] = dv[d][e];
+          }
+        }
+      }
+      __syncthreads();
+      if (!part) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            dk[d][e] += mine[(16 * d + e) * 64];
+            dv[d][e] += mine[(32 + 16 * d + e) * 64];
+          }
+        }
+      }
+    }
   }
+  if (KVS == 2 && part) return;
   if (!kept) {  // a masked key's lane may hold anything
     dk[0] = dk[1] = dv[0] = dv[1] = zero16();
   }
@@ -702,14 +764,13 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
 }
 
 // both gradients in one launch (they share nothing but their inputs): twice the workgroups, so that a single prompt fills the chip
-template <bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256, 3) void attn_relpos_bwd_kernel(RelposArgs r) {
+template <bool BIAS, bool CAUSAL, int KVS>
+__global__ __launch_bounds__(256, KVS == 1 ? 3 : 1) void attn_relpos_bwd_kernel(RelposArgs r) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int nt = (r.a.S + 127) / 128;
   int tile_x, hd, b;
-  wg_coords(2 * nt, r.a.B, tile_x, hd, b);
-  if (tile_x < nt) dq_role<BIAS, CAUSAL>(r, smem, tile_x, hd, b);
-  else dkv_role<BIAS, CAUSAL>(r, smem, tile_x - nt, hd, b);
+  wg_coords(2 * r.tiles, r.a.B, tile_x, hd, b);
+  if (tile_x < r.tiles) dq_role<BIAS, CAUSAL, KVS>(r, smem, tile_x, hd, b);
+  else dkv_role<BIAS, CAUSAL, KVS>(r, smem, tile_x - r.tiles, hd, b);
 }
 
 // dtable[j][head] (+)= sum over the samples' row tiles, in their order
@@ -717,7 +778,7 @@ __global__ __launch_bounds__(256) void attn_relpos_dtable_kernel(RelposArgs r) {
   const AitkAttnRelposArgs& a = r.a;
   const int i = blockIdx.x * 256 + threadIdx.x, n = a.H * a.num_buckets;
   if (i >= n) return;
-  const int rows = a.B * ((a.S + 127) / 128);
+  const int rows = a.B * r.tiles;
   float v = 0.f;
 #pragma unroll 8
   for (int k = 0; k < rows; ++k) v += r.part[(long)k * n + i];
@@ -767,7 +828,7 @@ int check(const AitkAttnRelposArgs* a, bool bwd, RelposArgs& r) {
   }
   if (((int64_t)a->S + 64) * widest * 2 >= 0x7fffffff) return AITK_ERR_SHAPE;  // a head's slice is one buffer descriptor with 31-bit offsets
   r.a = *a;
-  r.half = r.sat = r.line_p = 0;
+  r.half = r.sat = r.line_p = r.tiles = 0;
   r.delta = r.part = nullptr;
   for (int i = 0; i < MAX_HALF; ++i) r.first[i] = 0;
   if (a->table) {
@@ -790,7 +851,7 @@ int launch(K kernel, unsigned grid, size_t lds, const RelposArgs& r, hipStream_t
   return AITK_OK;
 }
 
-constexpr int64_t KVS2_MOST = 256;  // workgroups of 128 rows (at most one per CU) up to which two waves share their rows
+constexpr int64_t KVS2_MOST = 256;  // workgroups (one per CU) up to which two waves share their rows: of 128 rows in the forward, of 64 in the backward
 
 template <int KVS>
 int launch_fwd(const RelposArgs& r, hipStream_t s) {
@@ -799,6 +860,19 @@ int launch_fwd(const RelposArgs& r, hipStream_t s) {
   const size_t lds = KVS * 4 * TILE + 512 + (size_t)4 * r.line_p * 4;
   if (a.table) return a.causal ? launch(attn_relpos_fwd_kernel<true, true, KVS>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<true, false, KVS>, grid, lds, r, s);
   return a.causal ? launch(attn_relpos_fwd_kernel<false, true, KVS>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<false, false, KVS>, grid, lds, r, s);
+}
+// The backward takes 64 rows per workgroup as long as every workgroup has a CU to itself (the doubled stages leave room for one; delta and dtable launches included, 64 / 128 rows: 16 heads x 512,
+// 256 workgroups of 64 rows, 22.7 / 30.3 us; 4 x 2048, 256 too, 42.5 / 61.4; 3 x 6 x 333 21.5 / 27.2; with 512 it takes two rounds: 32 x 512 38.6 / 30.6, 8 x 2048 78.8 / 62.2); one key tile
+// cannot be shared
+int bwd_kvs(int B, int H, int S) { return S > 64 && (int64_t)((S + 63) / 64) * H * B * 2 <= KVS2_MOST ? 2 : 1; }
+
+template <int KVS>
+int launch_bwd(const RelposArgs& r, hipStream_t s) {
+  const AitkAttnRelposArgs& a = r.a;
+  const unsigned grid = (unsigned)r.tiles * a.H * a.B * 2;
+  const size_t lds = KVS * (4 * TILE + 1024) + (size_t)4 * r.line_p * 4 + (a.dtable ? ((size_t)4 * (2 * (r.sat + BAND_PAD) + 1) + 3 + 4 * 8 * SKEW_P) * 4 : 0);
+  if (a.table) return a.causal ? launch(attn_relpos_bwd_kernel<true, true, KVS>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<true, false, KVS>, grid, lds, r, s);
+  return a.causal ? launch(attn_relpos_bwd_kernel<false, true, KVS>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<false, false, KVS>, grid, lds, r, s);
 }
 }  // namespace
 
@@ -821,22 +895,22 @@ extern "C" int aitk_attn_relpos_fwd(const AitkAttnRelposArgs* a, aitk_stream_t s
 
 extern "C" int64_t aitk_attn_relpos_bwd_workspace_bytes(int32_t B, int32_t H, int32_t S, int32_t num_buckets) {
   if (B <= 0 || H <= 0 || S <= 0 || num_buckets < 0) return 0;
-  return ((int64_t)2 * B * H * S + (int64_t)B * ((S + 127) / 128) * H * num_buckets) * 4;
+  const int rows = 128 / bwd_kvs(B, H, S);
+  return ((int64_t)2 * B * H * S + (int64_t)B * ((S + rows - 1) / rows) * H * num_buckets) * 4;
 }
 
 extern "C" int aitk_attn_relpos_bwd(const AitkAttnRelposArgs* a, aitk_stream_t stream) {
   RelposArgs r;
   int rc = check(a, true, r);
   if (rc != AITK_OK) return rc;
+  const int kvs = bwd_kvs(a->B, a->H, a->S), rows = 128 / kvs;
+  r.tiles = (a->S + rows - 1) / rows;
   r.delta = a->ws;
   r.part = a->ws + (int64_t)2 * a->B * a->H * a->S;
   hipStream_t s = (hipStream_t)stream;
   hipLaunchKernelGGL(attn_relpos_delta_kernel, dim3((a->S + 31) / 32, a->H, a->B), dim3(256), 0, s, r);
   AITK_LAUNCH_CHECK();
-  const unsigned grid = (unsigned)((a->S + 127) / 128) * a->H * a->B * 2;
-  const size_t lds = 4 * TILE + 1024 + (size_t)4 * r.line_p * 4 + (a->dtable ? ((size_t)4 * (2 * (r.sat + BAND_PAD) + 1) + 3 + 4 * 8 * SKEW_P) * 4 : 0);
-  if (a->table) rc = a->causal ? launch(attn_relpos_bwd_kernel<true, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<true, false>, grid, lds, r, s);
-  else rc = a->causal ? launch(attn_relpos_bwd_kernel<false, true>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<false, false>, grid, lds, r, s);
+  rc = kvs == 2 ? launch_bwd<2>(r, s) : launch_bwd<1>(r, s);
   if (rc != AITK_OK) return rc;
   if (a->dtable) {
     hipLaunchKernelGGL(attn_relpos_dtable_kernel, dim3((a->H * a->num_buckets + 255) / 256), dim3(256), 0, s, r);

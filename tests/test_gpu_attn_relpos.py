@@ -44,6 +44,8 @@ def _mask(kind, B, S, seed=0):
             m[b] = torch.rand(S, generator=g, device="cuda") < 0.5
         elif kind == "tail":  # left padding: whole tiles at the front are masked
             m[b, S - 1 - (S // 3) * (b % 3):] = True
+        elif kind == "late":
+            m[b, S - 60:] = True
     return m
 
 
@@ -130,6 +132,19 @@ def test_table_gradient_in_bf16():
 def test_more_than_one_group_of_key_tiles(mask):
     """over 4096 keys: the tile masks come in groups of 64; left padding masks whole tiles of the first group"""
     _run(2, 1, 4200, mask=mask, train=mask != "prefix")
+
+
+@pytest.mark.parametrize("mask", [None, "late", "holes"])
+def test_more_than_one_group_of_key_tiles_shared_by_two_waves(mask):
+    _run(1, 1, 4200, mask=mask, seed=4)
+
+
+@pytest.mark.parametrize("S", [77, 130, 333])
+@pytest.mark.parametrize("kind", [None, "prefix", "holes", "tail"])
+@pytest.mark.parametrize("bias,causal", [(True, False), (True, True), (False, True), (False, False)])
+def test_more_workgroups_than_compute_units(S, kind, bias, causal):
+    """128 rows to a workgroup in the backward and from S = 130 on in the forward (smaller launches share their rows between two waves)"""
+    _run(3, 32, S, mask=kind, bias=bias, causal=causal, poison=kind is not None, seed=S)
 
 
 def test_large_encoder_shape():
