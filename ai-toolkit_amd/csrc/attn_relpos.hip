@@ -488,13 +488,12 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           f32x16_t s, dp = zero16();
-          if (BIAS && side == 0) {
-            s = load_line(line, r.line_p, ib + kv0 + 32 * j);
-          } else {
-            s = zero16();
-          }
+          const s16x8_t kf = frag_rm(kt, L, j, 0);
+          if (BIAS && side == 0) s = mfma32(kf, qf[0], load_line(line, r.line_p, ib + kv0 + 32 * j));
+          else s = mfma32(kf, qf[0], zero16());
+          dp = mfma32(frag_rm(vt, L, j, 0), gf[0], dp);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
+          for (int ks = 1; ks < 4; ++ks) {
             s = mfma32(frag_rm(kt, L, j, ks), qf[ks], s);
             dp = mfma32(frag_rm(vt, L, j, ks), gf[ks], dp);
           }
@@ -815,7 +814,7 @@ bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
 bool bad_view(const void* p, int64_t ld, const AitkAttnRelposArgs* a) { return (ld % 8) || ld < (int64_t)a->H * 64 || mis16(p); }
 
 int check(const AitkAttnRelposArgs* a, bool bwd, RelposArgs& r) {
-  if (!a || a->B <= 0 || a->H <= 0 || a->S <= 0 || a->H > 65535 || a->B > 65535 || !(a->scale > 0.f) || a->scale > 3.0e38f) return AITK_ERR_SHAPE;
+  if (!a || a->B <= 0 || a->H <= 0 || a->S <= 0 || a->H > 65535 || a->B > 65535 || !(a->scale >= 1e-6f) || a->scale > 1e6f) return AITK_ERR_SHAPE;
   if ((int64_t)a->B * a->H * ((a->S + 127) / 128) * 2 > 0x7fffffff) return AITK_ERR_SHAPE;
   if (!a->Q || !a->K || !a->V || !a->O || !a->LSE) return AITK_ERR_ARG;
   if (bad_view(a->Q, a->ldq, a) || bad_view(a->K, a->ldk, a) || bad_view(a->V, a->ldv, a) || bad_view(a->O, a->ldo, a)) return AITK_ERR_ALIGN;
