@@ -1319,8 +1319,8 @@ def norm_bwd(dy, x, weight, rstd, dx, *, mean=None, rms=False, dres=None, dweigh
 
 
 def _attn_relpos_check(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal):
-    if not (B >= 0 and H > 0 and S >= 0 and 0.0 < scale < 1e30):
-        raise ValueError(f"B, H, S, scale: got {B}, {H}, {S}, {scale} (scale must be positive and finite)")
+    if not (B >= 0 and H > 0 and S >= 0 and 1e-6 <= scale <= 1e6):
+        raise ValueError(f"B, H, S, scale: got {B}, {H}, {S}, {scale} (scale: 1e-6 to 1e6)")
     shape = (B * S, H * 64)
     pq, ldq = _rows(q, "q", shape)
     pk, ldk = _rows(k, "k", shape)
@@ -1350,7 +1350,7 @@ def attn_relpos_fwd(q, k, v, table, o, lse, *, B, H, S, scale=1.0, key_mask=None
     """o = softmax(scale q k^T + table[bucket(key - query)]) v: the text encoders' attention with a learned relative position bias.  q, k, v, o: [B*S, H*64] bf16 views
     (row pitch = token pitch); table: bf16 [num_buckets, H] (T5's relative_attention_bias.weight) or None (no bias: CLIP); lse: fp32 [B, H, S], written for the backward.
     key_mask: bool / uint8 [B, S], non-zero = attend; causal: keys up to the query, all buckets for the past.  A row that the masks leave empty gives 0 (lse = -inf);
-    what masked keys hold reaches nothing, NaN and infinities too."""
+    what masked keys hold reaches nothing, NaN and infinities too.  A score below -2e38 (a table entry of -inf or the type's lowest value) counts as masked."""
     _, nb, head = _attn_relpos_check(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
     a = _capi.AttnRelposArgs(*head, None, 0, None, None, None, 0, 0, 0, None, None, scale, B, H, S, nb, max_distance, 1 if causal else 0)
     _on_device("q, k, v, table, o, lse, key_mask", (q, k, v, table, o, lse, key_mask))
@@ -1362,12 +1362,16 @@ def attn_relpos_fwd(q, k, v, table, o, lse, *, B, H, S, scale=1.0, key_mask=None
 def attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable=None, *, B, H, S, scale=1.0, key_mask=None, max_distance=128, causal=False, accumulate=False):
     """dq, dk, dv ([B*S, H*64] bf16 views) and, if given, dtable ([num_buckets, H] bf16 or fp32: the table's gradient, added to what it holds with `accumulate` — T5's layers
     share one table) from attn_relpos_fwd's operands, o and lse.  The probabilities are recomputed; every sum has a fixed order.  dtable's fp32 form is as exact as the
-    bf16 operands o and do it is formed from, not more."""
+    bf16 operands o and do it is formed from, not more.  The gradients must not lie on the operands."""
     shape, nb, head = _attn_relpos_check(q, k, v, table, o, lse, B, H, S, scale, key_mask, max_distance, causal)
+    pq, pk, pv = head[:3]
     pdo, lddo = _rows(do, "do", shape)
     pdq, lddq = _rows(dq, "dq", shape)
     pdk, lddk = _rows(dk, "dk", shape)
     pdv, lddv = _rows(dv, "dv", shape)
+    read = (pq, pk, pv, head[6], pdo)  # whole tiles of the operands are read while the gradients are written
+    if B * S and (pdq in read or pdk in read or pdv in read or pdq == pdk or pdk == pdv or pdv == pdq):
+        raise ValueError("dq, dk and dv must not lie on each other or on q, k, v, o or do")
     if (S + 64) * lddo * 2 >= 2 ** 31 - 1:
         raise ValueError("a head's slice of do must stay below 2 GiB")
     pdt, f32 = None, 0
@@ -1415,10 +1419,12 @@ def _pitches(*lds):
 def gated_ffn_fwd(x, w_val, w_gate, out, *, act="gelu_tanh", b_val=None, b_gate=None, hg=None):
     """out = (x w_val^T + b_val) * act(x w_gate^T + b_gate) in one launch: x [M, K], weights [F, K] (one row pitch: two views of a fused [2F, K] matrix, or two matrices),
     biases [F] or None, out [M, F], all bf16.  act: "gelu_tanh" (T5 / UMT5), "gelu" (erf: GEGLU) or "silu".  hg [M, 2F]: also leaves [value | gate] before the
-    activation, which gated_ffn_bwd needs (geglu_fwd's layout).  K % 8 == F % 8 == 0."""
+    activation, which gated_ffn_bwd needs (geglu_fwd's layout).  K % 8 == F % 8 == 0.  The results must not lie on the operands."""
     M, K, F, px, ldx, pv, pg, ldw = _ffn_check(x, w_val, w_gate, act)
     po, ld_out = _rows(out, "out", (M, F))
     ph, ld_hg = (None, 0) if hg is None else _rows(hg, "hg", (M, 2 * F))
+    if M and (po in (px, pv, pg) or ph in (px, pv, pg, po)):
+        raise ValueError("out and hg must not lie on each other or on x or the weights")
     _pitches(ldx, ld_out, ld_hg, ldw)
     a = _capi.GatedFfnArgs(px, ldx, pv, pg, ldw, _vec(b_val, "b_val", F, (BF16,)), _vec(b_gate, "b_gate", F, (BF16,)), po, ld_out, ph, ld_hg, M, K, F, GATED_ACTS[act])
     _on_device("x, w_val, w_gate, out, b_val, b_gate, hg", (x, w_val, w_gate, out, b_val, b_gate, hg))
@@ -1429,7 +1435,8 @@ def gated_ffn_fwd(x, w_val, w_gate, out, *, act="gelu_tanh", b_val=None, b_gate=
 
 def gated_ffn_bwd(dh, x, w_val, w_gate, hg, *, act="gelu_tanh", dx=None, dw_val=None, dw_gate=None, db_val=None, db_gate=None):
     """gated_ffn_fwd's gradients from dh [M, F] and the saved hg: dx [M, K], dw_val / dw_gate [F, K] (one row pitch), db_val / db_gate [F], all bf16; only what is
-    given is computed (frozen weights: dx alone).  Nothing is transposed or copied beyond the one [M, 2F] gradient of hg.  Deterministic."""
+    given is computed (frozen weights: dx alone).  Nothing is transposed or copied beyond the one [M, 2F] gradient of hg.  Deterministic.  dx may lie on dh or hg, nothing
+    else on an operand."""
     M, K, F, px, ldx, pv, pg, ldw = _ffn_check(x, w_val, w_gate, act)
     pdh, ld_dh = _rows(dh, "dh", (M, F))
     phg, ld_hg = _rows(hg, "hg", (M, 2 * F))
@@ -1441,6 +1448,9 @@ def gated_ffn_bwd(dh, x, w_val, w_gate, hg, *, act="gelu_tanh", dx=None, dw_val=
         if dw_val is not None and ld != ld_dw:
             raise ValueError(f"dw_val and dw_gate must share one row pitch, got {ld_dw} and {ld}")
         ld_dw = ld
+    written = [p for p in (pdx, pdv, pdg) if p]
+    if len({px, pv, pg, *written}) < len({px, pv, pg}) + len(written):  # x and the weights are read while the gradients are written
+        raise ValueError("dx, dw_val and dw_gate must not lie on each other or on x or the weights")
     pbv, pbg = _vec(db_val, "db_val", F, (BF16,)), _vec(db_gate, "db_gate", F, (BF16,))
     _pitches(ld_dh, ldx, ld_hg, ldw, ld_dx, ld_dw)
     if M > 32 * 65535:

@@ -621,7 +621,8 @@ int aitk_norm_bwd(const AitkNormBwdArgs* args, aitk_stream_t stream);
  * table: bf16 [num_buckets, H] (T5's relative_attention_bias.weight), NULL = no bias (CLIP).  Buckets: of each sign's `half` (num_buckets / 2, the second half for keys
  * ahead of the query; causal: all num_buckets for the past) the first half / 2 are one distance each, the others split the logarithm up to max_distance, the last takes
  * the rest; 2 <= half <= 64, half / 2 < max_distance <= 1024.  LSE [B, H, S] fp32 is in the scaled log2 domain like AitkAttnArgs.LSE.
- * A row without any key gives o = 0, lse = -inf and zero gradients; what masked keys hold (NaN and infinities too) reaches nothing.
+ * A row without any key gives o = 0, lse = -inf and zero gradients; what masked keys hold (NaN and infinities too) reaches nothing.  A score below -2e38 counts as masked.
+ * scale: 1e-6 to 1e6.  dQ, dK, dV must not lie on each other or on an operand.
  * Backward writes dQ, dK, dV and, if dtable is set, [num_buckets, H] bucket sums (bf16, or fp32 with dtable_f32; added to what is there with accumulate): the bias's gradient,
  * summed in fp32 in a fixed order.  Deterministic.  ws: aitk_attn_relpos_bwd_workspace_bytes bytes (num_buckets 0 without dtable).
  * A head's slice stays below 2 GiB ((S + 64) * row pitch * 2 bytes); pitches % 8 == 0, 16-byte aligned. */
@@ -655,7 +656,8 @@ typedef struct AitkGatedFfnArgs {
 int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* args, aitk_stream_t stream);
 /* From dh [M, F] and the saved hg: dx [M, K], dw_val / dw_gate [F, K] (one row pitch), db_val / db_gate [F], all bf16, each may be NULL (frozen weights: dx alone).
  * [du | dz] is formed once in bf16 in ws (aitk_gated_ffn_bwd_workspace_bytes; dx .. bias_grads: which results are asked for); no transposed copy of any operand is made.
- * Where a product has few tiles and a long contraction, pieces of it are summed in fp32 in a fixed order.  Deterministic. */
+ * Where a product has few tiles and a long contraction, pieces of it are summed in fp32 in a fixed order.  Deterministic.  Results must not lie on x, the weights or each
+ * other (dx may lie on dh or hg). */
 typedef struct AitkGatedFfnBwdArgs {
   const aitk_bf16* dh; int64_t ld_dh;
   const aitk_bf16* x; int64_t ldx;

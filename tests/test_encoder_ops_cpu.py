@@ -170,7 +170,7 @@ def test_attention_wrapper_refusals():
                        (dict(table=_t(32, H, dtype=torch.float32)), "table"), (dict(max_distance=8), "max_distance"), (dict(max_distance=2000), "max_distance"),
                        (dict(lse=_t(B, H, S)), "lse"), (dict(lse=_t(B, H, S - 1, dtype=torch.float32)), "lse"), (dict(key_mask=torch.ones(B, S)), "key_mask"),
                        (dict(key_mask=torch.ones(B, S, dtype=torch.int64)), "key_mask"), (dict(key_mask=torch.ones(B, S + 1, dtype=torch.bool)), "key_mask"),
-                       (dict(key_mask=torch.ones(S, B, dtype=torch.bool).t()), "key_mask"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(B=3), "expected"),
+                       (dict(key_mask=torch.ones(S, B, dtype=torch.bool).t()), "key_mask"), (dict(scale=0.0), "scale"), (dict(scale=1e-7), "scale"), (dict(scale=float("nan")), "scale"), (dict(B=3), "expected"),
                        (dict(H=0), "B, H, S")):
         kw = dict(base, B=B, H=H, S=S)
         kw.update(bad)
@@ -184,7 +184,8 @@ def test_attention_wrapper_refusals():
         ops.attn_relpos_fwd(*_huge_views(), B=1, H=1, S=600)
     do, dq, dk, dv = mk(), mk(), mk(), mk()
     for bad, match in ((dict(dtable=_t(32, H, dtype=torch.float16)), "dtable"), (dict(dtable=_t(16, H)), "dtable"), (dict(table=None, dtable=_t(32, H)), "without a table"),
-                       (dict(do=_t(B * S, 64)), "do"), (dict(dv=mk().float()), "dv")):
+                       (dict(do=_t(B * S, 64)), "do"), (dict(dv=mk().float()), "dv"), (dict(dq=base["q"]), "must not lie"), (dict(dk=do), "must not lie"),
+                       (dict(dv=dq), "must not lie"), (dict(dq=base["o"]), "must not lie")):
         kw = dict(base, do=do, dq=dq, dk=dk, dv=dv, dtable=None)
         kw.update(bad)
         with pytest.raises(ValueError, match=match):
@@ -209,9 +210,10 @@ def _huge_views():
 def test_gated_ffn_wrapper_refusals():
     M, K, F = 4, 64, 128
     base = dict(x=_t(M, K), w_val=_t(F, K), w_gate=_t(F, K), out=_t(M, F))
+    same = _t(F, F)
     for bad, match in ((dict(act="relu"), "act"), (dict(x=_t(M, K + 8)), "do not match"), (dict(w_val=_t(F, 60), x=_t(M, 60)), "multiples of 8"), (dict(w_val=_t(12, K)), "multiples of 8"),
                        (dict(w_gate=_t(F + 8, K)), "w_gate"), (dict(w_gate=_t(F, K + 8)[:, :K]), "one row pitch"), (dict(out=_t(M, F + 8)), "out"), (dict(hg=_t(M, F)), "hg"),
-                       (dict(b_val=_t(F, dtype=torch.float32)), "b_val"), (dict(b_gate=_t(F + 8)), "b_gate"), (dict(x=_t(M, K).float()), "bf16")):
+                       (dict(out=same, w_val=same[:, :K], w_gate=same[:, :K], x=_t(F, K)), "must not lie"), (dict(b_val=_t(F, dtype=torch.float32)), "b_val"), (dict(b_gate=_t(F + 8)), "b_gate"), (dict(x=_t(M, K).float()), "bf16")):
         kw = dict(base)
         kw.update(bad)
         args = [kw.pop(n) for n in ("x", "w_val", "w_gate", "out")]
@@ -219,9 +221,10 @@ def test_gated_ffn_wrapper_refusals():
             ops.gated_ffn_fwd(*args, **kw)
     with pytest.raises(ValueError, match="GPU"):
         ops.gated_ffn_fwd(**base)
-    dh, hg = _t(M, F), _t(M, 2 * F)
+    dh, hg, dw = _t(M, F), _t(M, 2 * F), _t(F, K)
     for bad, match in ((dict(dh=_t(M, K)), "dh"), (dict(hg=_t(M, F)), "hg"), (dict(dx=_t(M, F)), "dx"), (dict(dw_val=_t(K, F)), "dw_val"), (dict(db_gate=_t(K)), "db_gate"),
-                       (dict(dw_val=_t(F, K), dw_gate=_t(F, K + 8)[:, :K]), "one row pitch")):
+                       (dict(dw_val=_t(F, K), dw_gate=_t(F, K + 8)[:, :K]), "one row pitch"), (dict(dx=base["x"]), "must not lie"), (dict(dw_gate=base["w_val"]), "must not lie"),
+                       (dict(dw_val=dw, dw_gate=dw), "must not lie")):
         kw = dict(dh=dh, x=base["x"], w_val=base["w_val"], w_gate=base["w_gate"], hg=hg)
         kw.update(bad)
         args = [kw.pop(n) for n in ("dh", "x", "w_val", "w_gate", "hg")]

@@ -115,6 +115,31 @@ def test_bucketings(buckets, max_distance, causal):
     _run(1, 2, 700, buckets=buckets, max_distance=max_distance, causal=causal)
 
 
+@pytest.mark.parametrize("value", [float("-inf"), torch.finfo(BF16).min])
+@pytest.mark.parametrize("S", [64, 200, 333])
+def test_table_entries_that_forbid_a_bucket(value, S):
+    """the type's lowest value and -inf in the table, near and far buckets, at both scales: those keys get no weight and no gradient, the others what is theirs"""
+    from ai_toolkit_amd import ops
+
+    for scale in (1.0, 0.125):
+        B, H = 2, 3
+        q, k, v, table, o, do, dq, dk, dv = _inputs(B, H, S, scale=scale, layout="pitched", seed=S)
+        table[17:, 0] = value  # every key ahead
+        table[15, 1] = value   # the far past
+        table[3:6, 2] = value  # a few distances
+        kw = dict(B=B, H=H, S=S, scale=scale, key_mask=None, max_distance=128, causal=False)
+        want = ref.attention(q, k, v, table, do=do, **kw)
+        lse = torch.zeros(B, H, S, device="cuda")
+        ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+        dtable = torch.empty(32, H, device="cuda")
+        ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable, **kw)
+        torch.cuda.synchronize()
+        for name, t in (("o", o), ("dv", dv), ("dq", dq), ("dk", dk)):
+            _near(t, want[name], want["tol_" + name], name)
+        _near(dtable, want["dtable"], want["tol_dtable"] * (1 + ref.U) + 1e-30, "dtable")
+        assert (dtable[17:, 0] == 0).all() and (dtable[3:6, 2] == 0).all()
+
+
 @pytest.mark.parametrize("bias,causal,scale", [(False, True, 0.125), (False, False, 0.125), (True, False, 0.125), (True, True, 0.3)])
 def test_without_bias_and_with_a_scale(bias, causal, scale):
     _run(2, 4, 150, bias=bias, causal=causal, scale=scale, layout="pitched")
