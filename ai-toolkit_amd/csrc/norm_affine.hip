@@ -134,12 +134,13 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(AitkNormArgs p) {
 // Backward.  A workgroup walks its rows with the next row's x and dy in flight; each thread owns fixed columns and sums dy xh and dy over its rows in registers; the column
 // sums of all its rows leave the workgroup as ONE row of partials.  A CU's registers hold 16 waves with 2 vectors per lane (two workgroups of 512 threads), 12 with 3 (one of 768), 8 with
 // 4 (one of 512): see bwd_form().
-#define NB_SLOTS(LPR) ((LPR) == 256 ? 1 : 4)  // column sums of so many row groups meet in LDS at a time (at most 32 KiB)
+#define NB_SLOTS(LPR) ((LPR) == 256 ? 1 : 4)  // column sums of so many row groups meet in LDS at a time (at most 32 KiB), of both gradients if they fit
+#define NB_PASS(RMS, LPR, NV) (!(RMS) && 2 * NB_SLOTS(LPR) * (NV) * 8 * (LPR) * 4 < 65000 ? 2 : 1)
 template <int TH, int LPR, int NV, bool RMS, bool GRADS>
 __global__ __launch_bounds__(TH) void norm_bwd_kernel(AitkNormBwdArgs p) {
   constexpr int RPW = TH / LPR;
   __shared__ float red[2][2][TH / 64];
-  extern __shared__ __attribute__((aligned(16))) float colsum[];  // [SLOTS][C] when GRADS
+  extern __shared__ __attribute__((aligned(16))) float colsum[];  // [NB_PASS][SLOTS][places] when GRADS
   const int t = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   const float inv_c = 1.0f / (float)p.C;
   float dw[NV][8] = {}, db[NV][8] = {};
@@ -225,67 +226,71 @@ __global__ __launch_bounds__(TH) void norm_bwd_kernel(AitkNormBwdArgs p) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int o = LPR; o < 64; o <<= 1) {
-            dw[i][e] += __shfl_xor(dw[i][e], o, 64);
-            if (!RMS) db[i][e] += __shfl_xor(db[i][e], o, 64);
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (LPR == 16) dw[i][e] = plus_swapped<16>(dw[i][e]);
+          dw[i][e] = plus_swapped<32>(dw[i][e]);
+          if constexpr (!RMS) {
+            if constexpr (LPR == 16) db[i][e] = plus_swapped<16>(db[i][e]);
+            db[i][e] = plus_swapped<32>(db[i][e]);
           }
+        }
     }
-    // the row groups of the workgroup meet in LDS in a fixed order, one vector after the other
-    constexpr int G = LPR < 64 ? TH / 64 : RPW, SLOTS = NB_SLOTS(LPR);
+    // The row groups of the workgroup meet in LDS in a fixed order.  A lane's element e of vector i goes to (8 i + e) LPR + t: neighbouring lanes, neighbouring banks (in the columns' own
+    // order eight lanes meet in a bank: 1 x 1280 12.3 us, of them 7 here); the partials keep that order, the last launch undoes it.
+    constexpr int G = LPR < 64 ? TH / 64 : RPW, SLOTS = NB_SLOTS(LPR), P = NV * 8 * LPR;
     const int g = LPR < 64 ? threadIdx.x >> 6 : grp;
     const bool holds = LPR >= 64 || (threadIdx.x & 63) < LPR;
-    for (int v = 0; v < (RMS ? 1 : 2); ++v) {
+    constexpr int PASS = NB_PASS(RMS, LPR, NV);
+    for (int v0 = 0; v0 < (RMS ? 1 : 2); v0 += PASS) {
       for (int r0 = 0; r0 < G; r0 += SLOTS) {
         __syncthreads();
         if (holds && g >= r0 && g < r0 + SLOTS) {
-          float* dst = colsum + (g - r0) * p.C;
 #pragma unroll
-          for (int i = 0; i < NV; ++i) {
-            const int c = (t + LPR * i) * 8;
-            if (c < p.C) {
+          for (int q = 0; q < PASS; ++q) {
+            float* const dst = colsum + (q * SLOTS + g - r0) * P + t;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const float a = v ? db[i][e] : dw[i][e];
-                dst[c + e] = r0 ? dst[c + e] + a : a;
+                const float a = v0 + q ? db[i][e] : dw[i][e];
+                float* const d = dst + (8 * i + e) * LPR;
+                *d = r0 ? *d + a : a;
               }
-            }
           }
         }
       }
       __syncthreads();
-      float* out = p.partial + ((long)blockIdx.x * (RMS ? 1 : 2) + v) * p.C;
-      for (int c = threadIdx.x; c < p.C; c += TH) {
-        float a = colsum[c];
-        for (int k = 1; k < SLOTS; ++k) a += colsum[k * p.C + c];
+      float* out = p.partial + ((long)blockIdx.x * (RMS ? 1 : 2) + v0) * P;
+      for (int c = threadIdx.x; c < PASS * P; c += TH) {
+        const float* q = colsum + (c < P ? c : c - P + SLOTS * P);
+        float a = q[0];
+#pragma unroll
+        for (int k = 1; k < SLOTS; ++k) a += q[k * P];
         out[c] = a;
       }
     }
   }
 }
 
-// the workgroups' partials [nwg][V][C] -> dw, db: 32 columns per workgroup (8 float4 lanes x 32 slices of the workgroups), fixed order
-__global__ __launch_bounds__(256) void norm_wgrad_finish_kernel(const float* partial, int nwg, int V, int C, float* dw, float* db, int accumulate) {
+// the workgroups' partials [nwg][V][P] -> dw, db: 32 places per workgroup (8 float4 lanes x 32 slices of the workgroups), fixed order
+__global__ __launch_bounds__(256) void norm_wgrad_finish_kernel(const float* partial, int nwg, int V, int P, int lanes, int C, float* dw, float* db, int accumulate) {
   __shared__ float4 part[32][8];
-  const int j = threadIdx.x & 7, sl = threadIdx.x >> 3;
-  const int c = blockIdx.x * 32 + j * 4, v = blockIdx.y;
+  const int j = threadIdx.x & 7, sl = threadIdx.x >> 3, v = blockIdx.y;
+  const float* q = partial + (long)v * P + blockIdx.x * 32 + j * 4;  // P is a multiple of 128
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (c < C) {
 #pragma unroll 8
-    for (int w = sl; w < nwg; w += 32) {
-      const float4 a = *reinterpret_cast<const float4*>(partial + ((long)w * V + v) * C + c);
-      s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
-    }
+  for (int w = sl; w < nwg; w += 32) {
+    const float4 a = *reinterpret_cast<const float4*>(q + (long)w * V * P);
+    s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
   }
   part[sl][j] = s;
   __syncthreads();
   float* out = v ? db : dw;
   if (threadIdx.x < 32) {
-    const int col = blockIdx.x * 32 + threadIdx.x;
+    const int at = blockIdx.x * 32 + threadIdx.x, t = at % lanes, k = at / lanes, col = (t + lanes * (k >> 3)) * 8 + (k & 7);
     if (out && col < C) {
       float a = 0.f;
-      for (int k = 0; k < 32; ++k) a += reinterpret_cast<const float*>(&part[k][0])[threadIdx.x];
+      for (int i = 0; i < 32; ++i) a += reinterpret_cast<const float*>(&part[i][0])[threadIdx.x];
       out[col] = accumulate ? out[col] + a : a;
     }
   }
@@ -293,18 +298,21 @@ __global__ __launch_bounds__(256) void norm_wgrad_finish_kernel(const float* par
 
 bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
 
-// form of the backward: threads and lanes per row, and the workgroups that the CUs hold at a time
+// form of the backward: threads, lanes per row, 16-byte vectors per lane, and the workgroups that the CUs hold at a time
 struct BwdForm {
-  int threads, lanes, most;
+  int threads, lanes, vecs, most;
+  int places() const { return lanes * vecs * 8; }  // of a row of partials
 };
 BwdForm bwd_form(int C) {
-  if (C <= 256) return {512, 16, 512};
-  if (C <= 512) return {512, 32, 512};
-  if (C <= 768) return {768, 32, 256};
-  if (C <= 1024) return {512, 64, 512};
-  if (C <= 1536) return {768, 64, 256};
-  if (C <= 2048) return {512, 64, 256};
-  return {512, 256, 256};
+  if (C <= 128) return {512, 16, 1, 512};
+  if (C <= 256) return {512, 16, 2, 512};
+  if (C <= 512) return {512, 32, 2, 512};
+  if (C <= 768) return {768, 32, 3, 256};
+  if (C <= 1024) return {512, 64, 2, 512};
+  if (C <= 1536) return {768, 64, 3, 256};
+  if (C <= 2048) return {512, 64, 4, 256};
+  if (C <= 4096) return {512, 256, 2, 256};
+  return {512, 256, 4, 256};
 }
 int bwd_grid(int M, int C) {
   const BwdForm f = bwd_form(C);
@@ -323,7 +331,7 @@ template <int TH, int LPR, int NV>
 void launch_bwd(const AitkNormBwdArgs& a, hipStream_t s) {
   const dim3 grid(bwd_grid(a.M, a.C));
   if (a.dweight || a.dbias) {
-    const size_t lds = (size_t)NB_SLOTS(LPR) * a.C * 4;
+    const size_t lds = (size_t)NB_SLOTS(LPR) * NV * 8 * LPR * 4 * (a.rms ? 1 : NB_PASS(false, LPR, NV));
     if (a.rms) hipLaunchKernelGGL((norm_bwd_kernel<TH, LPR, NV, true, true>), grid, dim3(TH), lds, s, a);
     else hipLaunchKernelGGL((norm_bwd_kernel<TH, LPR, NV, false, true>), grid, dim3(TH), lds, s, a);
   } else {  // without the sums' registers
@@ -355,7 +363,7 @@ extern "C" int aitk_norm_fwd(const AitkNormArgs* a, aitk_stream_t stream) {
 
 extern "C" int64_t aitk_norm_bwd_workspace_bytes(int32_t M, int32_t C, int32_t rms) {
   if (M <= 0 || C <= 0) return 0;
-  return (int64_t)bwd_grid(M, C) * (rms ? 1 : 2) * C * 4;
+  return (int64_t)bwd_grid(M, C) * (rms ? 1 : 2) * bwd_form(C).places() * 4;
 }
 
 extern "C" int aitk_norm_bwd(const AitkNormBwdArgs* a, aitk_stream_t stream) {
@@ -379,7 +387,9 @@ extern "C" int aitk_norm_bwd(const AitkNormBwdArgs* a, aitk_stream_t stream) {
   AITK_LAUNCH_CHECK();
   if (grads) {
     const int V = a->rms ? 1 : 2;
-    hipLaunchKernelGGL(norm_wgrad_finish_kernel, dim3((C + 31) / 32, V), dim3(256), 0, s, a->partial, bwd_grid(a->M, C), V, C, a->dweight, a->dbias, a->accumulate);
+    const BwdForm f = bwd_form(C);
+    hipLaunchKernelGGL(norm_wgrad_finish_kernel, dim3(f.places() / 32, V), dim3(256), 0, s, a->partial, bwd_grid(a->M, C), V, f.places(), f.lanes, C, a->dweight, a->dbias,
+                       a->accumulate);
     AITK_LAUNCH_CHECK();
   }
   return AITK_OK;
