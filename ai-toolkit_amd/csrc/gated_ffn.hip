@@ -383,8 +383,8 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_fwd_kernel(FfnArgs a, 
   }
 }
 
-// Forward for a few rows (at most 16 TB): bound by the weights' way from memory.  A workgroup takes 16 rows of both weights, its eight waves every eighth 32-wide step of the
-// contraction; weights and x go straight from global memory into the matrix operands (W is the A operand of the 16 x 16 x 32 product, the tokens are its columns), four steps of
+// Forward for few rows: bound by the weights' way from memory, in small layers by its latency.  A workgroup takes 16 rows of both weights and 16 TB of x, its eight waves every eighth
+// 32-wide step of the contraction; weights and x go straight from global memory into the matrix operands (W is the A operand of the 16 x 16 x 32 product, the tokens are its columns), four steps of
 // loads in flight per wave; the waves' sums meet in LDS in a fixed order.
 template <int TB>
 __global__ __launch_bounds__(512) void gated_ffn_few_kernel(FfnArgs a) {
@@ -392,13 +392,13 @@ __global__ __launch_bounds__(512) void gated_ffn_few_kernel(FfnArgs a) {
   __shared__ f32x4_t box[8][2 * TB][64];
   const Prod& p = a.p[0];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kg = lane >> 4;
-  const int f0 = blockIdx.x * 16;
+  const int f0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * TB;
   const bf16_t* w[2];
 #pragma unroll
   for (int v = 0; v < 2; ++v) w[v] = p.B[v] + (long)min(f0 + r16, p.N - 1) * p.ldb + kg * 8;
   const bf16_t* x[TB];
 #pragma unroll
-  for (int t = 0; t < TB; ++t) x[t] = p.A[0] + (long)min(t * 16 + r16, p.M - 1) * p.lda + kg * 8;
+  for (int t = 0; t < TB; ++t) x[t] = p.A[0] + (long)min(m0 + t * 16 + r16, p.M - 1) * p.lda + kg * 8;
   f32x4_t acc[2][TB];
 #pragma unroll
   for (int t = 0; t < TB; ++t) acc[0][t] = acc[1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(512) void gated_ffn_few_kernel(FfnArgs a) {
 #pragma unroll
     for (int t = 0; t < TB; ++t) box[wave][2 * t + v][lane] = acc[v][t];
   __syncthreads();
-  const int m = wave * 16 + r16, n = f0 + 4 * kg;  // wave t finishes token block t: lane -> token r16, rows 4 kg .. + 3 of the weights
+  const int m = m0 + wave * 16 + r16, n = f0 + 4 * kg;  // wave t finishes token block t: lane -> token r16, rows 4 kg .. + 3 of the weights
   if (wave >= TB || m >= p.M || n >= p.N) return;
   f32x4_t z = box[0][2 * wave][lane], u = box[0][2 * wave + 1][lane];
 #pragma unroll
@@ -683,14 +683,20 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   hipStream_t s = (hipStream_t)stream;
   const int64_t big = tiles(q->M, q->F, 256, 128), small = tiles(q->M, q->F, 128, 64);
   if (small > 0x7fffffff) return AITK_ERR_SHAPE;
-  const unsigned strips = (unsigned)((q->F + 15) / 16);
-  // up to 32 rows the weights' way bounds both forms: 4096 x 10240 16 rows 36 us against 48 us of the small tiles, 32 rows 45 against 48, 512 x 1024 3.8 / 4.5 against 11 us.  Up to 64
-  // rows the waves read x more often than W: 64 rows 69 us against 48 for 4096 x 10240 (168 MB), but 8.5 against 16.5 for 1024 x 2816 (12 MB): there the tiles' start-up decides.
-  if (q->M <= 32 || (q->M <= 64 && (int64_t)q->F * q->K <= (8 << 20))) {
-    if (q->M <= 16) return launch(gated_ffn_few_kernel<1>, strips, 512, 0, s, a);
-    if (q->M <= 32) return launch(gated_ffn_few_kernel<2>, strips, 512, 0, s, a);
-    return launch(gated_ffn_few_kernel<4>, strips, 512, 0, s, a);
-  }
+  // Few rows: blocks of 16 TB rows x strips of 16 columns, as long as a strip's work is short.  16 or 32 rows to a workgroup while every one of them has a CU to itself, 64 while two share
+  // one (us with 16 / 32 / 64 rows / tiles: 512 x 1024 64 rows 4.8 / 5.4 / 6.6 / 11, 128 rows 6.0 / 5.5 / 6.7 / 11, 256 rows 8.8 / 7.2 / 6.9 / 11; 4096 x 512 128 rows 14 / 18 / 25 / 47;
+  // 4096 x 4096 64 rows 47 / 33 / 26 / 47, 128 rows 91 / 61 / 49 / 48; 768 x 2048 256 rows - / 14.3 / 13.2 / 14.0, 512 rows - / 25 / 23 / 14), and up to 32 rows always: then the weights' way bounds every
+  // form (4096 x 10240: 16 rows 36 us against 48 of the tiles, 32 rows 45).
+  const int64_t strips = (q->F + 15) / 16;
+  const auto blocks = [&](int tb) { return (q->M + 16 * tb - 1) / (16 * tb); };
+  const auto few = [&](auto kernel, int tb) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)strips, (unsigned)blocks(tb)), dim3(512), 0, s, a);
+    AITK_LAUNCH_CHECK();
+    return (int)AITK_OK;
+  };
+  if (q->M <= 16 || strips * blocks(1) <= 256) return few(gated_ffn_few_kernel<1>, 1);
+  if (q->M <= 32 || strips * blocks(2) <= 256) return few(gated_ffn_few_kernel<2>, 2);
+  if (strips * blocks(4) <= 512) return few(gated_ffn_few_kernel<4>, 4);
   // Large tiles (one workgroup per CU), the last round in halves if they all find a CU; 128 x 128 tiles (two workgroups per CU) only while every one of them has a CU to itself.  Large
   // with halves / large / small, us: 4096 x 640 x 2560 (320 tiles) 44 / 50 / 50; 2048 x 4096 x 10240 (640) 301 / 316 / 397; 512 x 4096 x 10240 (160) 92 / 92 / 120; 1024 x 640 x 2560
   // (80 large, 320 small) 17.2 / 24 / 17.7; 1000 x 768 x 2048 (64, 256) 17.6 / 25 / 16.1; 77 x 4096 x 10240 (80, 160) 58 / 84 / 48.

@@ -119,6 +119,13 @@ def test_large_tiles(M, K, F, act):
     _case(M, K, F, act=act, bias=act == "gelu")
 
 
+# more strips of the weights than a launch for few rows takes, fewer tiles than compute units
+@pytest.mark.parametrize("M,K,F", [(600, 136, 1000), (130, 72, 4104), (700, 8, 1032), (129, 520, 6000), (1000, 768, 2048)])
+@pytest.mark.parametrize("bias,fused,pitch", [(False, False, 0), (True, True, 40)])
+def test_small_tiles(M, K, F, bias, fused, pitch):
+    _case(M, K, F, bias=bias, fused=fused, pitch=pitch, act="gelu" if bias else "silu")
+
+
 @pytest.mark.parametrize("act", ["gelu_tanh", "gelu", "silu"])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("fused", [False, True])
