@@ -527,18 +527,24 @@ __global__ __launch_bounds__(256) void gated_ffn_join_kernel(FfnArgs a) {
   }
 }
 
-// [du | dz] from dh and [u | z]; with SUMS the fp32 column sums of the workgroup's rows.  Memory bound: three reads, two writes.  A thread owns 8 columns.
-constexpr int DU_ROWS = 32;  // rows of a workgroup
+// [du | dz] from dh and [u | z]; with SUMS the fp32 column sums of the workgroup's rows.  Memory bound: three reads, two writes.  A thread owns 8 columns and every fourth row of its
+// workgroup's, the next one's loads in flight; without sums that is one row (du_rows()).
 template <bool SUMS>
-__global__ __launch_bounds__(256) void gated_ffn_du_kernel(const bf16_t* dh, long ld_dh, const bf16_t* hg, long ld_hg, bf16_t* du, int M, int F, int act, float* part) {
+__global__ __launch_bounds__(256) void gated_ffn_du_kernel(const bf16_t* dh, long ld_dh, const bf16_t* hg, long ld_hg, bf16_t* du, int M, int F, int act, int rows, float* part) {
   const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8, sub = threadIdx.x >> 6;
-  const int r0 = blockIdx.y * DU_ROWS, r1 = min(M, r0 + DU_ROWS);
+  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
   float sv[8] = {}, sz[8] = {};
-  if (c < F) {
+  if (c < F && r0 + sub < r1) {
+    uint4 dn, un, zn;
+    auto fetch = [&](int m) {
+      dn = *reinterpret_cast<const uint4*>(dh + (long)m * ld_dh + c);
+      un = *reinterpret_cast<const uint4*>(hg + (long)m * ld_hg + c);
+      zn = *reinterpret_cast<const uint4*>(hg + (long)m * ld_hg + F + c);
+    };
+    fetch(r0 + sub);
     for (int m = r0 + sub; m < r1; m += 4) {
-      const uint4 d4 = *reinterpret_cast<const uint4*>(dh + (long)m * ld_dh + c);
-      const uint4 u4 = *reinterpret_cast<const uint4*>(hg + (long)m * ld_hg + c);
-      const uint4 z4 = *reinterpret_cast<const uint4*>(hg + (long)m * ld_hg + F + c);
+      const uint4 d4 = dn, u4 = un, z4 = zn;
+      if (m + 4 < r1) fetch(m + 4);
       const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w}, zw[4] = {z4.x, z4.y, z4.z, z4.w};
       float ov[8], oz[8];
 #pragma unroll
@@ -607,6 +613,11 @@ int launch(K kernel, unsigned grid, unsigned threads, size_t lds, hipStream_t s,
 }
 int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return m <= 0 ? 0 : ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
 
+// Rows of a workgroup that forms [du | dz].  With bias gradients each leaves a row of partial sums: 32 rows to it, 8 while that leaves CUs without work.
+int du_rows(int M, int F, bool db) {
+  if (!db) return M <= 4 * 65535 ? 4 : 32;
+  return (int64_t)((M + 31) / 32) * ((F + 511) / 512) < 256 ? 8 : 32;
+}
 // How a backward pass is cut into workgroups: 256 x 256 tiles (one workgroup per CU) or 128 x 128 (two), and into how many pieces each product's contraction goes.  The time of a
 // plan is estimated from what was measured here: 0.9 us for a stage of a large tile, 0.6 us for one of two small ones side by side, 6 / 3 us for a workgroup's start and end,
 // 8 bytes per element and piece through memory at 4.5 TB/s and 5 us for the launch that joins them; a last round of workgroups is taken as half empty.
@@ -619,10 +630,10 @@ Plan plan(int M, int K, int F, bool dx, int ndw) {
   double best_us = 1e30;
   for (int big = 0; big < 2; ++big) {
     const int b = big ? 256 : 128, slots = big ? 256 : 512;
-    const double stage = big ? 0.9 : 0.6, ends = big ? 6.0 : 3.0;
+    double stage = big ? 0.9 : 0.6, ends = big ? 6.0 : 3.0;
     const double n[2] = {dx ? (double)tiles(M, K, b, b) : 0.0, (double)ndw * tiles(F, K, b, b)};
     const int st[2] = {2 * ((F + BK - 1) / BK), (M + BK - 1) / BK};
-    for (int chunk = 16; chunk <= 16384; chunk += chunk / 2) {
+    for (int chunk = 8; chunk <= 16384; chunk += chunk / 2) {
       int s[2];
       double work = 0, longest = 0, shortest = 1e30, bytes = 0, count = 0;
       for (int i = 0; i < 2; ++i) {
@@ -656,7 +667,8 @@ Layout layout(const Plan& pl, int M, int K, int F, bool dx, bool dwv, bool dwg, 
   Layout l;
   int64_t at = ((int64_t)M * 2 * F * 2 + 255) / 256 * 256;  // [du | dz]
   l.sums = at;
-  if (db) at += ((int64_t)((M + DU_ROWS - 1) / DU_ROWS) * 2 * F * 4 + 255) / 256 * 256;
+  const int rows = du_rows(M, F, db);
+  if (db) at += ((int64_t)((M + rows - 1) / rows) * 2 * F * 4 + 255) / 256 * 256;
   const bool want[3] = {dx, dwv, dwg};
   for (int i = 0; i < 3; ++i) {
     l.part[i] = at;
@@ -711,7 +723,7 @@ extern "C" int64_t aitk_gated_ffn_bwd_workspace_bytes(int32_t M, int32_t K, int3
 }
 
 extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t stream) {
-  if (!q || q->M <= 0 || q->K <= 0 || q->F <= 0 || (q->K % 8) || (q->F % 8) || (q->M + DU_ROWS - 1) / DU_ROWS > 65535) return AITK_ERR_SHAPE;
+  if (!q || q->M <= 0 || q->K <= 0 || q->F <= 0 || (q->K % 8) || (q->F % 8) || q->M > 32 * 65535) return AITK_ERR_SHAPE;
   const bool dw = q->dw_val || q->dw_gate, db = q->db_val || q->db_gate;
   if (!q->dh || !q->hg || !q->ws || q->act < 0 || q->act > 2 || (q->dx && (!q->w_val || !q->w_gate)) || (dw && !q->x)) return AITK_ERR_ARG;
   if (bad(q->dh, q->ld_dh, q->F) || bad(q->hg, q->ld_hg, 2 * (int64_t)q->F) || mis16(q->ws) || (q->dx && (bad(q->dx, q->ld_dx, q->K) || bad(q->w_val, q->ldw, q->K) || mis16(q->w_gate))) ||
@@ -725,10 +737,10 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
   bf16_t* du = reinterpret_cast<bf16_t*>(ws);
   float* part = reinterpret_cast<float*>(ws + l.sums);
   hipStream_t s = (hipStream_t)stream;
-  const int nchunk = (M + DU_ROWS - 1) / DU_ROWS;
+  const int rows = du_rows(M, F, db), nchunk = (M + rows - 1) / rows;
   const dim3 grid((F / 8 + 63) / 64, nchunk);
-  if (db) hipLaunchKernelGGL(gated_ffn_du_kernel<true>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, part);
-  else hipLaunchKernelGGL(gated_ffn_du_kernel<false>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, part);
+  if (db) hipLaunchKernelGGL(gated_ffn_du_kernel<true>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, rows, part);
+  else hipLaunchKernelGGL(gated_ffn_du_kernel<false>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, rows, part);
   AITK_LAUNCH_CHECK();
   if (db) {
     hipLaunchKernelGGL(gated_ffn_db_kernel, dim3((F + 63) / 64, 2), dim3(256), 0, s, part, nchunk, F, q->db_val, q->db_gate);
