@@ -384,22 +384,72 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
 
 // ============================================================================================ backward
 // delta[q] = dO[q].o[q], and minus the row statistic, -inf for rows without a key (2^(s - inf) = 0: their probabilities vanish).  A wave takes 8 rows of one head.
+// o has been rounded to bf16, so delta is off by up to 2^-8 |dO||o|, and ds = p (dp - delta) by p times that.  Over many keys that is small next to the rounding of ds; over a few, |o| is as large
+// as |v|, dp - delta may be small, and the gradients of two keys were off by 2 % in the worst of a few heads.  Samples of 2 to FEW keys therefore get delta as the sum of p dp (of one key
+// o = v needs no rounding).
+constexpr int FEW = 16;
 __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
+  __shared__ int keys[FEW];
+  __shared__ float bias[32][FEW + 1];
   const AitkAttnRelposArgs& a = r.a;
-  const int s = blockIdx.x * 32 + (threadIdx.x >> 3), hd = blockIdx.y, b = blockIdx.z, c = (threadIdx.x & 7) * 8;
-  if (s >= a.S) return;
-  const long row = (long)b * a.S + s;
+  const int tid = threadIdx.x, lane = tid & 63, S = a.S, s0 = blockIdx.x * 32, s = min(s0 + (tid >> 3), S - 1), hd = blockIdx.y, b = blockIdx.z, c = (tid & 7) * 8;
+  const long row = (long)b * S + s, i = ((long)b * a.H + hd) * S + s;
   const uint4 x = *reinterpret_cast<const uint4*>(a.O + row * a.ldo + hd * 64 + c);
   const uint4 y = *reinterpret_cast<const uint4*>(a.dO + row * a.lddo + hd * 64 + c);
-  float v = bf_lo(x.x) * bf_lo(y.x) + bf_hi(x.x) * bf_hi(y.x) + bf_lo(x.y) * bf_lo(y.y) + bf_hi(x.y) * bf_hi(y.y) + bf_lo(x.z) * bf_lo(y.z) +
-            bf_hi(x.z) * bf_hi(y.z) + bf_lo(x.w) * bf_lo(y.w) + bf_hi(x.w) * bf_hi(y.w);
+  const float lse = a.LSE[i];
+  const auto dot = [](const uint4& u, const uint4& w) {
+    return bf_lo(u.x) * bf_lo(w.x) + bf_hi(u.x) * bf_hi(w.x) + bf_lo(u.y) * bf_lo(w.y) + bf_hi(u.y) * bf_hi(w.y) + bf_lo(u.z) * bf_lo(w.z) + bf_hi(u.z) * bf_hi(w.z) +
+           bf_lo(u.w) * bf_lo(w.w) + bf_hi(u.w) * bf_hi(w.w);
+  };
+  const uint8_t* const mask = a.key_mask ? a.key_mask + (long)b * S : nullptr;
+  const auto kept = [&](int k0) { return __ballot(k0 + lane < S && (!mask || mask[k0 + lane < S ? k0 + lane : 0] != 0)); };
+  int n = mask ? 0 : S;
+  if (mask)
+    for (int k0 = 0; k0 < S && n <= FEW; k0 += 64) n += __popcll(kept(k0));
+  float v;
+  if (n > FEW || n <= 1) {
+    v = dot(x, y);
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  if (c == 0) {
-    const long i = ((long)b * a.H + hd) * a.S + s;
-    const float l = a.LSE[i];
+    for (int o = 4; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  } else {
+    if (tid < 64)
+      for (int k0 = 0, at = 0; k0 < S; k0 += 64) {
+        const unsigned long long bits = kept(k0);
+        if ((bits >> lane) & 1) keys[at + __popcll(bits & ((1ull << lane) - 1))] = k0 + lane;
+        at += __popcll(bits);
+      }
+    __syncthreads();
+    if (a.table) {
+      for (int p = tid; p < 32 * n; p += 256) {
+        const int q = p / n, d = keys[p - q * n] - (s0 + q), m = d > 0 ? (a.causal ? 0 : d) : -d;
+        int lo = 0, hi = r.half;  // the last bucket whose first distance is at most m
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (r.first[mid] <= m) lo = mid;
+          else hi = mid;
+        }
+        bias[q][p - q * n] = bf2f(a.table[(long)(lo + (d > 0 && !a.causal ? r.half : 0)) * a.H + hd]) * 1.4426950408889634f;
+      }
+      __syncthreads();
+    }
+    const uint4 qv = *reinterpret_cast<const uint4*>(a.Q + row * a.ldq + hd * 64 + c);
+    v = 0.f;
+    for (int k = 0; k < n; ++k) {
+      const long kr = (long)b * S + keys[k];
+      float sc = dot(qv, *reinterpret_cast<const uint4*>(a.K + kr * a.ldk + hd * 64 + c)), dp = dot(y, *reinterpret_cast<const uint4*>(a.V + kr * a.ldv + hd * 64 + c));
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        sc += __shfl_xor(sc, o, 64);
+        dp += __shfl_xor(dp, o, 64);
+      }
+      sc *= a.scale * 1.4426950408889634f;
+      if (a.table) sc += bias[tid >> 3][k];
+      if (lse != -INFINITY && !(a.causal && keys[k] > s)) v += __builtin_amdgcn_exp2f(sc - lse) * dp;
+    }
+  }
+  if (c == 0 && s0 + (tid >> 3) < S) {
     r.delta[i] = v;
-    r.delta[(long)a.B * a.H * a.S + i] = l == -INFINITY ? -INFINITY : -l;
+    r.delta[(long)a.B * a.H * S + i] = lse == -INFINITY ? -INFINITY : -lse;
   }
 }
 

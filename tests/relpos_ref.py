@@ -33,8 +33,8 @@ def bucket_index(S, num_buckets, max_distance, causal, device):
     return j if causal else j + (rel > 0).long() * half
 
 
-def attention(q, k, v, table, *, B, H, S, scale, key_mask, max_distance, causal, do=None):
-    """dict of float64 results and tolerances ([B*S, H*64] layout); `do` adds the gradients"""
+def attention(q, k, v, table, *, B, H, S, scale, key_mask, max_distance, causal, do=None, delta_from_o=True):
+    """dict of float64 results and tolerances ([B*S, H*64] layout); `do` adds the gradients; delta_from_o=False: delta is not formed from the rounded o"""
     split = lambda t: t.double().reshape(B, S, H, 64).transpose(1, 2).contiguous()  # noqa: E731
     join = lambda t: t.transpose(1, 2).reshape(B * S, H * 64)  # noqa: E731
     q, k, v = split(q), split(k), split(v)
@@ -69,7 +69,7 @@ def attention(q, k, v, table, *, B, H, S, scale, key_mask, max_distance, causal,
     vt = v.transpose(2, 3).contiguous()
     dp, delta = torch.matmul(do, vt), (do * o).sum(3, keepdim=True)
     ds = p * (dp - delta)
-    raw = p * ((do.abs() * tol_o).sum(3, keepdim=True) + FP * (torch.matmul(do.abs(), vt.abs()) + (do * o).abs().sum(3, keepdim=True)))
+    raw = p * (float(delta_from_o) * (do.abs() * tol_o).sum(3, keepdim=True) + FP * (torch.matmul(do.abs(), vt.abs()) + (do * o).abs().sum(3, keepdim=True)))
     err = raw + U * ds.abs()
     dq, dk = torch.matmul(ds, k) * scale, torch.matmul(ds.transpose(2, 3).contiguous(), q) * scale
     r["dq"], r["tol_dq"] = join(dq), join(torch.matmul(err, k.abs()) * scale + (U + FP) * dq.abs())

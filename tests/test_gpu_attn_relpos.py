@@ -115,6 +115,35 @@ def test_bucketings(buckets, max_distance, causal):
     _run(1, 2, 700, buckets=buckets, max_distance=max_distance, causal=causal)
 
 
+@pytest.mark.parametrize("causal,bias", [(False, True), (True, True), (False, False)])
+@pytest.mark.parametrize("S,keys", [(2, 2), (3, 3), (5, 5), (16, 16), (40, 1), (300, 2), (300, 9), (1100, 16), (1, 1)])
+def test_few_keys_have_exact_deltas(S, keys, causal, bias):
+    """where a sample keeps at most 16 keys, the rounding of o does not reach the gradients"""
+    from ai_toolkit_amd import ops
+
+    for seed in range(4):
+        B, H = (1, 1) if seed < 2 else (2, 3)
+        q, k, v, table, o, do, dq, dk, dv = _inputs(B, H, S, seed=seed + 10 * S, layout="pitched" if seed % 2 else "fused")
+        table = table if bias else None
+        mask = None
+        if keys < S:
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            mask = torch.zeros(B, S, dtype=torch.bool, device="cuda")
+            for b in range(B):
+                mask[b, torch.randperm(S, generator=g, device="cuda")[:keys]] = True
+        kw = dict(B=B, H=H, S=S, scale=1.0, key_mask=mask, max_distance=128, causal=causal)
+        want = ref.attention(q, k, v, table, do=do, delta_from_o=False, **kw)
+        lse = torch.zeros(B, H, S, device="cuda")
+        ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+        dtable = torch.empty(32, H, device="cuda") if bias else None
+        ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable, **kw)
+        torch.cuda.synchronize()
+        for name, t in (("dv", dv), ("dq", dq), ("dk", dk)):
+            assert ((t.double() - want[name]).abs() <= want["tol_" + name] + 1e-30).all(), (name, seed)
+        if bias:
+            assert ((dtable.double() - want["dtable"]).abs() <= want["tol_dtable"] * (1 + ref.U) + 1e-30).all(), seed
+
+
 @pytest.mark.parametrize("value", [float("-inf"), torch.finfo(BF16).min])
 @pytest.mark.parametrize("S", [64, 200, 333])
 def test_table_entries_that_forbid_a_bucket(value, S):
