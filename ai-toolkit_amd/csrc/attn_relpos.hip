@@ -14,6 +14,10 @@
 //
 // Tiles are [64 rows][64 columns] bf16, 128-byte rows, filled by LDS-DMA; physical 16-byte chunk = chunk ^ rkey(row).  The key makes both ways the tile is read free of bank
 // conflicts: b128 row fragments (eight row pairs meet eight different chunks) and 16-bit transpose reads (four rows x 64 bytes fill all 64 banks: bit 2 of the key is bit 1 of the row).
+//
+// Measured (32 heads x 2048, no mask): forward 58 us = 0.59 PFLOP/s, backward 160 us = 0.75 PFLOP/s over the seven products it forms, and 5.5 + 4.6 us for delta and the table's sums.
+// Bound by the issue of vector instructions: 64-wide heads give the matrix units 12 to 16 products per 32 x 32 scores, the exponentials, masks and sums take as long again (backward: matrix
+// units busy 39 % of the cycles, vector instructions 54 %, both at once 16 %).  The small launches are bound by the steps' latency: 64 heads x 512 15 us, 2 x 12 x 77 5.2 us, of them 3 for the launch.
 #include "common.h"
 #include "aitk_args.h"
 
@@ -203,7 +207,7 @@ __device__ __forceinline__ void fetch(lds_char* dst, const TileLane& L, long lda
 }
 // workgroup -> (row tile, head, sample): the tiles of one (head, sample) stay on one XCD, whose L2 then holds their slices (block i runs on XCD i % 8), and an XCD gets all the
 // samples of its heads: with a key mask the samples differ in length, and whole samples per XCD left the XCDs of the
-// short ones idle (4 x 64 heads x 512 with lengths 24 .. 512: backward 126 -> 105 us, forward 37 -> 32 us)
+// short ones idle (4 x 64 heads x 512 with lengths 24 .. 512: a sixth of the backward, an eighth of the forward)
 __device__ __forceinline__ void wg_coords(int ntiles, int B, int& tile, int& hd, int& b) {
   const int n = gridDim.x, id = blockIdx.x, x = id & 7, per = n >> 3, rem = n & 7;
   const int l = x * per + min(x, rem) + (id >> 3);
@@ -215,8 +219,8 @@ __device__ __forceinline__ void wg_coords(int ntiles, int B, int& tile, int& hd,
 // ============================================================================================ forward
 // 4 waves, key tiles of 64 in a double buffer.  S^T = K Q^T: a lane owns one query row, so the statistics are per-lane scalars and P^T feeds the next product straight from
 // the registers.  KVS = 1: 128 query rows, every wave walks all key tiles.  KVS = 2: 64 query rows, two waves share 32 of them and take every other key tile; their
-// (maximum, sum, output) meet in LDS at the end.  For launches of at most one 128-row workgroup per CU: twice the workgroups, half the steps (1 x 64 heads x 512: 18.0 -> 15.7 us,
-// 3 x 6 x 333: 13.7 -> 11.3 us; with two workgroups per CU it loses: 1 x 32 x 2048 61.7 -> 71.5 us).
+// (maximum, sum, output) meet in LDS at the end.  For launches of at most one 128-row workgroup per CU: twice the workgroups, half the steps (1 x 64 heads x 512: 15.6 -> 15.0 us,
+// 3 x 6 x 333: 12.5 -> 10.3, 2 x 12 x 77: 6.0 -> 5.2; with two workgroups per CU it loses: 1 x 32 x 2048 57.7 -> 70.2 us).
 template <bool BIAS, bool CAUSAL, int KVS>
 __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -488,8 +492,8 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   const int E = r.sat + BAND_PAD, n_line = 2 * E + 1;
   const bool sums = BIAS && a.dtable != nullptr;
   // Bucket sums.  The diagonals of a 32 x 32 block (one relative position each) become columns of a wave-private LDS patch, eight query rows at a time: row q is written q mod 8
-  // places to the left (with up to three places of slack so that its 16-byte stores are aligned; what a row never writes stays zero), a lane then adds up one column and
-  // joins it to the wave's accumulator of that distance.  Fixed order, no atomics (an LDS float add per element: 330 us for 4 x 64 heads x 512 against 137 us).  Eight rows and not all 32: the
+  // places to the left (with up to three places of slack so that its 16-byte stores are aligned; what a row never writes stays zero), a lane then adds up the column of its diagonal, and
+  // after all four times eight rows joins the sum to the wave's accumulator of that distance.  Fixed order, no atomics (an LDS float add per element took the launch 2.4 times as long).  Eight rows and not all 32: the
   // workgroup's LDS then lets three of them share a CU.
   lds_float* const acc = line + 4 * r.line_p + wave * n_line;
   lds_float* const skew = line + 4 * r.line_p + (4 * n_line + 3) / 4 * 4 + wave * (8 * SKEW_P);

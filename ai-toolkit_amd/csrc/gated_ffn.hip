@@ -11,6 +11,11 @@
 // K tails outside the buffer arrive as zeros), 16-byte chunks XOR-swizzled so that no read meets a bank twice.  An operand whose contraction index is contiguous in memory is
 // read as 16-byte row fragments; one whose contraction index is the ROW (W in dx; du and x in dW) lies in blocks of 64 columns and is read with 16-bit transpose reads: no
 // transposed copy of a weight or an activation exists anywhere.
+//
+// Measured: 2048 x 4096 x 10240 forward with hg 325 us = 1.06 PFLOP/s, all three gradients 600 - 720 us = 1.15 - 0.95 PFLOP/s as the card's power allows (the library's plain products of these
+// sizes: 371 and about 650 us), du 32 us = 6.5 TB/s (half of it still cached); 512 x 4096 x 10240 forward 92 - 102 us = 0.93 - 0.84 PFLOP/s on 160 of the 256 CUs; 4096 x 640 x 2560 forward with
+// hg and biases 50 us, all gradients 106 us; 1 x 4096 x 10240 32 us = 5.2 TB/s of weights.  The tile loop is bound by the power of the matrix units: 0.53 us (160 CUs) to 0.63 us (256) a stage of a
+// 256 x 256 tile with nothing but its matrix instructions, 0.66 to 0.82 as it is.
 #include "common.h"
 #include "aitk_args.h"
 
@@ -41,7 +46,7 @@ struct FfnArgs {
 
 // The normal distribution's Phi(z), and e = exp(-z^2 / 2), for the erf GELU: Phi(-x) = e P(1 / (1 + x / 4)) for x >= 0, where P is a polynomial of degree 7 fitted here to
 // exp(x^2 / 2) Phi(-x) (relative error 1.6e-7 up to x = 10, where Phi(-x) = 8e-24; with the roundings below 1e-6 up to 3, 5e-6 up to 10).  One exp and one reciprocal, where the library's erff has two
-// branches that a wave takes both (4096 x 640 x 2560 forward 57 us with it, 47 us so).
+// branches that a wave takes both (4096 x 640 x 2560 forward 57 us with it, 53 us so, both with the tiles of that time).
 __device__ __forceinline__ float phi_f(float z, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.25f, fabsf(z), 1.0f));
   e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
