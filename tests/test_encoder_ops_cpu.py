@@ -75,7 +75,7 @@ def test_c_norm_refusals():
     assert lib.aitk_norm_bwd(C.byref(b), None) == ARG  # gradients without scratch
     b.dweight, b.dres, b.ld_dres = None, 64, 32
     assert lib.aitk_norm_bwd(C.byref(b), None) == ALIGN
-    assert lib.aitk_norm_bwd_workspace_bytes(0, 64, 0) == 0 and lib.aitk_norm_bwd_workspace_bytes(1, 64, 0) == 2 * 64 * 4
+    assert lib.aitk_norm_bwd_workspace_bytes(0, 64, 0) == 0 and lib.aitk_norm_bwd_workspace_bytes(1, 64, 0) >= 2 * 64 * 4
 
 
 def _attn_args():
