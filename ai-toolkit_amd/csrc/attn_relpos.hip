@@ -38,7 +38,7 @@ struct RelposArgs {
   int half, sat, line_p;        // buckets per sign, first distance of the last one, floats per shifted copy of the line
   int tiles;                    // backward: row tiles of a workgroup's height
   int first[MAX_HALF];          // first distance of every bucket of one sign
-  float* delta;                 // backward: [2][B][H][S]: dO.o, and -lse (-inf for rows without a key)
+  float* delta;                 // backward: [2][B][H][S]: -dO.o, and -lse (-inf for rows without a key)
   float* part;                  // backward: [B * row tiles][H][num_buckets] bucket sums
 };
 
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
 }
 
 // ============================================================================================ backward
-// delta[q] = dO[q].o[q], and minus the row statistic, -inf for rows without a key (2^(s - inf) = 0: their probabilities vanish).  A wave takes 8 rows of one head.
+// Minus delta[q] = dO[q].o[q], and minus the row statistic, -inf for rows without a key (2^(s - inf) = 0: their probabilities vanish).  A wave takes 8 rows of one head.
 // o has been rounded to bf16, so delta is off by up to 2^-8 |dO||o|, and ds = p (dp - delta) by p times that.  Over many keys that is small next to the rounding of ds; over a few, |o| is as large
 // as |v|, dp - delta may be small, and the gradients of two keys were off by 2 % in the worst of a few heads.  Samples of 2 to FEW keys therefore get delta as the sum of p dp (of one key
 // o = v needs no rounding).
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
     }
   }
   if (c == 0 && s0 + (tid >> 3) < S) {
-    r.delta[i] = v;
+    r.delta[i] = -v;
     r.delta[(long)a.B * a.H * S + i] = lse == -INFINITY ? -INFINITY : -lse;
   }
 }
@@ -486,7 +486,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
     }
   }
   const long stat = ((long)b * a.H + hd) * S + qc;
-  const float delta = r.delta[stat];
+  const float delta = -r.delta[stat];
   const float l2 = live ? -r.delta[(long)a.B * a.H * S + stat] : INFINITY;  // rows past the end: p = 0, ds = 0
   const float c2 = a.scale * 1.4426950408889634f;
   const int E = r.sat + BAND_PAD, n_line = 2 * E + 1;
@@ -680,7 +680,7 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
   const AitkAttnRelposArgs& a = r.a;
   constexpr int ROWS = 128 / KVS, STEP = 2 * KVS * TILE;
   lds_char* const sm = (lds_char*)smem;                                // 2 x KVS x (Q tile, dO tile)
-  lds_float* const st = (lds_float*)(smem + 2 * STEP);                 // 2 x KVS x (64 -lse, 64 delta)
+  lds_float* const st = (lds_float*)(smem + 2 * STEP);                 // 2 x KVS x (64 -lse, 64 -delta)
   lds_float* const line = (lds_float*)(smem + 2 * STEP + KVS * 1024);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5, S = a.S;
@@ -743,7 +743,13 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
         const float far = past ? far_past : ahead ? far_ahead : 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          f32x16_t s, dp = zero16();
+          f32x16_t s, dp;  // dp starts from -delta: a subtraction per element less (32 x 2048: 1.5 % of the launch)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4_t nd = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(row + 64 + 32 * j + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * g + e] = nd[e];
+          }
           if (BIAS && !past && !ahead) {
             s = load_line(line, r.line_p, ib + qt0 + 32 * j);
           } else {
@@ -759,13 +765,12 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const f32x4_t nl = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(row + 32 * j + 8 * g + 4 * h);
-            const f32x4_t de = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(row + 64 + 32 * j + 8 * g + 4 * h);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], c2, nl[e]));
               if (CAUSAL && qt0 + 32 * j + 8 * g + 4 * h + e < key) p = 0.f;
               s[4 * g + e] = p;
-              dp[4 * g + e] = p * (dp[4 * g + e] - de[e]);
+              dp[4 * g + e] *= p;
             }
           }
 #pragma unroll
