@@ -124,3 +124,60 @@ def test_two_trained_layers(kind, B, H, F, S):
     for i, (a, b) in enumerate(zip(grads, wgrads)):
         for n in a:
             near(a[n], b[n], f"layer {i} {n}")
+
+
+def _flat(r):
+    out, dx, dtable, grads = r
+    return [out, dx] + ([] if dtable is None else [dtable]) + [t for g in grads for _, t in sorted(g.items())]
+
+
+@pytest.mark.parametrize("kind,B,H,F,S", [("t5", 2, 4, 640, 150), ("clip", 3, 2, 512, 77)])
+def test_two_trained_layers_in_a_replayed_graph(kind, B, H, F, S):
+    """captured once, replayed with other inputs in the captured tensors and eager passes between the replays: every replay gives the eager result, bit for bit"""
+    layers, table = _weights(kind, H, F, seed=S)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    inputs = [tuple(torch.randn(B * S, H * 64, generator=g, device="cuda").to(BF16) for _ in range(2)) for _ in range(3)]
+    mask = torch.arange(S, device="cuda")[None] < torch.tensor([S - 7 * b - 3 for b in range(B)], device="cuda")[:, None] if kind == "t5" else None
+    kw = dict(kind=kind, B=B, H=H, S=S)
+    want = [[t.clone() for t in _flat(_native(x, layers, table, d, mask, **kw))] for x, d in inputs]
+    x, dout = (t.clone() for t in inputs[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _flat(_native(x, layers, table, dout, mask, **kw))
+    for n in (1, 0, 2, 1):
+        x.copy_(inputs[n][0])
+        dout.copy_(inputs[n][1])
+        for t in got:
+            t.fill_(3.0)
+        graph.replay()
+        _native(*inputs[2][:1], layers, table, inputs[2][1], mask, **kw)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[n])), n
+
+
+def test_two_trained_layers_from_recorded_launch_lists():
+    """recorded while nothing runs, launched later beside another list: the eager results, scratch and operands alive until then"""
+    from ai_toolkit_amd import ops
+
+    kind, B, H, F, S = "t5", 2, 4, 640, 150
+    kw = dict(kind=kind, B=B, H=H, S=S)
+    sets = []
+    for seed in (1, 2):
+        layers, table = _weights(kind, H, F, seed=seed)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x, dout = (torch.randn(B * S, H * 64, generator=g, device="cuda").to(BF16) for _ in range(2))
+        sets.append((x, layers, table, dout, None))
+    want = [[t.clone() for t in _flat(_native(*a, **kw))] for a in sets]
+    lists, got = [], []
+    for a in sets:
+        with ops.recording() as launches:
+            got.append(_flat(_native(*a, **kw)))
+        lists.append(launches)
+    for r in got:
+        for t in r:
+            t.fill_(3.0)
+    ops.replay_paired(*lists)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
