@@ -170,7 +170,7 @@ struct TileLoop {
   typedef Operand<BM, NT, AK, false> OpA;
   typedef Operand<BN, NT, BKC, PAIR> OpB;
   static constexpr int STAGE = OpA::BYTES + OpB::BYTES, DMAS = OpA::NDMA + OpB::NDMA;
-  static_assert((DMAS == 3 || DMAS == 4) && NB % 2 == 0, "the counted waits below; stores of pairs of blocks");
+  static_assert(DMAS >= 2 && DMAS <= 4 && NB % 2 == 0, "the counted waits below; stores of pairs of blocks");
   f32x16_t acc[MB][NB];
   // a wave's j-th block of 32 columns within the tile: neighbours where a store joins two of them; otherwise one of either half of the tile (4096 x 640 x 2560, both gradients: 83 us
   // with neighbours, 80 us so)
@@ -253,10 +253,12 @@ struct TileLoop {
     auto landed = [&](int n) {
       if (n >= 2) {
         if constexpr (DMAS == 4) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        else if constexpr (DMAS == 3) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
       } else if (n == 1) {
         if constexpr (DMAS == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
+        else if constexpr (DMAS == 3) asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
       } else {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       }
@@ -700,10 +702,10 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   hipStream_t s = (hipStream_t)stream;
   const int64_t big = tiles(q->M, q->F, 256, 128), small = tiles(q->M, q->F, 128, 64);
   if (small > 0x7fffffff) return AITK_ERR_SHAPE;
-  // Few rows: blocks of 16 TB rows x strips of 16 columns, as long as a strip's work is short.  16 or 32 rows to a workgroup while every one of them has a CU to itself, 64 while two share
-  // one (us with 16 / 32 / 64 rows / tiles: 512 x 1024 64 rows 4.8 / 5.4 / 6.6 / 11, 128 rows 6.0 / 5.5 / 6.7 / 11, 256 rows 8.8 / 7.2 / 6.9 / 11; 4096 x 512 128 rows 14 / 18 / 25 / 47;
-  // 4096 x 4096 64 rows 47 / 33 / 26 / 47, 128 rows 91 / 61 / 49 / 48; 768 x 2048 256 rows - / 14.3 / 13.2 / 14.0, 512 rows - / 25 / 23 / 14), and up to 32 rows always: then the weights' way bounds every
-  // form (4096 x 10240: 16 rows 36 us against 48 of the tiles, 32 rows 45).
+  // Few rows: blocks of 16 TB rows x strips of 16 columns, as long as a strip's work is short.  16 or 32 rows to a workgroup while every one of them has a CU to itself, 64 up to one and a
+  // half per CU (us with 16 / 32 / 64 rows / tiles: 512 x 1024 64 rows 4.8 / 5.4 / 6.6 / 10, 128 rows 6.0 / 5.5 / 6.7 / 10, 256 rows 8.8 / 7.2 / 6.9 / 10; 4096 x 512 128 rows 14 / 18 / 25 / 42;
+  // 768 x 2048 150 rows - / 11.2 / 11.6 / 12.4, 256 rows - / 14.3 / 13.2 / 12.5; 4096 x 4096 64 rows 47 / 33 / 26 / 44), and up to 32 rows always: then the weights' way bounds every form
+  // (4096 x 10240: 16 rows 36 us against 45 of the tiles, 32 rows 45).
   const int64_t strips = (q->F + 15) / 16;
   const auto blocks = [&](int tb) { return (q->M + 16 * tb - 1) / (16 * tb); };
   const auto few = [&](auto kernel, int tb) {
@@ -713,11 +715,12 @@ extern "C" int aitk_gated_ffn_fwd(const AitkGatedFfnArgs* q, aitk_stream_t strea
   };
   if (q->M <= 16 || strips * blocks(1) <= 256) return few(gated_ffn_few_kernel<1>, 1);
   if (q->M <= 32 || strips * blocks(2) <= 256) return few(gated_ffn_few_kernel<2>, 2);
-  if (strips * blocks(4) <= 512) return few(gated_ffn_few_kernel<4>, 4);
-  // Large tiles (one workgroup per CU), the last round in halves if they all find a CU; 128 x 128 tiles (two workgroups per CU) only while every one of them has a CU to itself.  Large
-  // with halves / large / small, us: 4096 x 640 x 2560 (320 tiles) 44 / 50 / 50; 2048 x 4096 x 10240 (640) 301 / 316 / 397; 512 x 4096 x 10240 (160) 92 / 92 / 120; 1024 x 640 x 2560
-  // (80 large, 320 small) 17.2 / 24 / 17.7; 1000 x 768 x 2048 (64, 256) 17.6 / 25 / 16.1; 77 x 4096 x 10240 (80, 160) 58 / 84 / 48.
-  if (small <= 256) return launch(gated_ffn_fwd_kernel<128, 128, 2, 2>, (unsigned)small, 256, NST * 256 * BK * 2, s, a, (int)small);
+  if (strips * blocks(4) <= 384) return few(gated_ffn_few_kernel<4>, 4);
+  // Large tiles (one workgroup per CU), the last round in halves if they all find a CU; 128 x 128 tiles only while every one of them has a CU to itself, and then of eight waves (32 x 64 each): two
+  // to a SIMD hide each other's waits (four waves of 64 x 64: 512 x 1024 1000 rows 12.8 us, eight 11.4).  Large with halves / large / small, us: 4096 x 640 x 2560 (320 tiles) 44 / 50 / 50;
+  // 2048 x 4096 x 10240 (640) 301 / 316 / 397; 512 x 4096 x 10240 (160) 92 / 92 / 120; 1024 x 640 x 2560 (80 large, 320 small) 17.2 / 24 / 17.7; 1000 x 768 x 2048 (64, 256) 17.6 / 25 / 14.4;
+  // 77 x 4096 x 10240 (80, 160) 58 / 84 / 45.
+  if (small <= 256) return launch(gated_ffn_fwd_kernel<128, 128, 4, 2>, (unsigned)small, 512, NST * 256 * BK * 2, s, a, (int)small);
   const int64_t rest = big % 256, halves = rest <= 128 ? rest : 0;
   return launch(gated_ffn_fwd_kernel<256, 256, 2, 4>, (unsigned)(big + halves), 512, NST * 512 * BK * 2, s, a, (int)(big - halves));
 }
