@@ -140,26 +140,27 @@ __device__ __forceinline__ f32x16_t load_line(const lds_float* line, int line_p,
 }
 
 // The four shifted copies of the line: copy c, entry i = the bias of distance sign * (i + c - E), divided by the softmax scale (it joins the scores before they are multiplied by
-// it).  Eight lanes to a bucket walk its distances: one load of the table per lane, where a search of the bucket per distance cost every workgroup 1 us more.  Causal: what lies ahead
-// is masked and takes bucket 0.
+// it).  Eight lanes walk a bucket's distances, all threads those of the last ones (half the line): one load of the table each, where a search of the bucket per distance cost every workgroup
+// 1 us more, and eight lanes to the last bucket another.  Causal: what lies ahead is masked and takes bucket 0.
 __device__ __forceinline__ void build_line(lds_float* line, const RelposArgs& r, int hd, int sign) {
-  const int E = r.sat + BAND_PAD;
+  const int E = r.sat + BAND_PAD, H = r.a.H, narrow = r.half - 1;
   const float inv = 1.0f / r.a.scale;
   const bool causal = r.a.causal != 0;
-  for (int i = threadIdx.x; i < (causal ? r.half + 1 : 2 * r.half) * 8; i += 256) {
-    const int k = i >> 3;
-    const bool ahead = k >= r.half;
-    const int j = ahead ? (causal ? 0 : k - r.half) : k;
-    const float b = bf2f(r.a.table[(long)(causal ? j : k) * r.a.H + hd]) * inv;
-    const int n0 = j || !ahead ? r.first[j] : 1, n1 = j == r.half - 1 || (causal && ahead) ? E + 1 : r.first[j + 1];
-    const int dir = ahead == (sign > 0) ? 1 : -1;
-    for (int n = n0 + (i & 7); n < n1; n += 8) {
-      const int at = E + dir * n;
+  const float past = bf2f(r.a.table[(long)narrow * H + hd]) * inv, next = bf2f(r.a.table[(causal ? 0 : (long)(r.half + narrow) * H) + hd]) * inv;
+  const auto put = [&](int d, float b) {  // a place in front of a copy is padding of the copy before (line_p >= 2 E + 6)
+    lds_float* const at = line + E + sign * d;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (at - c >= 0) line[c * r.line_p + at - c] = b;
-    }
+    for (int c = 0; c < 4; ++c) at[c * (r.line_p - 1)] = b;
+  };
+  for (int i = threadIdx.x; i < (causal ? 1 : 2) * narrow * 8; i += 256) {
+    const int k = i >> 3;
+    const bool ahead = k >= narrow;
+    const int j = ahead ? k - narrow : k, n1 = r.first[j + 1];
+    const float b = bf2f(r.a.table[(long)(ahead ? r.half + j : j) * H + hd]) * inv;
+    for (int n = (j || !ahead ? r.first[j] : 1) + (i & 7); n < n1; n += 8) put(ahead ? n : -n, b);
   }
+  for (int n = r.sat + threadIdx.x; n <= E; n += 256) put(-n, past);
+  for (int n = (causal ? 1 : r.sat) + threadIdx.x; n <= E; n += 256) put(n, next);
 }
 // keep-bits of 64 key tiles [t0, t0 + 64) of one sample: lane t gets tile t0 + t.  `box`: 64 x 8 bytes of LDS, rewritten here; ends behind a barrier.
 __device__ __forceinline__ unsigned long long tile_masks(const AitkAttnRelposArgs& a, int b, int t0, int nt, unsigned long long* box, int lane, int wave) {
@@ -438,17 +439,32 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
     }
     const uint4 qv = *reinterpret_cast<const uint4*>(a.Q + row * a.ldq + hd * 64 + c);
     v = 0.f;
-    for (int k = 0; k < n; ++k) {
-      const long kr = (long)b * S + keys[k];
-      float sc = dot(qv, *reinterpret_cast<const uint4*>(a.K + kr * a.ldk + hd * 64 + c)), dp = dot(y, *reinterpret_cast<const uint4*>(a.V + kr * a.ldv + hd * 64 + c));
+    constexpr int U = 2;  // keys in flight
+    for (int k0 = 0; k0 < n; k0 += U) {
+      float sc[U], dp[U];
+      uint4 kv[U], vv[U];
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        sc += __shfl_xor(sc, o, 64);
-        dp += __shfl_xor(dp, o, 64);
+      for (int u = 0; u < U; ++u) {
+        const long kr = (long)b * S + keys[min(k0 + u, n - 1)];
+        kv[u] = *reinterpret_cast<const uint4*>(a.K + kr * a.ldk + hd * 64 + c);
+        vv[u] = *reinterpret_cast<const uint4*>(a.V + kr * a.ldv + hd * 64 + c);
       }
-      sc *= a.scale * 1.4426950408889634f;
-      if (a.table) sc += bias[tid >> 3][k];
-      if (lse != -INFINITY && !(a.causal && keys[k] > s)) v += __builtin_amdgcn_exp2f(sc - lse) * dp;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        sc[u] = dot(qv, kv[u]);
+        dp[u] = dot(y, vv[u]);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+          sc[u] += __shfl_xor(sc[u], o, 64);
+          dp[u] += __shfl_xor(dp[u], o, 64);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = min(k0 + u, n - 1);
+        const float x2 = fmaf(sc[u], a.scale * 1.4426950408889634f, a.table ? bias[tid >> 3][k] : 0.f);
+        if (k0 + u < n && lse != -INFINITY && !(a.causal && keys[k] > s)) v += __builtin_amdgcn_exp2f(x2 - lse) * dp[u];
+      }
     }
   }
   if (c == 0 && s0 + (tid >> 3) < S) {
