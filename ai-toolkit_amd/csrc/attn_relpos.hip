@@ -219,9 +219,10 @@ __device__ __forceinline__ void wg_coords(int ntiles, int B, int& tile, int& hd,
 
 // ============================================================================================ forward
 // 4 waves, key tiles of 64 in a double buffer.  S^T = K Q^T: a lane owns one query row, so the statistics are per-lane scalars and P^T feeds the next product straight from
-// the registers.  KVS = 1: 128 query rows, every wave walks all key tiles.  KVS = 2: 64 query rows, two waves share 32 of them and take every other key tile; their
-// (maximum, sum, output) meet in LDS at the end.  For launches of at most one 128-row workgroup per CU: twice the workgroups, half the steps (1 x 64 heads x 512: 15.6 -> 15.0 us,
-// 3 x 6 x 333: 12.5 -> 10.3, 2 x 12 x 77: 6.0 -> 5.2; with two workgroups per CU it loses: 1 x 32 x 2048 57.7 -> 70.2 us).
+// the registers.  KVS = 1: 128 query rows, every wave walks all key tiles.  KVS = 2 (4): 64 (32) query rows, two (four) waves share 32 of them and take every second (fourth) key tile; their
+// (maximum, sum, output) meet in LDS at the end.  More workgroups, fewer steps: KVS = 2 for launches of at most one 128-row workgroup per CU (1 x 64 heads x 512: 15.6 -> 15.0 us, 2 x 12 x 77:
+// 6.0 -> 5.2; with two workgroups per CU it loses: 1 x 32 x 2048 57.7 -> 70.2), KVS = 4, whose stages leave room for one workgroup on a CU, as long as that is all there are (3 x 6 x 333:
+// 8.9 -> 8.5 us, 1 x 8 x 512 8.9 -> 7.8, 1 x 4 x 2048 21.6 -> 16.3).
 template <bool BIAS, bool CAUSAL, int KVS>
 __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -358,9 +359,10 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
     }
   }
   float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-  if constexpr (KVS == 2) {
-    lds_float* const mine = (lds_float*)smem + qg * (34 * 64) + lane;  // the tiles are done with: every loop ends behind a barrier
+  if constexpr (KVS > 1) {
+    lds_float* const box_of = (lds_float*)smem + qg * (KVS - 1) * (34 * 64) + lane;  // the tiles are done with: every loop ends behind a barrier
     if (part) {
+      lds_float* const mine = box_of + (part - 1) * (34 * 64);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         mine[e * 64] = o[0][e];
@@ -371,15 +373,19 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
     }
     __syncthreads();
     if (part) return;
-    const float m2 = mine[32 * 64], l2 = mine[33 * 64];
-    const float m = fmaxf(m_run, m2), a1 = __builtin_amdgcn_exp2f(m_run - m), a2 = __builtin_amdgcn_exp2f(m2 - m);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      o[0][e] = o[0][e] * a1 + mine[e * 64] * a2;
-      o[1][e] = o[1][e] * a1 + mine[(16 + e) * 64] * a2;
+    for (int w = 0; w < KVS - 1; ++w) {
+      const lds_float* const his = box_of + w * (34 * 64);
+      const float m2 = his[32 * 64], l2 = his[33 * 64];
+      const float m = fmaxf(m_run, m2), a1 = __builtin_amdgcn_exp2f(m_run - m), a2 = __builtin_amdgcn_exp2f(m2 - m);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        o[0][e] = o[0][e] * a1 + his[e * 64] * a2;
+        o[1][e] = o[1][e] * a1 + his[(16 + e) * 64] * a2;
+      }
+      l_tot = l_tot * a1 + l2 * a2;
+      m_run = m;
     }
-    l_tot = l_tot * a1 + l2 * a2;
-    m_run = m;
   }
   const float inv = l_tot > 0.f ? 1.0f / l_tot : l_tot != l_tot ? l_tot : 0.f;
   const int q = q0 + l31;
@@ -473,7 +479,7 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
   }
 }
 
-// dQ (and the bucket sums of ds): 4 waves over the key tiles, 32 query rows each (KVS = 1) or two waves to 32 rows, every other tile each (KVS = 2), as in the forward
+// dQ (and the bucket sums of ds): 4 waves over the key tiles, 32 query rows each (KVS = 1), or two or four waves to 32 rows, a share of the tiles each, as in the forward
 template <bool BIAS, bool CAUSAL, int KVS>
 __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int tile_x, int hd, int b) {
   const AitkAttnRelposArgs& a = r.a;
@@ -628,9 +634,10 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       cur ^= 1;
     }
   }
-  if constexpr (KVS == 2) {
-    lds_float* const mine = (lds_float*)smem + qg * (37 * 64) + lane;  // the tiles are done with: every loop ends behind a barrier
+  if constexpr (KVS > 1) {
+    lds_float* const box_of = (lds_float*)smem + qg * (KVS - 1) * (37 * 64) + lane;  // the tiles are done with: every loop ends behind a barrier
     if (part) {
+      lds_float* const mine = box_of + (part - 1) * (37 * 64);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         mine[e * 64] = dq[0][e];
@@ -646,15 +653,19 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
     __syncthreads();
     if (!part) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        dq[0][e] += mine[e * 64];
-        dq[1][e] += mine[(16 + e) * 64];
+      for (int w = 0; w < KVS - 1; ++w) {
+        const lds_float* const his = box_of + w * (37 * 64);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          dq[0][e] += his[e * 64];
+          dq[1][e] += his[(16 + e) * 64];
+        }
+        row_ds += his[32 * 64];
+        fs_past += his[33 * 64];
+        fs_ahead += his[34 * 64];
+        fp_past += his[35 * 64];
+        fp_ahead += his[36 * 64];
       }
-      row_ds += mine[32 * 64];
-      fs_past += mine[33 * 64];
-      fs_ahead += mine[34 * 64];
-      fp_past += mine[35 * 64];
-      fp_ahead += mine[36 * 64];
     }
   }
   if (KVS == 1 || !part) store_row(a.dQ + ((long)b * S + qc) * a.lddq + hd * 64, dq, a.scale, h, live);
@@ -689,7 +700,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   }
 }
 
-// dK and dV: 4 waves over the query tiles, 32 keys each (KVS = 2: two waves to 32 keys).  S = Q K^T: a lane owns one key (column), its registers hold query rows, so the line of the bias runs backwards and
+// dK and dV: 4 waves over the query tiles, 32 keys each (KVS: waves to 32 keys).  S = Q K^T: a lane owns one key (column), its registers hold query rows, so the line of the bias runs backwards and
 // the row statistics come from LDS.  What a masked key computes stays in its own lane, which writes zeros.
 template <bool BIAS, bool CAUSAL, int KVS>
 __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int tile_x, int hd, int b) {
@@ -705,7 +716,7 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
   const bool inside = key < S;
   const bool kept = inside && (!a.key_mask || a.key_mask[(long)b * S + (inside ? key : 0)] != 0);
   f32x16_t dk[2] = {zero16(), zero16()}, dv[2] = {zero16(), zero16()};
-  const int ntiles = (S + 63) / 64, first_tile = CAUSAL ? tile_x * (ROWS / 64) : 0;
+  const int ntiles = (S + 63) / 64, first_tile = CAUSAL ? tile_x * ROWS / 64 : 0;
   if (__syncthreads_or(kept)) {  // a block of keys that are all masked has zero gradients
     const v4i_t srdQ = make_srd(a.Q + (long)b * S * a.ldq + hd * 64, ((long)(S - 1) * a.ldq + 64) * 2);
     const v4i_t srdG = make_srd(a.dO + (long)b * S * a.lddo + hd * 64, ((long)(S - 1) * a.lddo + 64) * 2);
@@ -803,9 +814,10 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
       dma_wait_all();
       __syncthreads();
     }
-    if constexpr (KVS == 2) {  // the tiles are done with
-      lds_float* const mine = (lds_float*)smem + wave / 2 * (64 * 64) + lane;
+    if constexpr (KVS > 1) {  // the tiles are done with
+      lds_float* const box_of = (lds_float*)smem + wave / KVS * (KVS - 1) * (64 * 64) + lane;
       if (part) {
+        lds_float* const mine = box_of + (part - 1) * (64 * 64);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
 #pragma unroll
@@ -818,17 +830,21 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
       __syncthreads();
       if (!part) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int w = 0; w < KVS - 1; ++w) {
+          const lds_float* const his = box_of + w * (64 * 64);
 #pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            dk[d][e] += mine[(16 * d + e) * 64];
-            dv[d][e] += mine[(32 + 16 * d + e) * 64];
+          for (int e = 0; e < 16; ++e) {
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              dk[d][e] += his[(16 * d + e) * 64];
+              dv[d][e] += his[(32 + 16 * d + e) * 64];
+            }
           }
         }
       }
     }
   }
-  if (KVS == 2 && part) return;
+  if (KVS > 1 && part) return;
   if (!kept) {  // a masked key's lane may hold anything
     dk[0] = dk[1] = dv[0] = dv[1] = zero16();
   }
@@ -925,26 +941,35 @@ int launch(K kernel, unsigned grid, size_t lds, const RelposArgs& r, hipStream_t
   return AITK_OK;
 }
 
-constexpr int64_t KVS2_MOST = 256;  // workgroups (one per CU) up to which two waves share their rows: of 128 rows in the forward, of 64 in the backward
+constexpr int64_t CUS = 256;       // launches of at most one workgroup per CU share rows between waves
+constexpr size_t LDS_MOST = 163840 - 256;  // of a CU, less what __syncthreads_or takes
+
+size_t fwd_lds(int kvs, const RelposArgs& r) { return (size_t)kvs * 4 * TILE + 512 + (size_t)4 * r.line_p * 4; }
 
 template <int KVS>
 int launch_fwd(const RelposArgs& r, hipStream_t s) {
   const AitkAttnRelposArgs& a = r.a;
   const unsigned grid = (unsigned)((a.S + 128 / KVS - 1) / (128 / KVS)) * a.H * a.B;
-  const size_t lds = KVS * 4 * TILE + 512 + (size_t)4 * r.line_p * 4;
+  const size_t lds = fwd_lds(KVS, r);
   if (a.table) return a.causal ? launch(attn_relpos_fwd_kernel<true, true, KVS>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<true, false, KVS>, grid, lds, r, s);
   return a.causal ? launch(attn_relpos_fwd_kernel<false, true, KVS>, grid, lds, r, s) : launch(attn_relpos_fwd_kernel<false, false, KVS>, grid, lds, r, s);
 }
 // The backward takes 64 rows per workgroup as long as every workgroup has a CU to itself (the doubled stages leave room for one; delta and dtable launches included, 64 / 128 rows: 16 heads x 512,
-// 256 workgroups of 64 rows, 22.7 / 30.3 us; 4 x 2048, 256 too, 42.5 / 61.4; 3 x 6 x 333 21.5 / 27.2; with 512 it takes two rounds: 32 x 512 38.6 / 30.6, 8 x 2048 78.8 / 62.2); one key tile
-// cannot be shared
-int bwd_kvs(int B, int H, int S) { return S > 64 && (int64_t)((S + 63) / 64) * H * B * 2 <= KVS2_MOST ? 2 : 1; }
+// 256 workgroups of 64 rows, 21 / 28 us; 4 x 2048, 256 too, 40 / 58; 3 x 6 x 333 20 / 26; with 512 it takes two rounds: 32 x 512 38.6 / 30.6, 8 x 2048 78.8 / 62.2); one key tile cannot be shared.
+// 32 rows and four waves to them where that holds again, from three key tiles on (8 x 512 20.6 -> 18.2 us, 1 x 2048 39 -> 29), unless many distances (max_distance above 256) take the LDS.
+int bwd_kvs(int B, int H, int S, bool lds4) {
+  if (S > 128 && lds4 && (int64_t)((S + 31) / 32) * H * B * 2 <= CUS) return 4;
+  return S > 64 && (int64_t)((S + 63) / 64) * H * B * 2 <= CUS ? 2 : 1;
+}
+size_t bwd_lds(int kvs, const RelposArgs& r) {
+  return (size_t)kvs * (4 * TILE + 1024) + (size_t)4 * r.line_p * 4 + (r.a.dtable ? ((size_t)4 * (2 * (r.sat + BAND_PAD) + 1) + 3 + 4 * 8 * SKEW_P) * 4 : 0);
+}
 
 template <int KVS>
 int launch_bwd(const RelposArgs& r, hipStream_t s) {
   const AitkAttnRelposArgs& a = r.a;
   const unsigned grid = (unsigned)r.tiles * a.H * a.B * 2;
-  const size_t lds = KVS * (4 * TILE + 1024) + (size_t)4 * r.line_p * 4 + (a.dtable ? ((size_t)4 * (2 * (r.sat + BAND_PAD) + 1) + 3 + 4 * 8 * SKEW_P) * 4 : 0);
+  const size_t lds = bwd_lds(KVS, r);
   if (a.table) return a.causal ? launch(attn_relpos_bwd_kernel<true, true, KVS>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<true, false, KVS>, grid, lds, r, s);
   return a.causal ? launch(attn_relpos_bwd_kernel<false, true, KVS>, grid, lds, r, s) : launch(attn_relpos_bwd_kernel<false, false, KVS>, grid, lds, r, s);
 }
@@ -964,12 +989,14 @@ extern "C" int aitk_attn_relpos_fwd(const AitkAttnRelposArgs* a, aitk_stream_t s
   const int rc = check(a, false, r);
   if (rc != AITK_OK) return rc;
   hipStream_t s = (hipStream_t)stream;
-  return (int64_t)((a->S + 127) / 128) * a->H * a->B <= KVS2_MOST ? launch_fwd<2>(r, s) : launch_fwd<1>(r, s);
+  const int64_t heads = (int64_t)a->H * a->B;
+  if (a->S > 128 && (a->S + 31) / 32 * heads <= CUS && fwd_lds(4, r) <= LDS_MOST) return launch_fwd<4>(r, s);
+  return (a->S + 127) / 128 * heads <= CUS ? launch_fwd<2>(r, s) : launch_fwd<1>(r, s);
 }
 
 extern "C" int64_t aitk_attn_relpos_bwd_workspace_bytes(int32_t B, int32_t H, int32_t S, int32_t num_buckets) {
   if (B <= 0 || H <= 0 || S <= 0 || num_buckets < 0) return 0;
-  const int rows = 128 / bwd_kvs(B, H, S);
+  const int rows = 128 / bwd_kvs(B, H, S, true);  // the most that a call can need: whether four waves share their rows follows from its buckets too
   return ((int64_t)2 * B * H * S + (int64_t)B * ((S + rows - 1) / rows) * H * num_buckets) * 4;
 }
 
@@ -977,14 +1004,14 @@ extern "C" int aitk_attn_relpos_bwd(const AitkAttnRelposArgs* a, aitk_stream_t s
   RelposArgs r;
   int rc = check(a, true, r);
   if (rc != AITK_OK) return rc;
-  const int kvs = bwd_kvs(a->B, a->H, a->S), rows = 128 / kvs;
+  const int kvs = bwd_kvs(a->B, a->H, a->S, bwd_lds(4, r) <= LDS_MOST), rows = 128 / kvs;
   r.tiles = (a->S + rows - 1) / rows;
   r.delta = a->ws;
   r.part = a->ws + (int64_t)2 * a->B * a->H * a->S;
   hipStream_t s = (hipStream_t)stream;
   hipLaunchKernelGGL(attn_relpos_delta_kernel, dim3((a->S + 31) / 32, a->H, a->B), dim3(256), 0, s, r);
   AITK_LAUNCH_CHECK();
-  rc = kvs == 2 ? launch_bwd<2>(r, s) : launch_bwd<1>(r, s);
+  rc = kvs == 4 ? launch_bwd<4>(r, s) : kvs == 2 ? launch_bwd<2>(r, s) : launch_bwd<1>(r, s);
   if (rc != AITK_OK) return rc;
   if (a->dtable) {
     hipLaunchKernelGGL(attn_relpos_dtable_kernel, dim3((a->H * a->num_buckets + 255) / 256), dim3(256), 0, s, r);

@@ -189,7 +189,7 @@ def test_more_than_one_group_of_key_tiles(mask):
 
 
 @pytest.mark.parametrize("mask", [None, "late", "holes"])
-def test_more_than_one_group_of_key_tiles_shared_by_two_waves(mask):
+def test_more_than_one_group_of_key_tiles_shared_by_waves(mask):
     _run(1, 1, 4200, mask=mask, seed=4)
 
 
@@ -199,6 +199,14 @@ def test_more_than_one_group_of_key_tiles_shared_by_two_waves(mask):
 def test_more_workgroups_than_compute_units(S, kind, bias, causal):
     """128 rows to a workgroup in the backward and from S = 130 on in the forward (smaller launches share their rows between two waves)"""
     _run(3, 32, S, mask=kind, bias=bias, causal=causal, poison=kind is not None, seed=S)
+
+
+@pytest.mark.parametrize("B,H,S", [(4, 8, 130), (4, 8, 200), (2, 8, 333)])
+@pytest.mark.parametrize("kind", [None, "prefix", "holes", "tail"])
+@pytest.mark.parametrize("bias,causal", [(True, False), (True, True), (False, True)])
+def test_two_waves_to_a_block_of_rows(B, H, S, kind, bias, causal):
+    """between the launches that give four waves to 32 rows (the smaller ones here) and those that give one"""
+    _run(B, H, S, mask=kind, bias=bias, causal=causal, poison=kind is not None, seed=S)
 
 
 def test_large_encoder_shape():
