@@ -398,10 +398,11 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
 // o has been rounded to bf16, so delta is off by up to 2^-8 |dO||o|, and ds = p (dp - delta) by p times that.  Over many keys that is small next to the rounding of ds; over a few, |o| is as large
 // as |v|, dp - delta may be small, and the gradients of two keys were off by 2 % in the worst of a few heads.  Samples of 2 to FEW keys therefore get delta as the sum of p dp (of one key
 // o = v needs no rounding).
-constexpr int FEW = 16;
+constexpr int FEW = 16;  // x 8 chunks x K and V: a load for every thread
 __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
   __shared__ int keys[FEW];
   __shared__ float bias[32][FEW + 1];
+  __shared__ uint4 rows[2][FEW][8];  // the kept keys' K and V
   const AitkAttnRelposArgs& a = r.a;
   const int tid = threadIdx.x, lane = tid & 63, S = a.S, s0 = blockIdx.x * 32, s = min(s0 + (tid >> 3), S - 1), hd = blockIdx.y, b = blockIdx.z, c = (tid & 7) * 8;
   const long row = (long)b * S + s, i = ((long)b * a.H + hd) * S + s;
@@ -429,8 +430,14 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
         if ((bits >> lane) & 1) keys[at + __popcll(bits & ((1ull << lane) - 1))] = k0 + lane;
         at += __popcll(bits);
       }
+    const uint4 qv = *reinterpret_cast<const uint4*>(a.Q + row * a.ldq + hd * 64 + c);
     __syncthreads();
-    if (a.table) {
+    const int key = (tid >> 3) & (FEW - 1);
+    if (key < n) {
+      const long at = (long)b * S + keys[key];
+      rows[tid >> 7][key][tid & 7] = *reinterpret_cast<const uint4*>((tid >> 7 ? a.V + at * a.ldv : a.K + at * a.ldk) + hd * 64 + c);
+    }
+    if (a.table)
       for (int p = tid; p < 32 * n; p += 256) {
         const int q = p / n, d = keys[p - q * n] - (s0 + q), m = d > 0 ? (a.causal ? 0 : d) : -d;
         int lo = 0, hi = r.half;  // the last bucket whose first distance is at most m
@@ -441,36 +448,12 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
         }
         bias[q][p - q * n] = bf2f(a.table[(long)(lo + (d > 0 && !a.causal ? r.half : 0)) * a.H + hd]) * 1.4426950408889634f;
       }
-      __syncthreads();
-    }
-    const uint4 qv = *reinterpret_cast<const uint4*>(a.Q + row * a.ldq + hd * 64 + c);
+    __syncthreads();
     v = 0.f;
-    constexpr int U = 2;  // keys in flight
-    for (int k0 = 0; k0 < n; k0 += U) {
-      float sc[U], dp[U];
-      uint4 kv[U], vv[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const long kr = (long)b * S + keys[min(k0 + u, n - 1)];
-        kv[u] = *reinterpret_cast<const uint4*>(a.K + kr * a.ldk + hd * 64 + c);
-        vv[u] = *reinterpret_cast<const uint4*>(a.V + kr * a.ldv + hd * 64 + c);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        sc[u] = dot(qv, kv[u]);
-        dp[u] = dot(y, vv[u]);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-          sc[u] += __shfl_xor(sc[u], o, 64);
-          dp[u] += __shfl_xor(dp[u], o, 64);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = min(k0 + u, n - 1);
-        const float x2 = fmaf(sc[u], a.scale * 1.4426950408889634f, a.table ? bias[tid >> 3][k] : 0.f);
-        if (k0 + u < n && lse != -INFINITY && !(a.causal && keys[k] > s)) v += __builtin_amdgcn_exp2f(x2 - lse) * dp[u];
-      }
+    for (int k = 0; k < n; ++k) {
+      const float sc = sum8(dot(qv, rows[0][k][tid & 7])), dp = sum8(dot(y, rows[1][k][tid & 7]));
+      const float x2 = fmaf(sc, a.scale * 1.4426950408889634f, a.table ? bias[tid >> 3][k] : 0.f);
+      if (lse != -INFINITY && !(a.causal && keys[k] > s)) v += __builtin_amdgcn_exp2f(x2 - lse) * dp;
     }
   }
   if (c == 0 && s0 + (tid >> 3) < S) {
@@ -691,8 +674,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       const int n0 = ahead && j == 0 ? 1 : r.first[j], n1 = last ? E + 1 : r.first[j + 1];
       float v = 0.f;
       for (int n = n0 + (i & 7); n < n1; n += 8) v += all[E + (ahead ? n : -n)];
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+      v = sum8(v);
       const int f = ahead ? 4 : 0;
       if (last) v += (fars[f] + fars[f + 1]) + (fars[f + 2] + fars[f + 3]);
       if ((i & 7) == 0) r.part[(((long)b * r.tiles + tile_x) * a.H + hd) * a.num_buckets + bucket] = v;

@@ -63,6 +63,14 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// v plus the value of the lane that DPP control `CTRL` names
+template <int CTRL>
+__device__ __forceinline__ float plus_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// sum over 8 neighbouring lanes, in every one of them: neighbours, pairs, mirrored quads
+__device__ __forceinline__ float sum8(float v) { return plus_dpp<0x141>(plus_dpp<0x4E>(plus_dpp<0xB1>(v))); }
+
 // tanh-approximate GELU, torch.nn.functional.gelu(approximate="tanh"):  0.5 x (1 + tanh(u)),  u = k0 (x + k1 x^3).
 // Written through the logistic function (tanh(u) = 2 sigmoid(2u) - 1) so it costs one v_exp_f32 + one v_rcp_f32 instead
 // of libm tanhf (~60 instructions): the GELU / dGELU GEMM epilogues were spending ~50 us per 256x256 tile round on it.

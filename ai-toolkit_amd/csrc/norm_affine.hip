@@ -36,11 +36,6 @@ __device__ __forceinline__ void load_w8(const void* w, int f32, int c, float* f)
   }
 }
 
-// v plus the value of the lane that DPP control `CTRL` names
-template <int CTRL>
-__device__ __forceinline__ float plus_dpp(float v) {
-  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
-}
 // v plus the value of the neighbouring row of 16 lanes (of the other half of the wave)
 template <int ROWS>
 __device__ __forceinline__ float plus_swapped(float v) {
