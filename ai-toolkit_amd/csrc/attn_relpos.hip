@@ -397,9 +397,10 @@ __global__ __launch_bounds__(256, 2) void attn_relpos_fwd_kernel(RelposArgs r) {
 // ============================================================================================ backward
 // Minus delta[q] = dO[q].o[q], and minus the row statistic, -inf for rows without a key (2^(s - inf) = 0: their probabilities vanish).  A wave takes 8 rows of one head.
 // o has been rounded to bf16, so delta is off by up to 2^-8 |dO||o|, and ds = p (dp - delta) by p times that.  Over many keys that is small next to the rounding of ds; over a few, |o| is as large
-// as |v|, dp - delta may be small, and the gradients of two keys were off by 2 % in the worst of a few heads.  Samples of 2 to FEW keys therefore get delta as the sum of p dp (of one key
-// o = v needs no rounding).
-constexpr int FEW = 16;  // x 8 chunks x K and V: a load for every thread
+// as |v|, dp - delta may be small, and the gradients of two keys were off by 2 % in the worst of a few heads.  Samples of 2 to FEW keys therefore get delta as the sum of p dp.  With a
+// single key ds is zero whatever it holds: such samples are marked, and both roles leave it out.
+constexpr int FEW = 16;                      // x 8 chunks x K and V: a load for every thread
+constexpr unsigned ONE_KEY = 0xffffffffu;  // in the place of -delta (a NaN that no arithmetic gives)
 __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
   __shared__ int keys[FEW];
   __shared__ float bias[32][FEW + 1];
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(256) void attn_relpos_delta_kernel(RelposArgs r) {
     }
   }
   if (c == 0 && s0 + (tid >> 3) < S) {
-    r.delta[i] = -v;
+    r.delta[i] = n == 1 ? __builtin_bit_cast(float, ONE_KEY) : -v;
     r.delta[(long)a.B * a.H * S + i] = lse == -INFINITY ? -INFINITY : -lse;
   }
 }
@@ -493,6 +494,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   }
   const long stat = ((long)b * a.H + hd) * S + qc;
   const float delta = -r.delta[stat];
+  const bool one_key = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(unsigned, r.delta[stat])) == ONE_KEY;  // of the sample: the same in every wave
   const float l2 = live ? -r.delta[(long)a.B * a.H * S + stat] : INFINITY;  // rows past the end: p = 0, ds = 0
   const float c2 = a.scale * 1.4426950408889634f;
   const int E = r.sat + BAND_PAD, n_line = 2 * E + 1;
@@ -509,7 +511,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
   float far_past = 0.f, far_ahead = 0.f, fs_past = 0.f, fs_ahead = 0.f, fp_past = 0.f, fp_ahead = 0.f, row_ds = 0.f;
   const int ib = E + 4 * h - q0 - l31;
   f32x16_t dq[2] = {zero16(), zero16()};
-  const int ntiles = CAUSAL ? min((S + 63) / 64, (tile_x * ROWS + ROWS - 1) / 64 + 1) : (S + 63) / 64;
+  const int ntiles = one_key ? 0 : CAUSAL ? min((S + 63) / 64, (tile_x * ROWS + ROWS - 1) / 64 + 1) : (S + 63) / 64;
   for (int t0 = 0; t0 < ntiles; t0 += 64) {
     const unsigned long long masks = tile_masks(a, b, t0, ntiles, box, lane, wave);
     unsigned long long todo = __ballot(masks != 0);
@@ -653,7 +655,10 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
     }
   }
   if (KVS == 1 || !part) store_row(a.dQ + ((long)b * S + qc) * a.lddq + hd * 64, dq, a.scale, h, live);
-  if (sums) {
+  float* const bucket_sums = r.part + (((long)b * r.tiles + tile_x) * a.H + hd) * a.num_buckets;
+  if (sums && one_key) {
+    for (int i = tid; i < a.num_buckets; i += 256) bucket_sums[i] = 0.f;
+  } else if (sums) {
     lds_float* const fars = (lds_float*)box;  // the tile masks are done with
     row_ds += __shfl_xor(row_ds, 32, 64);  // the row's two lanes
     fs_past = wave_sum(fs_past - row_ds * fp_past);
@@ -678,7 +683,7 @@ __device__ __forceinline__ void dq_role(const RelposArgs& r, char* smem, int til
       v = sum8(v);
       const int f = ahead ? 4 : 0;
       if (last) v += (fars[f] + fars[f + 1]) + (fars[f + 2] + fars[f + 3]);
-      if ((i & 7) == 0) r.part[(((long)b * r.tiles + tile_x) * a.H + hd) * a.num_buckets + bucket] = v;
+      if ((i & 7) == 0) bucket_sums[bucket] = v;
     }
   }
 }
@@ -831,6 +836,7 @@ __device__ __forceinline__ void dkv_role(const RelposArgs& r, char* smem, int ti
   if (!kept) {  // a masked key's lane may hold anything
     dk[0] = dk[1] = dv[0] = dv[1] = zero16();
   }
+  if (__builtin_bit_cast(unsigned, r.delta[((long)b * a.H + hd) * S]) == ONE_KEY) dk[0] = dk[1] = zero16();
   const long row = (long)b * S + (inside ? key : 0);
   store_row(a.dK + row * a.lddk + hd * 64, dk, a.scale, h, inside);
   store_row(a.dV + row * a.lddv + hd * 64, dv, 1.0f, h, inside);

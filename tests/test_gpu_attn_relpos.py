@@ -144,6 +144,34 @@ def test_few_keys_have_exact_deltas(S, keys, causal, bias):
             assert ((dtable.double() - want["dtable"]).abs() <= want["tol_dtable"] * (1 + ref.U) + 1e-30).all(), seed
 
 
+@pytest.mark.parametrize("causal,bias", [(False, True), (True, True), (False, False)])
+@pytest.mark.parametrize("S", [1, 2, 40, 200, 1300])
+@pytest.mark.parametrize("B,H", [(1, 1), (3, 4), (2, 64)])
+def test_a_single_key_has_zero_gradients_but_for_its_value(B, H, S, causal, bias):
+    """p = 1 whatever the scores are: dq, dk and dtable are exactly zero, dv is the sum of dO.  One sample keeps no key, where there is more than one"""
+    from ai_toolkit_amd import ops
+
+    q, k, v, table, o, do, dq, dk, dv = _inputs(B, H, S, seed=S)
+    for t in (dq, dk, dv):
+        t.fill_(5.0)
+    table = table if bias else None
+    mask = None
+    if S > 1:
+        mask = torch.zeros(B, S, dtype=torch.bool, device="cuda")
+        for b in range(B - (B > 1)):
+            mask[b, (7 * b + 1) % S] = True
+    kw = dict(B=B, H=H, S=S, scale=1.0, key_mask=mask, max_distance=128, causal=causal)
+    want = ref.attention(q, k, v, table, do=do, **kw)
+    lse = torch.zeros(B, H, S, device="cuda")
+    ops.attn_relpos_fwd(q, k, v, table, o, lse, **kw)
+    dtable = torch.full((32, H), 5.0, device="cuda") if bias else None
+    ops.attn_relpos_bwd(q, k, v, table, o, lse, do, dq, dk, dv, dtable, **kw)
+    torch.cuda.synchronize()
+    _near(o, want["o"], want["tol_o"], "o")
+    assert ((dv.double() - want["dv"]).abs() <= want["tol_dv"] + 1e-30).all()
+    assert (dq == 0).all() and (dk == 0).all() and (dtable is None or (dtable == 0).all())
+
+
 @pytest.mark.parametrize("value", [float("-inf"), torch.finfo(BF16).min])
 @pytest.mark.parametrize("S", [64, 200, 333])
 def test_table_entries_that_forbid_a_bucket(value, S):
