@@ -14,7 +14,7 @@
 //
 // Measured: 2048 x 4096 x 10240 forward with hg 325 us = 1.06 PFLOP/s, all three gradients 600 - 720 us = 1.15 - 0.95 PFLOP/s as the card's power allows (the library's plain products of these
 // sizes: 371 and about 650 us), du 32 us = 6.5 TB/s (half of it still cached); 512 x 4096 x 10240 forward 92 - 102 us = 0.93 - 0.84 PFLOP/s on 160 of the 256 CUs; 4096 x 640 x 2560 forward with
-// hg and biases 50 us, all gradients 106 us; 1 x 4096 x 10240 32 us = 5.2 TB/s of weights.  The tile loop is bound by the power of the matrix units: 0.53 us (160 CUs) to 0.63 us (256) a stage of a
+// hg and biases 50 us, all gradients 102 us; 1 x 4096 x 10240 32 us = 5.2 TB/s of weights.  The tile loop is bound by the power of the matrix units: 0.53 us (160 CUs) to 0.63 us (256) a stage of a
 // 256 x 256 tile with nothing but its matrix instructions, 0.66 to 0.82 as it is.
 #include "common.h"
 #include "aitk_args.h"
@@ -41,7 +41,10 @@ struct FfnArgs {
   const bf16_t* bg;
   bf16_t* hg;  // [M, 2F] = [u | z], may be NULL
   long ld_hg;
-  int act, _pad;
+  int act;
+  int sum_rows, sum_cols;  // backward with bias gradients: [sum_rows][2][sum_cols] partial column sums of du and dz
+  const float* sums;
+  bf16_t* db[2];  // where they go; either may be NULL
 };
 
 // The normal distribution's Phi(z), and e = exp(-z^2 / 2), for the erf GELU: Phi(-x) = e P(1 / (1 + x / 4)) for x >= 0, where P is a polynomial of degree 7 fitted here to
@@ -490,7 +493,7 @@ __device__ __forceinline__ void grad_tile(const Prod& p, int ti, int tj, int pie
   }
 }
 
-// dx and the two weight gradients in one launch.  dx contracts over 2 F and has few tiles, the weights contract over M and have many: pieces of a product's contraction
+// dx, the two weight gradients and the last step of the bias gradients in one launch.  dx contracts over 2 F and has few tiles, the weights contract over M and have many: pieces of a product's contraction
 // (plan() below) make the workgroups alike; the longest go first.
 template <int BM, int BN, int WR, int WC>
 __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_grads_kernel(FfnArgs a) {
@@ -510,6 +513,22 @@ __global__ __launch_bounds__(WR * WC * 64) void gated_ffn_grads_kernel(FfnArgs a
     if (p.a_rows) grad_tile<BM, BN, WR, WC, false>(p, ti, tj, piece, smem);
     else grad_tile<BM, BN, WR, WC, true>(p, ti, tj, piece, smem);
     return;
+  }
+  // the workgroups behind the tiles: 64 columns of a bias gradient each, the waves' shares of the partial rows joined in a fixed order
+  constexpr int SL = WR * WC;
+  const int nb = (a.sum_cols + 63) / 64, v = id / nb, l = threadIdx.x & 63, sl = threadIdx.x >> 6, c = (id - v * nb) * 64 + l;
+  float* const box = reinterpret_cast<float*>(smem);
+  float s = 0.f;
+  if (c < a.sum_cols && a.db[v]) {
+#pragma unroll 8
+    for (int k = sl; k < a.sum_rows; k += SL) s += a.sums[((long)k * 2 + v) * a.sum_cols + c];
+  }
+  box[sl * 64 + l] = s;
+  __syncthreads();
+  if (sl == 0 && c < a.sum_cols && a.db[v]) {
+#pragma unroll
+    for (int k = 1; k < SL; ++k) s += box[k * 64 + l];
+    a.db[v][c] = f2bf(s);
   }
 }
 // the pieces' fp32 sums, in their order, rounded once: 8 columns per thread
@@ -590,21 +609,6 @@ __global__ __launch_bounds__(256) void gated_ffn_du_kernel(const bf16_t* dh, lon
     }
   }
 }
-// column sums of the workgroups' partials: 64 columns x 4 slices of the workgroups, joined in a fixed order
-__global__ __launch_bounds__(256) void gated_ffn_db_kernel(const float* part, int nchunk, int F, bf16_t* dbv, bf16_t* dbg) {
-  __shared__ float box[4][64];
-  const int l = threadIdx.x & 63, sl = threadIdx.x >> 6, c = blockIdx.x * 64 + l, v = blockIdx.y;
-  bf16_t* out = v ? dbg : dbv;
-  float s = 0.f;
-  if (c < F && out) {
-#pragma unroll 8
-    for (int k = sl; k < nchunk; k += 4) s += part[((long)k * 2 + v) * F + c];
-  }
-  box[sl][l] = s;
-  __syncthreads();
-  if (sl == 0 && c < F && out) out[c] = f2bf(box[0][l] + box[1][l] + box[2][l] + box[3][l]);
-}
-
 bool mis16(const void* q) { return ((uintptr_t)q & 15) != 0; }
 bool bad(const void* p, int64_t ld, int64_t width) { return mis16(p) || (ld % 8) || ld < width || ld > (1 << 20); }
 
@@ -750,10 +754,6 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
   if (db) hipLaunchKernelGGL(gated_ffn_du_kernel<true>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, rows, part);
   else hipLaunchKernelGGL(gated_ffn_du_kernel<false>, grid, dim3(256), 0, s, q->dh, (long)q->ld_dh, q->hg, (long)q->ld_hg, du, M, F, q->act, rows, part);
   AITK_LAUNCH_CHECK();
-  if (db) {
-    hipLaunchKernelGGL(gated_ffn_db_kernel, dim3((F + 63) / 64, 2), dim3(256), 0, s, part, nchunk, F, q->db_val, q->db_gate);
-    AITK_LAUNCH_CHECK();
-  }
   FfnArgs a = {};
   const auto partial = [&](int i) { return pl.split[i] > 1 ? reinterpret_cast<float*>(ws + l.part[i]) : nullptr; };
   const Prod x = {{du, du + F}, {q->w_val, q->w_gate}, q->dx, 2 * (long)F, q->ldw, q->ld_dx, partial(0), q->dx ? M : 0, K, F, 2, pl.split[0], 0};
@@ -764,6 +764,14 @@ extern "C" int aitk_gated_ffn_bwd(const AitkGatedFfnBwdArgs* q, aitk_stream_t st
   a.p[dx_first ? 1 : 0] = wv;
   a.p[dx_first ? 2 : 1] = wg;
   int64_t n = 0, joined = 0;
+  if (db) {
+    a.sum_rows = nchunk;
+    a.sum_cols = F;
+    a.sums = part;
+    a.db[0] = q->db_val;
+    a.db[1] = q->db_gate;
+    n = 2 * ((F + 63) / 64);
+  }
   const int b = pl.big ? 256 : 128;
   for (const Prod& p : a.p) {
     n += tiles(p.M, p.N, b, b) * p.split;
